@@ -4,15 +4,20 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libyolact_post.so")
-SOURCES = ["api.hip", "score_filter.hip", "nms.hip", "mask.hip", "priors.hip", "rle.hip", "loss_grad.hip"]
-HEADERS = ["common.hpp", os.path.join("..", "..", "include", "yolact_post.h")]
+SOURCES = ["api.hip", "score_filter.hip", "nms.hip", "mask.hip", "priors.hip", "rle.hip", "loss_grad.hip",
+           "class_loss.hip", "quantized.hip", "dropout.hip"]
+HEADERS = ["common.hpp", "gemm_tile.hpp", "gemm_launch.hpp", os.path.join("..", "..", "include", "yolact_post.h")]
 # -ffp-contract=off: YP-MATH writes every fma explicitly.
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off",
-         "-fno-fast-math", "-Wall", "-Wno-unused-function"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
+         "-fno-fast-math", "-Wall", "-Wno-unused-function",
+         # no packed f32 instructions: the compiler must not form them (the host pass warns that it has no such feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def needs_build() -> bool:
@@ -29,10 +34,16 @@ def build_lib(force: bool = False, verbose: bool = False, extra_flags=(), out: s
         return LIB_PATH
     out = out or LIB_PATH
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc] + FLAGS + list(extra_flags) + [os.path.join(CSRC, s) for s in SOURCES] + ["-o", out]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    subprocess.check_call(cmd)
+    # one object per source, in parallel, in a folder of this build's own; then one link
+    with tempfile.TemporaryDirectory(prefix="yp_build_") as tmp:
+        objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        cmds = [[hipcc] + FLAGS + list(extra_flags) + ["-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objs)]
+        link = [hipcc, "--offload-arch=gfx950", "-fPIC", "-shared"] + objs + ["-o", out]
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds + [link]), file=sys.stderr)
+        with ThreadPoolExecutor(max_workers=min(8, int(os.environ.get("MAX_JOBS", "8")))) as pool:
+            list(pool.map(subprocess.check_call, cmds))
+        subprocess.check_call(link)
     return out
 
 
