@@ -283,6 +283,62 @@ int yp_rle_string(const uint32_t* counts, int32_t n, char* out, int32_t cap);
 int64_t yp_rle_strings(const uint32_t* counts, const int64_t* starts, const int32_t* lens, int32_t n_lists,
                        int64_t n_counts, char* out, int64_t out_cap, int64_t* offsets);
 
+/* ---- operators of the prediction head ----
+ * What produces Detect's inputs and what trains it, for class sets up to large vocabularies.  No counterpart in the
+ * reference's Python code beyond Keras layers (layers/head.py) and tf.nn.softmax_cross_entropy in its loss.
+ * Element types: */
+enum { YP_F32 = 0, YP_BF16 = 1, YP_F16 = 2, YP_INT8 = 3 };
+
+/* Class loss: softmax cross entropy of features [n,d] against a class matrix weight [v,d] and bias [v] (may be NULL), the
+ * logits z = features weight^T + bias never stored:   lse[i] = log sum_c exp z[i,c]   losses[i] = lse[i] - z[i,labels[i]]
+ *   dtype        YP_F32, YP_BF16 or YP_F16: features, weight, bias and their gradients
+ *   labels [n]   int32 or int64 (label_bytes 4 or 8).  A row whose label is ignore_index takes no part: loss 0, no
+ *                gradient, whatever its features hold (NaN included).  Any other label outside [0, v): loss NaN, no
+ *                gradient, counted.
+ *   bias         a class whose bias is -inf takes no part: probability 0, no gradient, whatever its weights hold; as a
+ *                label its loss is +inf.
+ *   losses, lse  [n] float32          reduced [3] float32, may be NULL: the rows' sum, their mean over the rows that are
+ *                not ignored (0 without one), and how many those are
+ *   workspace    yp_class_loss_workspace(n, v, d, dtype, has_bias, backward) bytes, 256-byte aligned
+ * The backward pass takes the forward's inputs and its lse, and grad = dL/dlosses: [n] float32 (grad_stride 1) or one
+ * value for every row (grad_stride 0); with count != NULL the values are divided by max(*count, 1) (the mean: pass
+ * reduced + 2).  grad_bias is NULL without a bias.  Products accumulate in float32, gradients are rounded once; dz =
+ * grad (softmax - onehot) is rounded to dtype before its products.  Fixed order of sums, no float atomics.
+ * 0 <= n <= 2^20, 1 <= v <= 2^24, 1 <= d <= 65536; contiguous tensors, aligned to their elements.  All pointers on the
+ * device; asynchronous on hip_stream; allocates nothing, may be captured. */
+int64_t yp_class_loss_workspace(int32_t n, int32_t v, int32_t d, int32_t dtype, int32_t has_bias, int32_t backward);
+int yp_class_loss(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
+                  const void* bias, const void* labels, int32_t label_bytes, int64_t ignore_index, void* workspace,
+                  float* losses, float* lse, float* reduced, void* hip_stream);
+int yp_class_loss_backward(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
+                           const void* bias, const void* labels, int32_t label_bytes, int64_t ignore_index, const float* lse,
+                           const float* grad, int32_t grad_stride, const float* count, void* workspace,
+                           void* grad_features, void* grad_weight, void* grad_bias, void* hip_stream);
+
+/* Matrix product in 8-bit integers, one scale per row of x (token) and per row of the weight (channel):
+ *   scale[r] = max_k |x[r,k]| / 127     q[r,k] = x[r,k] / scale[r] to the nearest integer, ties to even (0 for a row of
+ *   zeros)                              out[i,j] = (sum_k xq[i,k] wq[j,k]) x_scale[i] w_scale[j] + bias[j]
+ * q rows are yp_quantized_row_bytes(k) bytes apart (k padded to 128), the padding is zero; 16-byte aligned.  A row that
+ * holds an infinity or NaN gets the scale NaN, so its results are NaN.  1 <= k <= 131072 (the integer sums fit 32 bits).
+ *   yp_quantize_rows     x [rows,k] contiguous, dtype YP_F32 / YP_BF16 / YP_F16 -> q, scale [rows] float32
+ *   yp_quantized_linear  x: dtype YP_INT8 (x = q rows, x_scale their scales) or a float type, x [rows,k] contiguous,
+ *                        quantized on the way into workspace (yp_quantized_linear_workspace(rows, k) bytes, 256-byte
+ *                        aligned; x_scale NULL).  bias [v] float32 or NULL.  out [rows,v] of out_dtype, one rounding.
+ * Asynchronous on hip_stream; allocates nothing, may be captured. */
+int64_t yp_quantized_row_bytes(int32_t k);
+int64_t yp_quantized_linear_workspace(int32_t rows, int32_t k);
+int yp_quantize_rows(int32_t device_id, int32_t rows, int32_t k, int32_t dtype, const void* x, void* q, float* scale, void* hip_stream);
+int yp_quantized_linear(int32_t device_id, int32_t rows, int32_t v, int32_t k, int32_t dtype, const void* x, const float* x_scale,
+                        const void* wq, const float* w_scale, const float* bias, void* workspace, void* out, int32_t out_dtype,
+                        void* hip_stream);
+
+/* Dropout whose mask is never stored: element i of x (count elements, contiguous) is kept if word i % 4 of
+ * Philox4x32-10 (Salmon et al. 2011) under the 64-bit key state[0] at the 64-bit counter state[1] + i / 4 is
+ * >= floor(p 2^32), and then y = x / (1 - p); otherwise y = 0, whatever x holds.  0 <= p <= 1.  The backward pass is the
+ * same call on the gradient with the same state.  state [2] int64 on the device: a captured call reads it on every
+ * replay; advance state[1] by (count + 3) / 4 between uses.  y may be x.  Asynchronous on hip_stream. */
+int yp_dropout(int32_t device_id, int64_t count, int32_t dtype, double p, const int64_t* state, const void* x, void* y, void* hip_stream);
+
 /* Bytes of device scratch the handle holds. */
 int64_t yp_scratch_bytes(const yp_handle* h);
 

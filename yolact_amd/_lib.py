@@ -17,6 +17,7 @@ YP_NMS_PER_CLASS = 1
 YP_RESIZE_THEN_THRESHOLD = 0
 YP_THRESHOLD_THEN_RESIZE = 1
 YP_NUM_KERNELS = 3
+YP_F32, YP_BF16, YP_F16, YP_INT8 = 0, 1, 2, 3
 YP_STATIC_SCRATCH_BYTES = 64 << 20
 KERNEL_NAMES = ("score_filter", "nms", "mask_assemble")
 
@@ -25,7 +26,9 @@ EXPORTS = ("yp_create", "yp_destroy", "yp_run", "yp_sync", "yp_last_survivors", 
            "yp_profile_read", "yp_scratch_bytes", "yp_last_error", "yp_version", "yp_make_priors", "yp_run_static",
            "yp_masks_to_rle", "yp_rle_string", "yp_rle_strings", "yp_assemble_masks", "yp_assemble_masks_backward",
            "yp_assemble_masks_backward_workspace", "yp_create_bounded", "yp_overflowed", "yp_masks_to_rle_sized",
-           "yp_kept_create", "yp_kept_destroy", "yp_kept_reset", "yp_run_kept")
+           "yp_kept_create", "yp_kept_destroy", "yp_kept_reset", "yp_run_kept",
+           "yp_class_loss", "yp_class_loss_backward", "yp_class_loss_workspace", "yp_quantized_row_bytes",
+           "yp_quantized_linear_workspace", "yp_quantize_rows", "yp_quantized_linear", "yp_dropout")
 
 
 class YpConfig(ctypes.Structure):
@@ -111,6 +114,23 @@ def load():
     L.yp_create_bounded.argtypes = [vp, ctypes.c_int32, vp]
     L.yp_overflowed.restype = ctypes.c_int
     L.yp_overflowed.argtypes = [vp]
+    i32, i64 = ctypes.c_int32, ctypes.c_int64
+    L.yp_class_loss_workspace.restype = i64
+    L.yp_class_loss_workspace.argtypes = [i32] * 6
+    L.yp_class_loss.restype = ctypes.c_int
+    L.yp_class_loss.argtypes = [i32] * 5 + [vp] * 4 + [i32, i64] + [vp] * 4 + [vp]
+    L.yp_class_loss_backward.restype = ctypes.c_int
+    L.yp_class_loss_backward.argtypes = [i32] * 5 + [vp] * 4 + [i32, i64, vp, vp, i32] + [vp] * 5 + [vp]
+    L.yp_quantized_row_bytes.restype = i64
+    L.yp_quantized_row_bytes.argtypes = [i32]
+    L.yp_quantized_linear_workspace.restype = i64
+    L.yp_quantized_linear_workspace.argtypes = [i32] * 2
+    L.yp_quantize_rows.restype = ctypes.c_int
+    L.yp_quantize_rows.argtypes = [i32] * 4 + [vp] * 3 + [vp]
+    L.yp_quantized_linear.restype = ctypes.c_int
+    L.yp_quantized_linear.argtypes = [i32] * 5 + [vp] * 7 + [i32, vp]
+    L.yp_dropout.restype = ctypes.c_int
+    L.yp_dropout.argtypes = [i32, i64, i32, ctypes.c_double] + [vp] * 3 + [vp]
     L.yp_version.restype = ctypes.c_int
     L.yp_version.argtypes = []
     _lib = L

@@ -739,3 +739,138 @@ extern "C" int64_t yp_rle_strings(const uint32_t* counts, const int64_t* starts,
 }
 
 extern "C" int64_t yp_scratch_bytes(const yp_handle* h) { return h ? h->scratch_bytes : 0; }
+
+// ---- operators of the prediction head ---------------------------------------------------------------
+static bool head_type(int t) { return t == YP_F32 || t == YP_BF16 || t == YP_F16; }
+static bool elem_aligned(const void* p, int t) { return ((uintptr_t)p & (t == YP_F32 ? 3 : 1)) == 0; }
+
+static int check_class_loss_sizes(const char* who, int n, int v, int d, int dtype) {
+  if (!head_type(dtype)) return fail(YP_EINVAL, "%s: dtype must be YP_F32, YP_BF16 or YP_F16", who);
+  if (n < 0 || n > (1 << 20)) return fail(YP_EINVAL, "%s: n must be in [0, 2^20]", who);
+  if (v < 1 || v > (1 << 24)) return fail(YP_EINVAL, "%s: v must be in [1, 2^24]", who);
+  if (d < 1 || d > 65536) return fail(YP_EINVAL, "%s: d must be in [1, 65536]", who);
+  return YP_OK;
+}
+
+extern "C" int64_t yp_class_loss_workspace(int32_t n, int32_t v, int32_t d, int32_t dtype, int32_t has_bias, int32_t backward) {
+  const int rc = check_class_loss_sizes("yp_class_loss_workspace", n, v, d, dtype);
+  if (rc != YP_OK) return rc;
+  return n == 0 ? 0 : yp_class_loss_bytes(n, v, d, dtype, has_bias, backward);
+}
+
+static int check_class_loss(const char* who, const yp_class_loss_args& a) {
+  const int rc = check_class_loss_sizes(who, a.n, a.v, a.d, a.type);
+  if (rc != YP_OK) return rc;
+  if (a.label_bytes != 4 && a.label_bytes != 8) return fail(YP_EINVAL, "%s: label_bytes must be 4 or 8", who);
+  if (!a.weight || (a.n > 0 && (!a.features || !a.labels || !a.lse || !a.workspace))) return fail(YP_EINVAL, "%s: null argument", who);
+  if (!elem_aligned(a.features, a.type) || !elem_aligned(a.weight, a.type) || !elem_aligned(a.bias, a.type) ||
+      ((uintptr_t)a.labels & (a.label_bytes - 1)) != 0 || ((uintptr_t)a.lse & 3) != 0)
+    return fail(YP_EINVAL, "%s: a tensor is not aligned to its elements", who);
+  if (((uintptr_t)a.workspace & 255) != 0) return fail(YP_EINVAL, "%s: workspace must be 256-byte aligned", who);
+  return YP_OK;
+}
+
+extern "C" int yp_class_loss(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
+                             const void* bias, const void* labels, int32_t label_bytes, int64_t ignore_index, void* workspace,
+                             float* losses, float* lse, float* reduced, void* hip_stream) {
+  yp_class_loss_args a = {};
+  a.n = n; a.v = v; a.d = d; a.type = dtype; a.features = features; a.weight = weight; a.bias = bias; a.labels = labels;
+  a.label_bytes = label_bytes; a.ignore_index = ignore_index; a.workspace = workspace; a.losses = losses; a.lse = lse; a.reduced = reduced;
+  const int rc = check_class_loss("yp_class_loss", a);
+  if (rc != YP_OK) return rc;
+  if (n > 0 && !losses) return fail(YP_EINVAL, "yp_class_loss: null argument");
+  if ((((uintptr_t)losses | (uintptr_t)reduced) & 3) != 0) return fail(YP_EINVAL, "yp_class_loss: a tensor is not aligned to its elements");
+  YP_ON_DEVICE(device_id);
+  YP_HIP(yp_launch_class_loss(a, (hipStream_t)hip_stream));
+  return YP_OK;
+}
+
+extern "C" int yp_class_loss_backward(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
+                                      const void* bias, const void* labels, int32_t label_bytes, int64_t ignore_index, const float* lse,
+                                      const float* grad, int32_t grad_stride, const float* count, void* workspace,
+                                      void* grad_features, void* grad_weight, void* grad_bias, void* hip_stream) {
+  yp_class_loss_args a = {};
+  a.n = n; a.v = v; a.d = d; a.type = dtype; a.features = features; a.weight = weight; a.bias = bias; a.labels = labels;
+  a.label_bytes = label_bytes; a.ignore_index = ignore_index; a.workspace = workspace; a.lse = const_cast<float*>(lse);
+  a.grad = grad; a.grad_stride = grad_stride; a.count = count;
+  a.grad_features = grad_features; a.grad_weight = grad_weight; a.grad_bias = grad_bias;
+  const int rc = check_class_loss("yp_class_loss_backward", a);
+  if (rc != YP_OK) return rc;
+  if (grad_stride != 0 && grad_stride != 1) return fail(YP_EINVAL, "yp_class_loss_backward: grad_stride must be 0 or 1");
+  if (!grad_weight || (n > 0 && (!grad || !grad_features)) || (bias != nullptr) != (grad_bias != nullptr))
+    return fail(YP_EINVAL, "yp_class_loss_backward: null argument (grad_bias goes with bias)");
+  if (!elem_aligned(grad_features, dtype) || !elem_aligned(grad_weight, dtype) || !elem_aligned(grad_bias, dtype) ||
+      (((uintptr_t)grad | (uintptr_t)count) & 3) != 0)
+    return fail(YP_EINVAL, "yp_class_loss_backward: a tensor is not aligned to its elements");
+  YP_ON_DEVICE(device_id);
+  YP_HIP(yp_launch_class_loss_backward(a, (hipStream_t)hip_stream));
+  return YP_OK;
+}
+
+static int check_quantized(const char* who, int rows, int k) {
+  if (rows < 0) return fail(YP_EINVAL, "%s: rows must be >= 0", who);
+  if (k < 1 || k > 131072) return fail(YP_EINVAL, "%s: k must be in [1, 131072]", who);
+  return YP_OK;
+}
+
+extern "C" int64_t yp_quantized_row_bytes(int32_t k) {
+  const int rc = check_quantized("yp_quantized_row_bytes", 0, k);
+  return rc != YP_OK ? rc : yp_qrow_bytes(k);
+}
+
+extern "C" int64_t yp_quantized_linear_workspace(int32_t rows, int32_t k) {
+  const int rc = check_quantized("yp_quantized_linear_workspace", rows, k);
+  return rc != YP_OK ? rc : (int64_t)rows * yp_qrow_bytes(k) + (int64_t)rows * 4;
+}
+
+extern "C" int yp_quantize_rows(int32_t device_id, int32_t rows, int32_t k, int32_t dtype, const void* x, void* q, float* scale, void* hip_stream) {
+  const int rc = check_quantized("yp_quantize_rows", rows, k);
+  if (rc != YP_OK) return rc;
+  if (!head_type(dtype)) return fail(YP_EINVAL, "yp_quantize_rows: dtype must be YP_F32, YP_BF16 or YP_F16");
+  if (rows == 0) return YP_OK;
+  if (!x || !q || !scale) return fail(YP_EINVAL, "yp_quantize_rows: null argument");
+  if (!elem_aligned(x, dtype) || ((uintptr_t)q & 15) != 0 || ((uintptr_t)scale & 3) != 0)
+    return fail(YP_EINVAL, "yp_quantize_rows: x and scale must be aligned to their elements, q to 16 bytes");
+  YP_ON_DEVICE(device_id);
+  YP_HIP(yp_launch_quantize_rows(rows, k, dtype, x, q, scale, (hipStream_t)hip_stream));
+  return YP_OK;
+}
+
+extern "C" int yp_quantized_linear(int32_t device_id, int32_t rows, int32_t v, int32_t k, int32_t dtype, const void* x, const float* x_scale,
+                                   const void* wq, const float* w_scale, const float* bias, void* workspace, void* out, int32_t out_dtype,
+                                   void* hip_stream) {
+  const int rc = check_quantized("yp_quantized_linear", rows, k);
+  if (rc != YP_OK) return rc;
+  if (dtype != YP_INT8 && !head_type(dtype)) return fail(YP_EINVAL, "yp_quantized_linear: dtype must be YP_INT8, YP_F32, YP_BF16 or YP_F16");
+  if (!head_type(out_dtype)) return fail(YP_EINVAL, "yp_quantized_linear: out_dtype must be YP_F32, YP_BF16 or YP_F16");
+  if (v < 1 || v > (1 << 24)) return fail(YP_EINVAL, "yp_quantized_linear: v must be in [1, 2^24]");
+  if (((int64_t)rows + 127) / 128 * (((int64_t)v + 127) / 128) >= (1ll << 30)) return fail(YP_EINVAL, "yp_quantized_linear: rows * v is too large");
+  if (rows == 0) return YP_OK;
+  if (!x || !wq || !w_scale || !out || (dtype == YP_INT8 ? !x_scale : !workspace)) return fail(YP_EINVAL, "yp_quantized_linear: null argument");
+  if (((uintptr_t)wq & 15) != 0 || (dtype == YP_INT8 ? ((uintptr_t)x & 15) != 0 : !elem_aligned(x, dtype)) || !elem_aligned(out, out_dtype) ||
+      (((uintptr_t)x_scale | (uintptr_t)w_scale | (uintptr_t)bias) & 3) != 0)
+    return fail(YP_EINVAL, "yp_quantized_linear: a tensor is not aligned (8-bit rows to 16 bytes, the others to their elements)");
+  if (((uintptr_t)workspace & 255) != 0) return fail(YP_EINVAL, "yp_quantized_linear: workspace must be 256-byte aligned");
+  YP_ON_DEVICE(device_id);
+  const void* xq = x;
+  if (dtype != YP_INT8) {
+    xq = workspace;
+    float* const s = (float*)((char*)workspace + (int64_t)rows * yp_qrow_bytes(k));
+    YP_HIP(yp_launch_quantize_rows(rows, k, dtype, x, workspace, s, (hipStream_t)hip_stream));
+    x_scale = s;
+  }
+  YP_HIP(yp_launch_quantized_linear(rows, v, k, xq, x_scale, wq, w_scale, bias, out, out_dtype, (hipStream_t)hip_stream));
+  return YP_OK;
+}
+
+extern "C" int yp_dropout(int32_t device_id, int64_t count, int32_t dtype, double p, const int64_t* state, const void* x, void* y, void* hip_stream) {
+  if (!head_type(dtype)) return fail(YP_EINVAL, "yp_dropout: dtype must be YP_F32, YP_BF16 or YP_F16");
+  if (!(p >= 0.0 && p <= 1.0)) return fail(YP_EINVAL, "yp_dropout: p must be in [0, 1]");
+  if (count < 0) return fail(YP_EINVAL, "yp_dropout: negative count");
+  if (count == 0) return YP_OK;
+  if (!state || !x || !y) return fail(YP_EINVAL, "yp_dropout: null argument");
+  if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || ((uintptr_t)state & 7) != 0) return fail(YP_EINVAL, "yp_dropout: a tensor is not aligned to its elements");
+  YP_ON_DEVICE(device_id);
+  YP_HIP(yp_launch_dropout(count, dtype, p, state, x, y, (hipStream_t)hip_stream));
+  return YP_OK;
+}

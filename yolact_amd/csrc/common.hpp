@@ -286,3 +286,26 @@ size_t yp_loss_grads_workspace_floats(int batch, int rows, int ph);
 hipError_t yp_launch_loss_grads(int batch, int rows, int ph, int pw, int img_h, int img_w, int use_crop, const float* proto,
                                 const float* coef, const float* boxes, const int32_t* num_rows, const float* masks,
                                 const float* grad_masks, float* workspace, float* grad_proto, float* grad_coef, hipStream_t st);
+
+// Prediction-head operators (class_loss.hip, quantized.hip, dropout.hip).
+struct yp_class_loss_args {
+  int n, v, d, type;                       // rows, classes, features, YP_F32 / YP_BF16 / YP_F16
+  const void *features, *weight, *bias;    // bias may be null
+  const void* labels;
+  int label_bytes;                         // 4 or 8
+  int64_t ignore_index;
+  void* workspace;
+  float *losses, *lse, *reduced;           // forward results (lse is an input of the backward); reduced may be null
+  const float* grad;                       // backward: dL/dloss of every row (stride 1) or of all of them (stride 0)
+  int grad_stride;
+  const float* count;                      // null, or the grads are divided by max(*count, 1)
+  void *grad_features, *grad_weight, *grad_bias;
+};
+int64_t yp_class_loss_bytes(int64_t n, int64_t v, int64_t d, int type, int has_bias, int backward);
+hipError_t yp_launch_class_loss(const yp_class_loss_args& a, hipStream_t st);
+hipError_t yp_launch_class_loss_backward(const yp_class_loss_args& a, hipStream_t st);
+int64_t yp_qrow_bytes(int64_t k);
+hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x, void* q, float* scale, hipStream_t st);
+hipError_t yp_launch_quantized_linear(int rows, int v, int k, const void* xq, const float* x_scale, const void* wq, const float* w_scale,
+                                      const float* bias, void* out, int out_type, hipStream_t st);
+hipError_t yp_launch_dropout(int64_t count, int type, double p, const int64_t* state, const void* x, void* y, hipStream_t st);

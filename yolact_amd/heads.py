@@ -1,0 +1,261 @@
+"""Operators of the prediction head, on the device: what trains the class head and what runs it in 8 bits.
+
+* ``class_loss`` / ``class_loss_backward`` / ``ClassLoss`` - softmax cross entropy of features against a class matrix,
+  for vocabularies of any size: the logits are never stored (``csrc/class_loss.hip``).  It stands beside the mask part
+  of the training loss (``consumer.LossMaskAssembly``).
+* ``quantize_rows`` / ``quantized_linear`` - the head's products in 8-bit integers with one scale per row of either
+  operand, float32 out as ``Detect`` takes it (``csrc/quantized.hip``); ``QuantizedHeads`` puts the three of them together.
+* ``dropout`` / ``Dropout`` - a mask that is computed again instead of stored (``csrc/dropout.hip``);
+  ``class_head_loss`` applies it to the features on their way into the class loss.
+
+torch is plumbing (device memory, current stream, autograd); there is no CPU fallback.  Tensors live on one CUDA device,
+are contiguous, and results are stream-ordered on torch's current stream of that device.  Workspaces are torch tensors of
+the call itself, so calls on different streams or captured graphs share nothing.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: _lib.YP_F32, torch.bfloat16: _lib.YP_BF16, torch.float16: _lib.YP_F16}
+_REDUCTIONS = ("none", "sum", "mean")
+
+
+def _check(name, t, dtypes, shape=None, device=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name} must be a CUDA tensor" + (f" on {device}" if device is not None else ""))
+    if t.dtype not in dtypes or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+        want = " or ".join(str(d) for d in dtypes)
+        raise ValueError(f"{name} must be contiguous {want}" + (f" of shape {tuple(shape)}" if shape is not None else "") +
+                         f", got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _stream(device):
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _workspace(nbytes, device):
+    if nbytes < 0:
+        _lib.check(int(nbytes))
+    return torch.empty((int(nbytes),), dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+# ---- class loss ------------------------------------------------------------------------------------------------------
+def _class_loss_args(features, weight, labels, bias):
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be a CUDA tensor [classes, features]")
+    V, D = weight.shape
+    if not isinstance(features, torch.Tensor) or features.dim() < 1 or features.shape[-1] != D:
+        raise ValueError(f"features must be a CUDA tensor [..., {D}]")
+    dev, lead = weight.device, features.shape[:-1]
+    p_w = _check("weight", weight, tuple(_TYPES))
+    p_h = _check("features", features, (weight.dtype,), device=dev)
+    p_y = _check("labels", labels, (torch.int64, torch.int32), lead, dev)
+    p_b = _check("bias", bias, (weight.dtype,), (V,), dev) if bias is not None else None
+    return p_h, p_w, p_b, p_y, labels.numel(), V, D, lead, dev
+
+
+def _class_loss_forward(features, weight, labels, bias, ignore_index, reduce):
+    p_h, p_w, p_b, p_y, N, V, D, lead, dev = _class_loss_args(features, weight, labels, bias)
+    L, dt = _lib.load(), _TYPES[weight.dtype]
+    ws = _workspace(L.yp_class_loss_workspace(N, V, D, dt, bias is not None, 0), dev)
+    losses = torch.empty(lead, dtype=torch.float32, device=dev)
+    lse = torch.empty(lead, dtype=torch.float32, device=dev)
+    reduced = torch.empty((3,), dtype=torch.float32, device=dev) if reduce else None
+    _lib.check(L.yp_class_loss(dev.index, N, V, D, dt, p_h, p_w, p_b, p_y, labels.element_size(), int(ignore_index), _ptr(ws),
+                               losses.data_ptr(), lse.data_ptr(), _ptr(reduced), _stream(dev)))
+    return losses, lse, reduced
+
+
+def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
+    """Softmax cross entropy of ``features`` [..., D] against the class matrix ``weight`` [V, D] (and ``bias`` [V]), all of
+    one type (float32, bfloat16, float16): returns ``(losses, lse)``, float32 of the shape of ``labels`` [...] (int64 or
+    int32), with ``lse = log sum exp`` of the logits and ``losses = lse - logit[label]``.
+
+    A row labelled ``ignore_index`` takes no part (loss 0) whatever its features hold; any other label outside [0, V) has
+    loss NaN.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf."""
+    losses, lse, _ = _class_loss_forward(features, weight, labels, bias, ignore_index, False)
+    return losses, lse
+
+
+def _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad, per_row, count):
+    p_h, p_w, p_b, p_y, N, V, D, lead, dev = _class_loss_args(features, weight, labels, bias)
+    p_l = _check("lse", lse, (torch.float32,), lead, dev)
+    p_g = _check("grad_losses", grad, (torch.float32,), lead if per_row else (), dev)
+    L, dt = _lib.load(), _TYPES[weight.dtype]
+    ws = _workspace(L.yp_class_loss_workspace(N, V, D, dt, bias is not None, 1), dev)
+    gh, gw = torch.empty_like(features), torch.empty_like(weight)
+    gb = torch.empty_like(bias) if bias is not None else None
+    _lib.check(L.yp_class_loss_backward(dev.index, N, V, D, dt, p_h, p_w, p_b, p_y, labels.element_size(), int(ignore_index), p_l,
+                                        p_g, int(per_row), _ptr(count), _ptr(ws), gh.data_ptr(), gw.data_ptr(), _ptr(gb), _stream(dev)))
+    return gh, gw, gb
+
+
+def class_loss_backward(features, weight, labels, lse, grad_losses, bias=None, ignore_index: int = -1):
+    """Gradients of ``class_loss``'s losses: ``(grad_features, grad_weight, grad_bias or None)`` given ``lse`` as the forward
+    returned it for the same inputs and ``grad_losses`` (float32, the shape of ``labels``).  The logits are computed again,
+    in pieces of the vocabulary; sums run in float32 in a fixed order, each gradient is rounded once."""
+    return _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad_losses, True, None)
+
+
+class ClassLoss(torch.autograd.Function):
+    """Differentiable class loss: ``ClassLoss.apply(features, weight, bias, labels, ignore_index=-1, reduction="mean")``.
+    ``reduction`` "none" gives the rows' losses, "sum" and "mean" one value, "mean" over the rows that are not ignored (0 if
+    there are none).  Gradients flow to features, weight and bias (which may be None).  When forward and backward are
+    captured into a graph, capture both, on leaves whose eager graphs are gone."""
+
+    @staticmethod
+    def forward(ctx, features, weight, bias, labels, ignore_index=-1, reduction="mean"):
+        if reduction not in _REDUCTIONS:
+            raise ValueError(f"reduction must be one of {_REDUCTIONS}")
+        features, weight, labels = features.contiguous(), weight.contiguous(), labels.contiguous()
+        bias = bias.contiguous() if bias is not None else None
+        losses, lse, reduced = _class_loss_forward(features, weight, labels, bias, ignore_index, reduction != "none")
+        ctx.save_for_backward(features, weight, bias, labels, lse, reduced)
+        ctx.cfg = (int(ignore_index), reduction)
+        return losses if reduction == "none" else reduced[_REDUCTIONS.index(reduction) - 1]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        features, weight, bias, labels, lse, reduced = ctx.saved_tensors
+        ignore_index, reduction = ctx.cfg
+        gh, gw, gb = _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad.contiguous(), reduction == "none",
+                                          reduced[2:] if reduction == "mean" else None)
+        return gh, gw, gb, None, None, None
+
+
+# ---- dropout ---------------------------------------------------------------------------------------------------------
+def dropout(x, p: float, state, out=None):
+    """``x`` (float32, bfloat16, float16, any shape) with every element kept with probability 1 - p, then divided by it, else
+    0 (also where x is not finite).  ``state`` is an int64 CUDA tensor [2]: the key and the first counter; element i uses
+    word i % 4 of Philox4x32-10 at counter ``state[1] + i // 4``.  The same state gives the same mask - which is how the
+    backward pass has it - so advance ``state[1]`` by ``(x.numel() + 3) // 4`` before the next use, and not before the
+    backward of this one.  It is read on the device: a captured call follows it on every replay.  ``out`` may be x."""
+    p_x = _check("x", x, tuple(_TYPES))
+    dev = x.device
+    p_s = _check("state", state, (torch.int64,), (2,), dev)
+    if not 0.0 <= float(p) <= 1.0:
+        raise ValueError("p must be in [0, 1]")
+    if out is None:
+        out = torch.empty_like(x)
+    p_o = _check("out", out, (x.dtype,), x.shape, dev)
+    _lib.check(_lib.load().yp_dropout(dev.index, x.numel(), _TYPES[x.dtype], float(p), p_s, p_x, p_o, _stream(dev)))
+    return out
+
+
+class Dropout(torch.autograd.Function):
+    """Differentiable dropout: ``Dropout.apply(x, p, state)``.  Only ``state`` is kept for the backward pass, which computes
+    the mask again; changing ``state`` in between is an error that torch reports."""
+
+    @staticmethod
+    def forward(ctx, x, p, state):
+        y = dropout(x.contiguous(), p, state)
+        ctx.save_for_backward(state)
+        ctx.p = float(p)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        state, = ctx.saved_tensors
+        return dropout(grad.contiguous(), ctx.p, state), None, None
+
+
+def class_head_loss(features, weight, bias, labels, dropout_p: float = 0.0, state=None, ignore_index: int = -1, reduction: str = "mean"):
+    """The class head's training step: dropout on the features (``dropout_p`` > 0 needs ``state``), then ``ClassLoss``."""
+    if dropout_p:
+        if state is None:
+            raise ValueError("dropout needs its state")
+        features = Dropout.apply(features, dropout_p, state)
+    return ClassLoss.apply(features, weight, bias, labels, ignore_index, reduction)
+
+
+# ---- quantized linear ------------------------------------------------------------------------------------------------
+class QuantizedRows:
+    """Rows in 8 bits: ``q`` int8 [rows, padded k] (the padding is zero), ``scale`` float32 [rows], ``k``; row r stands for
+    ``q[r, :k] * scale[r]``."""
+
+    def __init__(self, q, scale, k, lead):
+        self.q, self.scale, self.k, self.lead = q, scale, int(k), tuple(lead)
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def dequantize(self):
+        """The values the rows stand for, float32 [..., k]."""
+        return (self.q[:, :self.k].float() * self.scale[:, None]).reshape(*self.lead, self.k)
+
+
+def quantize_rows(x) -> QuantizedRows:
+    """``x`` [..., k] (float32, bfloat16, float16) in 8 bits, one scale per row: scale = max|x| / 127, q = x / scale to the
+    nearest, ties to even.  A row that holds an infinity or NaN has scale NaN.  k <= 131072."""
+    p_x = _check("x", x, tuple(_TYPES))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have at least one element per row")
+    dev, k, lead = x.device, x.shape[-1], x.shape[:-1]
+    rows = x.numel() // k
+    L = _lib.load()
+    kp = int(L.yp_quantized_row_bytes(k))
+    if kp < 0:
+        _lib.check(kp)
+    q = torch.empty((rows, kp), dtype=torch.int8, device=dev)
+    scale = torch.empty((rows,), dtype=torch.float32, device=dev)
+    _lib.check(L.yp_quantize_rows(dev.index, rows, k, _TYPES[x.dtype], p_x, q.data_ptr(), scale.data_ptr(), _stream(dev)))
+    return QuantizedRows(q, scale, k, lead)
+
+
+def quantized_linear(x, weight: QuantizedRows, bias=None, out_dtype=torch.float32):
+    """``x @ weight^T + bias`` with 8-bit integer products: ``x`` [..., k] float32 / bfloat16 / float16 (quantized row by row
+    on the way) or ``QuantizedRows``; ``weight`` = ``quantize_rows`` of a [v, k] matrix; ``bias`` float32 [v].  Returns
+    [..., v] of ``out_dtype``: integer sums are exact, scales and bias are applied in float32, one rounding to the type."""
+    if not isinstance(weight, QuantizedRows) or len(weight.lead) != 1 or weight.lead[0] < 1:
+        raise ValueError("weight must be quantize_rows of a [v, k] matrix")
+    if out_dtype not in _TYPES:
+        raise ValueError("out_dtype must be float32, bfloat16 or float16")
+    dev, v, k = weight.device, weight.lead[0], weight.k
+    L = _lib.load()
+    p_b = _check("bias", bias, (torch.float32,), (v,), dev) if bias is not None else None
+    ws = None
+    if isinstance(x, QuantizedRows):
+        if x.k != k or x.device != dev:
+            raise ValueError(f"x must hold rows of {k} on {dev}")
+        lead, rows, dt, p_x, p_s = x.lead, x.scale.shape[0], _lib.YP_INT8, x.q.data_ptr(), x.scale.data_ptr()
+    else:
+        p_x, p_s = _check("x", x, tuple(_TYPES), device=dev), None
+        if x.dim() < 1 or x.shape[-1] != k:
+            raise ValueError(f"x must have rows of {k}")
+        lead, rows, dt = x.shape[:-1], x.numel() // k, _TYPES[x.dtype]
+        ws = _workspace(L.yp_quantized_linear_workspace(rows, k), dev)
+    out = torch.empty((*lead, v), dtype=out_dtype, device=dev)
+    _lib.check(L.yp_quantized_linear(dev.index, rows, v, k, dt, p_x, p_s, weight.q.data_ptr(), weight.scale.data_ptr(), p_b, _ptr(ws),
+                                     out.data_ptr(), _TYPES[out_dtype], _stream(dev)))
+    return out
+
+
+class QuantizedHeads:
+    """The three products of the prediction head in 8 bits: class logits, box offsets and mask coefficients of every anchor's
+    features, in the shapes and the type ``Detect`` takes.  Each head is a float weight [out, D], or a pair of it and a
+    float32 bias [out] (layers/head.py's last layers, with an anchor's features as the row)."""
+
+    def __init__(self, cls, offset, mask_coef):
+        def keep(h):
+            w, b = h if isinstance(h, (tuple, list)) else (h, None)
+            return quantize_rows(w), b
+        self.heads = {"pred_cls": keep(cls), "pred_offset": keep(offset), "pred_mask_coef": keep(mask_coef)}
+
+    def __call__(self, features):
+        """features [B, A, D] -> {"pred_cls": [B, A, C], "pred_offset": [B, A, 4], "pred_mask_coef": [B, A, K]} float32, the
+        features quantized once.  The coefficients are what the product gives: the reference's tanh (layers/head.py:81) is
+        the caller's, who may want it in place."""
+        x = quantize_rows(features)
+        return {name: quantized_linear(x, w, bias=b) for name, (w, b) in self.heads.items()}
