@@ -46,20 +46,20 @@ struct yp_epi_stats {
   yp_softmax_part* part;       // [tiles_i * WI][N]
   float* picked;               // [N] z of the label
   template <int TYPE, int BM, int BN, int WI, int WJ, int MI, int NJ, class Acc>
-  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], char*, int ti, int tj, int, int wi, int wj, int lane) const {
-    const int ib = ti * BM + wi * (BM / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / WJ) + (lane & 15);
+  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], int ti, int tj, int, int wi, int wj, int lane) const {
+    const int ib = ti * BM + wi * (BM / 2 / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / 2 / WJ) + (lane & 15);
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = ib + m * 16 + r;
+        const int i = ib + yp_frag_at<BM, MI>(m) + r;
         const float b = i >= V ? -INFINITY : (bias ? yp_load_as_float(bias, i, TYPE) : 0.0f);
 #pragma unroll
         for (int n = 0; n < NJ; ++n) acc[m][n][r] = b == -INFINITY ? -INFINITY : acc[m][n][r] + b;
       }
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
-      const int j = jb + n * 16;
+      const int j = jb + yp_frag_at<BN, NJ>(n);
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
       for (int m = 0; m < MI; ++m)
@@ -72,11 +72,11 @@ struct yp_epi_stats {
         for (int r = 0; r < 4; ++r) sum += yp_exp_hw(acc[m][n][r] - ref);
       if (j < g.J) {
         const int64_t at = yp_label_at(labels, j, label_bytes) - ib;
-        if (at >= 0 && at < MI * 16) {
+        if (at >= 0 && at < BM) {
 #pragma unroll
           for (int m = 0; m < MI; ++m)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) if (at == m * 16 + r) picked[j] = acc[m][n][r];
+            for (int r = 0; r < 4; ++r) if (at == yp_frag_at<BM, MI>(m) + r) picked[j] = acc[m][n][r];
         }
       }
 #pragma unroll
@@ -99,17 +99,17 @@ struct yp_epi_dz {
   int kv, kn;                  // elements, padded: dz is zero in [V, kv), dzt in [N, kn)
   float* bias_part;            // [tiles_j * WJ][V], null without bias
   template <int TYPE, int BM, int BN, int WI, int WJ, int MI, int NJ, class Acc>
-  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], char*, int ti, int tj, int, int wi, int wj, int lane) const {
+  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], int ti, int tj, int, int wi, int wj, int lane) const {
     typedef typename yp_type<TYPE>::elem elem;
     typedef elem e4 __attribute__((ext_vector_type(4)));
-    const int ib = ti * BM + wi * (BM / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / WJ) + (lane & 15);
+    const int ib = ti * BM + wi * (BM / 2 / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / 2 / WJ) + (lane & 15);
     elem* const z0 = reinterpret_cast<elem*>(dz);
     elem* const zt = reinterpret_cast<elem*>(dzt);
     float l[NJ], gr[NJ];
     int lab[NJ];
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
-      const int j = jb + n * 16;
+      const int j = jb + yp_frag_at<BN, NJ>(n);
       const bool in = j < g.J;
       l[n] = in ? lse[j] : 0.0f;
       gr[n] = in ? row_grad[j] : 0.0f;
@@ -118,14 +118,14 @@ struct yp_epi_dz {
     }
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-      const int i = ib + m * 16;
+      const int i = ib + yp_frag_at<BM, MI>(m);
       float col[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       float b[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) b[r] = i + r >= V ? -INFINITY : (bias ? yp_load_as_float(bias, i + r, TYPE) : 0.0f);
 #pragma unroll
       for (int n = 0; n < NJ; ++n) {
-        const int j = jb + n * 16;
+        const int j = jb + yp_frag_at<BN, NJ>(n);
         e4 o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -311,7 +311,9 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const float
   for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < total; e += (int64_t)gridDim.x * YP_CL_THREADS) {
     float s = 0.0f;
     for (int p = 0; p < parts; ++p) s += part[(int64_t)p * stride + e];
-    yp_store_from_float(out, e, out_type, s * sc);
+    if (out_type == YP_F32) reinterpret_cast<float*>(out)[e] = s * sc;
+    else if (out_type == YP_BF16) reinterpret_cast<__bf16*>(out)[e] = (__bf16)(s * sc);
+    else reinterpret_cast<_Float16*>(out)[e] = (_Float16)(s * sc);
   }
 }
 
@@ -368,7 +370,7 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   p.dzp = yp_plan_tiles(piece, p.kn / b, p.kd / YP_TILE_KB, false);   // (the padded rows too: their columns of dzt are zeros)
   p.dwp = yp_plan_tiles(D, piece, p.kn / YP_TILE_KB, true);
   p.dhp = yp_plan_tiles(D, N, p.kv / YP_TILE_KB, true);
-  p.bias_parts = p.dzp.tiles_j * (p.dzp.shape == YP_TILE_L ? 4 : p.dzp.shape == YP_TILE_M ? 2 : 1);
+  p.bias_parts = p.dzp.tiles_j * (p.dzp.shape == YP_TILE_S ? 1 : 2);
   p.o_rg = take(N * 4);
   p.o_rl = take(N * 4);
   p.o_factor = take(8);
@@ -492,7 +494,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     gw.steps = (int)(p.kn / YP_TILE_KB);
     char* const gwo = (char*)a.grad_weight + (int64_t)v0 * a.d * b;
     yp_epi_store ew = {};
-    ew.out = gwo; ew.ld = a.d; ew.out_type = TYPE; ew.scale = back;
+    ew.out = gwo; ew.ld = a.d; ew.scale = back;
     ew.vec = a.d % 4 == 0 && ((uintptr_t)a.grad_weight & 15) == 0;
     ew.part = p.dwp.splits > 1 ? (float*)(ws + p.o_dwpart) : nullptr;
     yp_tile_plan twp = p.dwp;
@@ -509,7 +511,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     gh.b = ws + p.o_dz; gh.ldb = (int64_t)e.kv * b; gh.J = a.n;
     gh.steps = (int)((int64_t)e.kv * b / YP_TILE_KB);
     yp_epi_store eh = {};
-    eh.out = a.grad_features; eh.ld = a.d; eh.out_type = TYPE; eh.scale = back;
+    eh.out = a.grad_features; eh.ld = a.d; eh.scale = back;
     eh.vec = a.d % 4 == 0 && ((uintptr_t)a.grad_features & 15) == 0;
     eh.part = dh_joined ? dhpart : nullptr;
     eh.add = s > 0;

@@ -45,7 +45,8 @@ __global__ __launch_bounds__(YP_DO_THREADS) void yp_dropout_kernel(const void* x
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) v[u] = (uint64_t)w[u] >= least ? v[u] * scale : 0.0f;
-    yp_store4(yp, i * 4, TYPE, v, n, vec != 0);
+    if (vec) yp_store4<TYPE, true>(yp, i * 4, v, n);
+    else yp_store4<TYPE, false>(yp, i * 4, v, n);
   }
 }
 

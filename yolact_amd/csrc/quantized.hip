@@ -109,47 +109,60 @@ hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x,
        : type == YP_BF16 ? quantize_t<YP_T_BF16>(rows, k, x, q, scale, st) : quantize_t<YP_T_F16>(rows, k, x, q, scale, st);
 }
 
+template <int OUT>
 struct yp_epi_scaled {
   const float *x_scale, *w_scale, *bias;
   void* out;
-  int out_type, vec;
+  int vec;
   template <int TYPE, int BM, int BN, int WI, int WJ, int MI, int NJ, class Acc>
-  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], char*, int ti, int tj, int, int wi, int wj, int lane) const {
-    const int ib = ti * BM + wi * (BM / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / WJ) + (lane & 15);
+  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], int ti, int tj, int, int wi, int wj, int lane) const {
+    const int ib = ti * BM + wi * (BM / 2 / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / 2 / WJ) + (lane & 15);
+    if (vec) put<BM, BN, true>(g, acc, ib, jb);
+    else put<BM, BN, false>(g, acc, ib, jb);
+  }
+  template <int BM, int BN, bool VEC, int MI, int NJ, class Acc>
+  __device__ __forceinline__ void put(const yp_gemm& g, Acc (&acc)[MI][NJ], int ib, int jb) const {
     float sx[NJ];
 #pragma unroll
-    for (int n = 0; n < NJ; ++n) sx[n] = jb + n * 16 < g.J ? x_scale[jb + n * 16] : 0.0f;
+    for (int n = 0; n < NJ; ++n) sx[n] = jb + yp_frag_at<BN, NJ>(n) < g.J ? x_scale[jb + yp_frag_at<BN, NJ>(n)] : 0.0f;
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-      const int i = ib + m * 16, left = g.I - i;
-      if (left <= 0) continue;
-      yp_f4 sw, b = {0.0f, 0.0f, 0.0f, 0.0f};
+      const int i = ib + yp_frag_at<BM, MI>(m), left = g.I - i;
+      if (left > 0) {
+        yp_f4 sw, b;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        sw[r] = r < left ? w_scale[i + r] : 0.0f;
-        if (bias && r < left) b[r] = bias[i + r];
-      }
+        for (int r = 0; r < 4; ++r) {
+          sw[r] = r < left ? w_scale[i + r] : 0.0f;
+          b[r] = bias && r < left ? bias[i + r] : 0.0f;
+        }
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) {
-        const int j = jb + n * 16;
-        if (j >= g.J) continue;
-        yp_f4 y;
+        for (int n = 0; n < NJ; ++n) {
+          if (jb + yp_frag_at<BN, NJ>(n) < g.J) {
+            yp_f4 y;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = __builtin_fmaf((float)acc[m][n][r] * sx[n], sw[r], b[r]);
-        yp_store4(out, (int64_t)j * g.I + i, out_type, y, left, vec != 0);
+            for (int r = 0; r < 4; ++r) y[r] = __builtin_fmaf((float)acc[m][n][r] * sx[n], sw[r], b[r]);
+            yp_store4<OUT, VEC>(out, (int64_t)(jb + yp_frag_at<BN, NJ>(n)) * g.I + i, y, left);
+          }
+        }
       }
     }
   }
 };
 
+template <int OUT>
+static hipError_t linear_t(const yp_gemm& g, const float* x_scale, const float* w_scale, const float* bias, void* out, hipStream_t st) {
+  yp_epi_scaled<OUT> e;
+  e.x_scale = x_scale; e.w_scale = w_scale; e.bias = bias; e.out = out;
+  e.vec = g.I % 4 == 0 && ((uintptr_t)out & 15) == 0;
+  return yp_launch_gemm<YP_T_I8>(yp_plan_tiles(g.I, g.J, g.steps, false), g, e, st);
+}
+
 hipError_t yp_launch_quantized_linear(int rows, int v, int k, const void* xq, const float* x_scale, const void* wq, const float* w_scale,
                                       const float* bias, void* out, int out_type, hipStream_t st) {
-  const int64_t kp = yp_qrow_bytes(k);
   yp_gemm g = {};
-  g.a = (const char*)wq; g.b = (const char*)xq; g.lda = g.ldb = kp;
-  g.I = v; g.J = rows; g.steps = (int)(kp / YP_TILE_KB);
-  yp_epi_scaled e;
-  e.x_scale = x_scale; e.w_scale = w_scale; e.bias = bias; e.out = out; e.out_type = out_type;
-  e.vec = v % 4 == 0 && ((uintptr_t)out & 15) == 0;
-  return yp_launch_gemm<YP_T_I8>(yp_plan_tiles(v, rows, g.steps, false), g, e, st);
+  g.lda = g.ldb = yp_qrow_bytes(k);
+  g.a = (const char*)wq; g.b = (const char*)xq;
+  g.I = v; g.J = rows; g.steps = (int)(g.lda / YP_TILE_KB);
+  return out_type == YP_F32 ? linear_t<YP_T_F32>(g, x_scale, w_scale, bias, out, st)
+       : out_type == YP_BF16 ? linear_t<YP_T_BF16>(g, x_scale, w_scale, bias, out, st) : linear_t<YP_T_F16>(g, x_scale, w_scale, bias, out, st);
 }
