@@ -4,8 +4,6 @@
 
 #include "gemm_tile.hpp"
 
-enum { YP_TILE_L = 0, YP_TILE_M = 1, YP_TILE_S = 2 };
-
 struct yp_tile_plan {
   int shape;      // YP_TILE_*
   int bi, bj;     // its tile
@@ -15,33 +13,65 @@ struct yp_tile_plan {
 // L 256 x 256 (4 waves of 128 x 128: 256 rows of fragments read for 128 x 128 results, half of what M reads),
 // M 128 x 128 (4 waves of 64 x 64, two workgroups a CU), S 128 x 64 (4 waves of 32 x 64, three workgroups a CU) for few
 // rows, where only streaming A counts.  L needs about a full round of tiles; below that M's finer cut wins.
-static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps, bool may_split) {
-  const int cus = 256;   // MI355X
+static inline yp_tile_plan yp_plan_shape(int shape, int64_t I, int64_t J) {
   yp_tile_plan p;
-  const int64_t tl = ((I + 255) / 256) * ((J + 255) / 256);
-  p.shape = J <= 64 ? YP_TILE_S : (tl * 4 >= (int64_t)cus * 3 ? YP_TILE_L : YP_TILE_M);
-  p.bi = p.shape == YP_TILE_L ? 256 : 128;
-  p.bj = p.shape == YP_TILE_L ? 256 : (p.shape == YP_TILE_M ? 128 : 64);
+  p.shape = shape;
+  p.bi = shape == YP_TILE_L ? 256 : 128;
+  p.bj = shape == YP_TILE_L ? 256 : (shape == YP_TILE_M ? 128 : 64);
   p.tiles_i = (int)((I + p.bi - 1) / p.bi);
   p.tiles_j = (int)((J + p.bj - 1) / p.bj);
   p.splits = 1;
-  const int64_t tiles = (int64_t)p.tiles_i * p.tiles_j;
-  if (may_split && tiles < cus) {   // few tiles: deal the k axis to more workgroups, at least 4 steps each
-    int64_t s = (2 * cus + tiles - 1) / tiles;
-    if (s > steps / 4) s = steps / 4;
-    p.splits = s < 1 ? 1 : (int)s;
-  }
   return p;
+}
+// Few tiles: deal the k axis to more workgroups, up to two for each of `cus` compute units, at least 4 steps each.
+static inline void yp_plan_splits(yp_tile_plan* p, int64_t steps, int cus) {
+  const int64_t tiles = (int64_t)p->tiles_i * p->tiles_j;
+  if (tiles >= cus) return;
+  int64_t s = (2 * cus + tiles - 1) / tiles;
+  if (s > steps / 4) s = steps / 4;
+  p->splits = s < 1 ? 1 : (int)s;
+}
+static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps, bool may_split) {
+  const int64_t tl = ((I + 255) / 256) * ((J + 255) / 256);
+  yp_tile_plan p = yp_plan_shape(J <= 64 ? YP_TILE_S : tl >= 192 ? YP_TILE_L : YP_TILE_M, I, J);
+  if (may_split) yp_plan_splits(&p, steps, 256);
+  return p;
+}
+static inline int yp_plan_waves_i(const yp_tile_plan& p) { return p.shape == YP_TILE_S ? 4 : 2; }
+
+// Two products that share a launch, and so a shape: the larger one's.  Each splits for half of the card.
+static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I2, int64_t J2, int64_t steps2, yp_tile_plan* p1, yp_tile_plan* p2) {
+  const int64_t tl = ((I1 + 255) / 256) * ((J1 + 255) / 256) + ((I2 + 255) / 256) * ((J2 + 255) / 256);
+  const int shape = J1 <= 64 && J2 <= 64 ? YP_TILE_S : tl >= 192 ? YP_TILE_L : YP_TILE_M;
+  *p1 = yp_plan_shape(shape, I1, J1);
+  *p2 = yp_plan_shape(shape, I2, J2);
+  yp_plan_splits(p1, steps1, 128);
+  yp_plan_splits(p2, steps2, 128);
 }
 
 #ifdef __HIPCC__
+static inline yp_gemm yp_with_plan(yp_gemm g, const yp_tile_plan& p) { g.tiles_i = p.tiles_i; g.tiles_j = p.tiles_j; g.splits = p.splits; return g; }
+static inline int64_t yp_plan_workgroups(const yp_tile_plan& p) { return (int64_t)p.tiles_i * p.tiles_j * p.splits; }
+
 template <int TYPE, class Epi>
-static hipError_t yp_launch_gemm(const yp_tile_plan& p, yp_gemm g, const Epi& epi, hipStream_t st) {
-  g.tiles_i = p.tiles_i; g.tiles_j = p.tiles_j; g.splits = p.splits;
-  const dim3 grid((unsigned)((int64_t)p.tiles_i * p.tiles_j * p.splits));
-  if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, 256, 256, 2, 2, 1, Epi>), grid, dim3(256), 0, st, g, epi);
-  else if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, 128, 128, 2, 2, 2, Epi>), grid, dim3(256), 0, st, g, epi);
-  else hipLaunchKernelGGL((yp_gemm_kernel<TYPE, 128, 64, 4, 1, 3, Epi>), grid, dim3(256), 0, st, g, epi);
+static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const Epi& epi, hipStream_t st) {
+  const yp_gemm g = yp_with_plan(g0, p);
+  const dim3 grid((unsigned)yp_plan_workgroups(p));
+  if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
+  else if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
+  else hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_S, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
+  return hipGetLastError();
+}
+
+// the gradient products: the first reads both operands by k, the second A by k and B by rows
+template <int TYPE, class Epi>
+static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const Epi& e1, const yp_tile_plan& p2, const yp_gemm& g2, const Epi& e2, hipStream_t st) {
+  const yp_gemm a = yp_with_plan(g1, p1), b = yp_with_plan(g2, p2);
+  const int n1 = (int)yp_plan_workgroups(p1);
+  const dim3 grid((unsigned)(n1 + yp_plan_workgroups(p2)));
+  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
+  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
+  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_S, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
   return hipGetLastError();
 }
 
@@ -68,49 +98,20 @@ __device__ __forceinline__ void yp_store4(void* p, int64_t i, const yp_f4 v, int
 struct yp_epi_store {
   void* out;
   int64_t ld;             // elements
-  int vec;                // ld (for part: I) and out are aligned to four elements
+  int vec, part_vec;      // rows of out / of part are multiples of 16 bytes
   const float* scale;     // device scalar, null = 1
   float* part;
   int add;
-  template <int TYPE, int BM, int BN, bool VEC, bool PART, int MI, int NJ, class Acc>
-  __device__ __forceinline__ void put(Acc (&acc)[MI][NJ], void* to, int64_t ldo, int I, int J, int ib, int jb, float sc) const {
-#pragma unroll
-    for (int n = 0; n < NJ; ++n) {
-      if (jb + yp_frag_at<BN, NJ>(n) < J) {
-        const int64_t row = (int64_t)(jb + yp_frag_at<BN, NJ>(n)) * ldo + ib;
-#pragma unroll
-        for (int m = 0; m < MI; ++m) {
-          const int di = yp_frag_at<BM, MI>(m), left = I - ib - di;
-          if (left > 0) {
-            yp_f4 v = acc[m][n];
-            if (PART) {
-              if (add) {
-                const float* const at = reinterpret_cast<const float*>(to) + row + di;
-                if (VEC && left >= 4) v = v + *reinterpret_cast<const yp_f4*>(at);
-                else
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) if (r < left) v[r] += at[r];
-              }
-              yp_store4<YP_T_F32, VEC>(to, row + di, v, left);
-            } else {
-              yp_store4<TYPE, VEC>(to, row + di, v * sc, left);
-            }
-          }
-        }
-      }
-    }
-  }
-  template <int TYPE, int BM, int BN, int WI, int WJ, int MI, int NJ, class Acc>
-  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], int ti, int tj, int split, int wi, int wj, int lane) const {
-    const int ib = ti * BM + wi * (BM / 2 / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / 2 / WJ) + (lane & 15);
+  template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
+  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], const yp_place& at) const {
     if (part) {
-      float* const to = part + (int64_t)split * g.J * g.I;
-      if (vec) put<TYPE, BM, BN, true, true>(acc, to, g.I, g.I, g.J, ib, jb, 1.0f);
-      else put<TYPE, BM, BN, false, true>(acc, to, g.I, g.I, g.J, ib, jb, 1.0f);
+      float* const to = part + (int64_t)at.split * g.J * g.I;
+      auto val = [&](int m, int n) { return acc[m][n]; };
+      if (add) yp_put_tile<YP_T_F32, SHAPE, true, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
+      else yp_put_tile<YP_T_F32, SHAPE, false, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
     } else {
       const float sc = scale ? *scale : 1.0f;
-      if (vec) put<TYPE, BM, BN, true, false>(acc, out, ld, g.I, g.J, ib, jb, sc);
-      else put<TYPE, BM, BN, false, false>(acc, out, ld, g.I, g.J, ib, jb, sc);
+      yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, out, ld, g.I, g.J, vec != 0, [&](int m, int n) { return acc[m][n] * sc; });
     }
   }
 };

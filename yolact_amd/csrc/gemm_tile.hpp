@@ -1,15 +1,19 @@
 // Matrix-core tile engine of the prediction-head operators (gfx950).
 //
-//   C[j][i] = sum_k A[i][k] * B[j][k]        i < I (contiguous in the output), j < J
+//   C[j][i] = sum_k A(i, k) * B(j, k)        i < I (contiguous in the output), j < J
 //
-// Both operands are rows of K contiguous elements, so a step of k is always 128 BYTES of a row - 64 bf16 / f16, 32 f32 or
-// 128 int8, a whole cache line - and one body serves every type: the global loads, the LDS image and the fragment
-// addresses only know bytes.  K is a multiple of 128 bytes (callers pad with zeros), rows start on 16-byte boundaries.
+// An operand is either rows of K contiguous elements ("by rows": [I][K]) or K rows of its elements ("by k": [K][I]),
+// chosen at compile time, so that the gradient products read what the other products read and wrote, without transposed
+// copies.  A step of k is always 128 BYTES of elements - 64 bf16 / f16, 32 f32 or 128 int8 - and the loads and the LDS
+// image only know bytes.  By rows, K is a multiple of 128 bytes (callers pad with zeros); by k, rows of k past the end
+// read the last one again, and the other operand is zero there.  Rows start on 16-byte boundaries.
 //
-// LDS image: two buffers, one step each.  Row r of a buffer is 8 chunks of 16 bytes; chunk c sits at slot c ^ (r & 7), so
-// that the 8 rows a fragment read touches at a time fall into different banks (no conflicts counted).  It is filled by
-// direct global -> LDS loads (16 bytes a lane, 8 rows a wave instruction), whose LDS side is fixed to lane order: the
-// exclusive-or is applied to the global side.
+// LDS image: two buffers of one step; the halves of each side lie apart.  By rows, a row is 8 chunks of 16 bytes and chunk
+// c sits at slot c ^ (r & 7), so that the 8 rows a fragment read touches at a time fall into different banks (no conflicts
+// counted).  By k, a row of k is the half side's elements; its chunks are exclusive-ored by a function of k that spreads
+// the rows of k one transposing read (16 bit) or four word reads (f32) touch.  The image is filled by direct global -> LDS
+// loads (16 bytes a lane, 1024 a wave instruction), whose LDS side is fixed to lane order: the exclusive-or is applied to
+// the global side.
 //
 // A lane of a 16 x 16 fragment holds row (lane & 15) and 16 bytes of k at chunk (lane >> 4) (+ 4 for the second half
 // of the step); f32 feeds its 4 elements to 4 matrix instructions - which k goes to which instruction does not
@@ -19,6 +23,7 @@
 
 #include "common.hpp"
 
+enum { YP_TILE_L = 0, YP_TILE_M = 1, YP_TILE_S = 2 };
 enum { YP_T_F32 = YP_F32, YP_T_BF16 = YP_BF16, YP_T_F16 = YP_F16, YP_T_I8 = 3 };
 
 typedef float yp_f4 __attribute__((ext_vector_type(4)));
@@ -37,11 +42,12 @@ template <> struct yp_type<YP_T_I8> { typedef signed char elem; typedef yp_i4 fr
 static inline int64_t yp_pad_k(int64_t k, int bytes) { return (k * bytes + YP_TILE_KB - 1) / YP_TILE_KB * YP_TILE_KB; }   // in bytes
 
 struct yp_gemm {
-  const char* a;      // [I] rows of lda bytes
-  const char* b;      // [J] rows of ldb bytes
-  int64_t lda, ldb;
-  int I, J;           // rows of a / b that exist (tiles past them read the last row again)
-  int steps;          // K / YP_TILE_KB
+  const char* a;
+  const char* b;
+  int64_t lda, ldb;   // bytes between rows (of I / J elements' k, or of k)
+  int I, J;           // rows of the result's axes that exist (tiles past them read the last one again)
+  int K;              // by k: rows of k that exist
+  int steps;          // steps of 128 bytes of k
   int splits;         // the steps are dealt to this many workgroups per tile (epilogues that take a split only)
   int tiles_i, tiles_j;
 };
@@ -119,57 +125,138 @@ __device__ __forceinline__ void yp_tile_of(const yp_gemm& g, int wg, int nwg, in
   tj = j0 + p - ti * h;
 }
 
-// BM x BN tile, WI x WJ waves, each (BM / WI) x (BN / WJ).
-//
+// One operand of a tile: SIDE rows (of I or J), shared by WAVES waves for the loads and by W of them for the fragments.
+template <int TYPE, int SIDE, int WAVES, int W, bool BY_K>
+struct yp_side {
+  typedef typename yp_type<TYPE>::frag frag;
+  static constexpr int B = yp_type<TYPE>::bytes;
+  static constexpr int P = SIDE / 16 / WAVES;          // a wave's loads of one half
+  static constexpr int FH = SIDE / 32 / W;             // a wave's fragments in one half
+  static constexpr int HALF = SIDE * (YP_TILE_KB / 2); // bytes of a half in LDS
+  static constexpr int KR = YP_TILE_KB / B;            // elements of k per step
+  static constexpr int HB = SIDE / 2 * B;              // by k: bytes of a row of k
+  static constexpr int CH = HB / 16;                   //       its chunks
+  static_assert(P * WAVES * 16 == SIDE, "every wave issues as many loads: the waits count them");
+
+  const char* base;
+  int64_t stride;          // bytes from step to step
+  uint32_t off[2][P];      // this lane's source offsets
+  uint32_t ld, colmax;     // by k
+  int K;
+  uint32_t lds;            // LDS address of the first half's first load of this wave
+  int fbase;               // this lane's first fragment, relative to the half
+
+  static __device__ __forceinline__ int swizzle(int k) {
+    if (B == 4) return HB >= 256 ? 4 * ((k >> 2) & 3) : 4 * ((k >> 2) & 1);
+    if (HB == 256) return 2 * ((k & 3) | ((k >> 3) & 1) << 2);
+    if (HB == 128) return 2 * (((k >> 1) & 1) | ((k >> 3) & 1) << 1);
+    return 2 * ((k >> 3) & 1);
+  }
+  // rows past the end read the last row: in bounds, and their results are dropped (a tile may lie past the end altogether)
+  __device__ __forceinline__ void init(const char* p, int64_t row_bytes, int first, int count, int krows, uint32_t lds_at, int wave, int w, int lane) {
+    lds = lds_at + (uint32_t)(wave * P) * 1024u;
+    if constexpr (!BY_K) {
+      const int f = min(first, count - 1);
+      base = p + (int64_t)f * row_bytes;
+      stride = YP_TILE_KB;
+      const uint32_t col = (uint32_t)(((lane & 7) ^ (lane >> 3)) * 16);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+          off[x][u] = (uint32_t)min(x * (SIDE / 2) + (wave * P + u) * 8 + (lane >> 3), count - 1 - f) * (uint32_t)row_bytes + col;
+      fbase = (w * (SIDE / 2 / W) + (lane & 15)) * YP_TILE_KB + (((lane >> 4) ^ (lane & 7)) * 16);
+    } else {
+      const int64_t c0 = min((int64_t)first * B, row_bytes - 16);
+      base = p + c0;
+      stride = (int64_t)KR * row_bytes;
+      ld = (uint32_t)row_bytes;
+      K = krows;
+      colmax = (uint32_t)min(row_bytes - 16 - c0, (int64_t)SIDE * B);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+          const int k = (wave * P + u) * (64 / CH) + lane / CH;
+          off[x][u] = (uint32_t)k * ld + min((uint32_t)(x * HB + ((lane % CH) ^ swizzle(k)) * 16), colmax);
+        }
+      const int t = lane & 15, g = lane >> 4;
+      if (B == 4) fbase = g * 4 * HB + (((w * (HB / W / 16) + (t >> 2)) ^ swizzle(g * 4)) * 16) + (t & 3) * 4;
+      else fbase = (g * 8 + (t >> 2)) * HB + (((w * (HB / W / 16) + ((t & 3) >> 1)) ^ swizzle(g * 8 + (t >> 2))) * 16) + (t & 1) * 8;
+    }
+  }
+  // load u of half x of step k, into a buffer `at` bytes into the LDS
+  __device__ __forceinline__ void load(int at, int k, int x, int u) const {
+    const uint32_t to = lds + (uint32_t)(at + x * HALF + u * 1024);
+    if constexpr (!BY_K) yp_load_lds16(base + k * stride, off[x][u], to);
+    else yp_load_lds16(base + k * stride, min(off[x][u], (uint32_t)(min(K - k * KR, KR) - 1) * ld + colmax), to);
+  }
+  // fragment f of half x, half step q
+  __device__ __forceinline__ frag read(const char* buf, int x, int f, int q) const {
+    if constexpr (!BY_K) {
+      return *reinterpret_cast<const frag*>(buf + x * HALF + ((fbase ^ (q * 64)) + f * 16 * YP_TILE_KB));
+    } else if constexpr (B == 4) {
+      const char* const p = buf + x * HALF + (fbase ^ (f * 64)) + q * 16 * HB;
+      frag r;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r[u] = *reinterpret_cast<const float*>(p + u * HB);
+      return r;
+    } else {
+      // 16 lanes read 4 rows of k x 16 elements and get them transposed: 4 consecutive k of one element each
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      const char* const p = buf + x * HALF + (fbase ^ (f * 32)) + q * 32 * HB;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p));
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 4 * HB));
+      return __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// The tile shapes: BM x BN by WI x WJ waves, each (BM / WI) x (BN / WJ).
+template <int SHAPE> struct yp_shape;
+template <> struct yp_shape<YP_TILE_L> { static constexpr int BM = 256, BN = 256, WI = 2, WJ = 2, WPS = 1; };
+template <> struct yp_shape<YP_TILE_M> { static constexpr int BM = 128, BN = 128, WI = 2, WJ = 2, WPS = 2; };
+template <> struct yp_shape<YP_TILE_S> { static constexpr int BM = 128, BN = 64, WI = 4, WJ = 1, WPS = 3; };
+template <int SHAPE> constexpr int yp_lds_bytes = 2 * (yp_shape<SHAPE>::BM + yp_shape<SHAPE>::BN) * YP_TILE_KB;
+
+// What an epilogue knows about its place.
+struct yp_place {
+  int ti, tj, split;   // tile, part of the k axis
+  int wi, wj, lane;
+  char* lds;           // all of the tile's LDS, after yp_arrive<0>
+};
+
 // A wave's share is four quadrants, A0 and A1 by B0 and B1, half of its rows in each half of the tile.  A step is four
 // phases of products, and each phase reads from LDS the fragments of the next:
 //   p0  A0 B0, reads B1     p1  A0 B1, reads A1     p2  A1 B0, reads A0 of the next step     p3  A1 B1, reads its B0
 // so every fragment has one set of registers, and half of a buffer is free half a step before the other: the loads of
 // step s + 2 go into the buffer of step s in two groups, A0 B0 in p0 and p1 of s, B1 A1 in p2 and p3, each group a step
 // and a half before it is read.  (With the whole buffer loaded at once, half a step to a step before: 1057 TFLOP/s.  With
-// more stages of 64 bytes of k, every cache line fetched twice: 985.  bf16, 16384 x 8192 x 4096.)
-template <int TYPE, int BM, int BN, int WI, int WJ, int WAVES_PER_SIMD, class Epi>
-__global__ __launch_bounds__(WI * WJ * 64, WAVES_PER_SIMD) void yp_gemm_kernel(const yp_gemm g, const Epi epi) {
+// more stages of 64 bytes of k, every cache line fetched twice: 985.  This: 1257.  bf16, 16384 x 8192 x 4096.)
+template <int TYPE, int SHAPE, bool A_BY_K, bool B_BY_K, class Epi>
+__device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, int wg, int nwg, char* lds) {
   typedef typename yp_type<TYPE>::frag frag;
   typedef typename yp_type<TYPE>::acc accv;
-  constexpr int WAVES = WI * WJ, MI = BM / WI / 16, NJ = BN / WJ / 16, MH = MI / 2, NH = NJ / 2;
-  constexpr int PA = BM / 16 / WAVES, PB = BN / 16 / WAVES;   // a wave's loads of half of A, of half of B (8 rows each)
-  static_assert(PA * WAVES * 16 == BM && PB * WAVES * 16 == BN, "every wave issues as many loads: the waits count them");
+  typedef yp_shape<SHAPE> S;
+  constexpr int BM = S::BM, BN = S::BN, WI = S::WI, WJ = S::WJ, WAVES = WI * WJ;
+  constexpr int MI = BM / WI / 16, NJ = BN / WJ / 16, MH = MI / 2, NH = NJ / 2;
   constexpr int BUF = (BM + BN) * YP_TILE_KB;
   constexpr bool INPLACE = MI * NJ * 4 == 256;
-  __shared__ __align__(1024) char lds[2 * BUF];
-  const int lane = (int)threadIdx.x & 63;
+  yp_place at;
+  at.lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  int ti, tj, split;
-  yp_tile_of(g, (int)blockIdx.x, (int)gridDim.x, ti, tj, split);
-  const int i0 = ti * BM, j0 = tj * BN;
-  const int k0 = (int)((int64_t)g.steps * split / g.splits), k1 = (int)((int64_t)g.steps * (split + 1) / g.splits);
-
-  // this lane's source offsets (rows past the end read the last row: in bounds, and their results are dropped; a tile
-  // may lie past the end altogether)
-  const int ifirst = min(i0, g.I - 1), jfirst = min(j0, g.J - 1);
-  const char* const abase = g.a + (int64_t)ifirst * g.lda;
-  const char* const bbase = g.b + (int64_t)jfirst * g.ldb;
-  const uint32_t col = (uint32_t)(((lane & 7) ^ (lane >> 3)) * 16);
-  uint32_t aoff[2][PA], boff[2][PB];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-#pragma unroll
-    for (int u = 0; u < PA; ++u)
-      aoff[x][u] = (uint32_t)min(x * (BM / 2) + (wave * PA + u) * 8 + (lane >> 3), g.I - 1 - ifirst) * (uint32_t)g.lda + col;
-#pragma unroll
-    for (int u = 0; u < PB; ++u)
-      boff[x][u] = (uint32_t)min(x * (BN / 2) + (wave * PB + u) * 8 + (lane >> 3), g.J - 1 - jfirst) * (uint32_t)g.ldb + col;
-  }
+  yp_tile_of(g, wg, nwg, at.ti, at.tj, at.split);
+  at.wi = wave % WI; at.wj = wave / WI;
+  at.lds = lds;
+  const int k0 = (int)((int64_t)g.steps * at.split / g.splits), k1 = (int)((int64_t)g.steps * (at.split + 1) / g.splits);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  auto load_a = [&](int buf, int k, int x, int u) {
-    yp_load_lds16(abase + (int64_t)k * YP_TILE_KB, aoff[x][u], lds0 + (uint32_t)(buf * BUF + (x * (BM / 2) + (wave * PA + u) * 8) * YP_TILE_KB));
-  };
-  auto load_b = [&](int buf, int k, int x, int u) {
-    yp_load_lds16(bbase + (int64_t)k * YP_TILE_KB, boff[x][u], lds0 + (uint32_t)(buf * BUF + (BM + x * (BN / 2) + (wave * PB + u) * 8) * YP_TILE_KB));
-  };
+  typedef yp_side<TYPE, BM, WAVES, WI, A_BY_K> SA;
+  typedef yp_side<TYPE, BN, WAVES, WJ, B_BY_K> SB;
+  SA sa;
+  SB sb;
+  sa.init(g.a, g.lda, at.ti * BM, g.I, g.K, lds0, wave, at.wi, at.lane);
+  sb.init(g.b, g.ldb, at.tj * BN, g.J, g.K, lds0 + BM * YP_TILE_KB, wave, at.wj, at.lane);
 
-  const int wi = wave % WI, wj = wave / WI;
   accv acc[MI][NJ];
 #pragma unroll
   for (int m = 0; m < MI; ++m)
@@ -177,15 +264,9 @@ __global__ __launch_bounds__(WI * WJ * 64, WAVES_PER_SIMD) void yp_gemm_kernel(c
     for (int n = 0; n < NJ; ++n) acc[m][n] = accv{0, 0, 0, 0};
   if constexpr (INPLACE) yp_settle<MI, NJ>(acc);
 
-  const int fo = (lane & 15) * YP_TILE_KB + (((lane >> 4) ^ (lane & 7)) * 16);
-  const int fa = wi * (BM / 2 / WI) * YP_TILE_KB + fo, fb = (BM + wj * (BN / 2 / WJ)) * YP_TILE_KB + fo;
   frag a[2][MH][2], b[2][NH][2];          // [half][fragment][half step]
-  auto read_a = [&](int buf, int x, int q) {
-    a[x][q >> 1][q & 1] = *reinterpret_cast<const frag*>(lds + buf * BUF + ((fa ^ ((q & 1) * 64)) + (x * (BM / 2) + (q >> 1) * 16) * YP_TILE_KB));
-  };
-  auto read_b = [&](int buf, int x, int q) {
-    b[x][q >> 1][q & 1] = *reinterpret_cast<const frag*>(lds + buf * BUF + ((fb ^ ((q & 1) * 64)) + (x * (BN / 2) + (q >> 1) * 16) * YP_TILE_KB));
-  };
+  auto read_a = [&](int buf, int x, int q) { a[x][q >> 1][q & 1] = sa.read(lds + buf * BUF, x, q >> 1, q & 1); };
+  auto read_b = [&](int buf, int x, int q) { b[x][q >> 1][q & 1] = sb.read(lds + buf * BUF + BM * YP_TILE_KB, x, q >> 1, q & 1); };
   typedef yp_const<0> E0; typedef yp_const<1> E1; typedef yp_const<2> E2;
 
   // products of half X of A and half Y of B; meanwhile reads half RX of A (RD = 1) or of B (RD = 2) in rbuf, and loads
@@ -193,7 +274,7 @@ __global__ __launch_bounds__(WI * WJ * 64, WAVES_PER_SIMD) void yp_gemm_kernel(c
   auto phase = [&](auto X, auto Y, auto RD, auto RX, int rbuf, auto LD, auto LX, int lbuf, int lk) {
     constexpr int x = decltype(X)::value, y = decltype(Y)::value, rdk = decltype(RD)::value, rx = decltype(RX)::value;
     constexpr int ldk = decltype(LD)::value, lx = decltype(LX)::value;
-    constexpr int G = 2 * MH, RN = rdk == 1 ? 2 * MH : rdk == 2 ? 2 * NH : 0, LN = ldk == 1 ? PA : ldk == 2 ? PB : 0;
+    constexpr int G = 2 * MH, RN = rdk == 1 ? 2 * MH : rdk == 2 ? 2 * NH : 0, LN = ldk == 1 ? SA::P : ldk == 2 ? SB::P : 0;
     int rd = 0, ld = 0;
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) {
@@ -205,8 +286,8 @@ __global__ __launch_bounds__(WI * WJ * 64, WAVES_PER_SIMD) void yp_gemm_kernel(c
       }
 #pragma unroll
       for (; ld * G < (gi + 1) * LN; ++ld) {
-        if constexpr (ldk == 1) load_a(lbuf, lk, lx, ld);
-        else if constexpr (ldk == 2) load_b(lbuf, lk, lx, ld);
+        if constexpr (ldk == 1) sa.load(lbuf * BUF, lk, lx, ld);
+        else if constexpr (ldk == 2) sb.load(lbuf * BUF, lk, lx, ld);
       }
       if constexpr (INPLACE) {
 #pragma unroll
@@ -230,17 +311,17 @@ __global__ __launch_bounds__(WI * WJ * 64, WAVES_PER_SIMD) void yp_gemm_kernel(c
     const int last = k1 - 1;
     // past the last step the last one is loaded again: the number of loads in flight, which the waits count, is always
     // the same
-    constexpr int GROUP = PA + PB;
+    constexpr int GROUP = SA::P + SB::P;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int u = 0; u < PA; ++u) load_a(s, min(k0 + s, last), 0, u);
+      for (int u = 0; u < SA::P; ++u) sa.load(s * BUF, min(k0 + s, last), 0, u);
 #pragma unroll
-      for (int u = 0; u < PB; ++u) load_b(s, min(k0 + s, last), 0, u);
+      for (int u = 0; u < SB::P; ++u) sb.load(s * BUF, min(k0 + s, last), 0, u);
 #pragma unroll
-      for (int u = 0; u < PB; ++u) load_b(s, min(k0 + s, last), 1, u);
+      for (int u = 0; u < SB::P; ++u) sb.load(s * BUF, min(k0 + s, last), 1, u);
 #pragma unroll
-      for (int u = 0; u < PA; ++u) load_a(s, min(k0 + s, last), 1, u);
+      for (int u = 0; u < SA::P; ++u) sa.load(s * BUF, min(k0 + s, last), 1, u);
     }
     yp_arrive<3 * GROUP>();
 #pragma unroll
@@ -262,9 +343,88 @@ __global__ __launch_bounds__(WI * WJ * 64, WAVES_PER_SIMD) void yp_gemm_kernel(c
     phase(E0{}, E1{}, E1{}, E1{}, buf, E0{}, E0{}, 0, 0);
     phase(E1{}, E0{}, E0{}, E0{}, 0, E0{}, E0{}, 0, 0);
     phase(E1{}, E1{}, E0{}, E0{}, 0, E0{}, E0{}, 0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the surplus loads: nothing may arrive in LDS after the workgroup has left it
   }
   if constexpr (INPLACE) yp_settle<MI, NJ>(acc);
-  epi.template apply<TYPE, BM, BN, WI, WJ, MI, NJ>(g, acc, ti, tj, split, wi, wj, lane);
+  yp_arrive<0>();    // the surplus loads of every wave have landed: the LDS is the epilogue's
+  epi.template apply<TYPE, SHAPE, MI, NJ>(g, acc, at);
+}
+
+template <int TYPE, int SHAPE, bool A_BY_K, bool B_BY_K, class Epi>
+__global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_gemm_kernel(const yp_gemm g, const Epi epi) {
+  __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
+  yp_gemm_tile<TYPE, SHAPE, A_BY_K, B_BY_K>(g, epi, (int)blockIdx.x, (int)gridDim.x, lds);
+}
+
+// Two independent products of one tile shape in one launch: the first `n1` workgroups are the first one's.
+template <int TYPE, int SHAPE, bool A1, bool B1, bool A2, bool B2, class Epi>
+__global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_two_gemms_kernel(const yp_gemm g1, const Epi e1, int n1, const yp_gemm g2, const Epi e2) {
+  __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
+  if ((int)blockIdx.x < n1) yp_gemm_tile<TYPE, SHAPE, A1, B1>(g1, e1, (int)blockIdx.x, n1, lds);
+  else yp_gemm_tile<TYPE, SHAPE, A2, B2>(g2, e2, (int)blockIdx.x - n1, (int)gridDim.x - n1, lds);
+}
+
+// Where an epilogue's fragment (0, 0), element 0 lies: i and j of this lane.
+template <int SHAPE>
+__device__ __forceinline__ void yp_origin(const yp_place& at, int& i, int& j) {
+  typedef yp_shape<SHAPE> S;
+  i = at.ti * S::BM + at.wi * (S::BM / 2 / S::WI) + (at.lane >> 4) * 4;
+  j = at.tj * S::BN + at.wj * (S::BN / 2 / S::WJ) + (at.lane & 15);
+}
+
+// Stores a tile, val(m, n) = the four values of a lane's fragment, as rows of out ([j][i], `ld` elements apart, i < I,
+// j < J), or adds them to what is there: through LDS, so that the stores are whole lines.  Stored from the fragments
+// directly - 16 rows of 32 bytes an instruction - 134 MB took 60 us, with this 26 (8192 x 8192 bf16).
+// vec: out and ld are multiples of 16 bytes.
+template <int OUT, int SHAPE, bool ADD, int MI, int NJ, class Val>
+__device__ __forceinline__ void yp_put_tile(const yp_place& at, void* out, int64_t ld, int I, int J, bool vec, const Val& val) {
+  typedef yp_shape<SHAPE> S;
+  typedef typename yp_type<OUT>::elem elem;
+  constexpr int OB = yp_type<OUT>::bytes, E = 16 / OB, CPR = S::BM / E;      // elements per chunk, chunks per row
+  constexpr int PASSES = S::BM * S::BN * OB > yp_lds_bytes<SHAPE> ? 2 : 1;
+  typedef elem e4 __attribute__((ext_vector_type(4)));
+  typedef elem eE __attribute__((ext_vector_type(E)));
+  const int tid = (int)threadIdx.x;
+  const int iw = at.wi * (S::BM / 2 / S::WI) + (at.lane >> 4) * 4;
+#pragma unroll
+  for (int pass = 0; pass < PASSES; ++pass) {
+    if (pass) yp_arrive<0>();
+#pragma unroll
+    for (int n = pass * NJ / PASSES; n < (pass + 1) * NJ / PASSES; ++n) {
+      const int jl = at.wj * (S::BN / 2 / S::WJ) + (at.lane & 15) + yp_frag_at<S::BN, NJ>(n) - pass * (S::BN / 2);
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int byte = (iw + yp_frag_at<S::BM, MI>(m)) * OB;
+        const yp_f4 v = val(m, n);
+        *reinterpret_cast<e4*>(at.lds + jl * (S::BM * OB) + (((byte >> 4) ^ (at.lane & 15)) << 4) + (byte & 15)) =
+            e4{(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
+      }
+    }
+    yp_arrive<0>();
+    constexpr int ROWS = S::BN / PASSES;
+    const int j0 = at.tj * S::BN + pass * ROWS, i0 = at.ti * S::BM;
+    if (vec) {
+      const int c = tid % CPR, i = i0 + c * E;
+      for (int r = tid / CPR; r < ROWS && j0 + r < J; r += 256 / CPR) {
+        if (i >= I) break;
+        eE v = *reinterpret_cast<const eE*>(at.lds + r * (S::BM * OB) + ((c ^ (r & 15)) << 4));
+        elem* const to = reinterpret_cast<elem*>(out) + (int64_t)(j0 + r) * ld + i;
+        if (i + E <= I) {
+          if (ADD) v = v + *reinterpret_cast<const eE*>(to);
+          *reinterpret_cast<eE*>(to) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) if (i + e < I) to[e] = ADD ? (elem)(v[e] + to[e]) : v[e];
+        }
+      }
+    } else {   // odd rows: element by element, consecutive lanes to consecutive elements
+      const int c = tid % S::BM, i = i0 + c;
+      if (i < I)
+        for (int r = tid / S::BM; r < ROWS && j0 + r < J; r += 256 / S::BM) {
+          const elem v = *reinterpret_cast<const elem*>(at.lds + r * (S::BM * OB) + (((c / E) ^ (r & 15)) << 4) + (c % E) * OB);
+          elem* const to = reinterpret_cast<elem*>(out) + (int64_t)(j0 + r) * ld + i;
+          *to = ADD ? (elem)(v + *to) : v;
+        }
+    }
+  }
 }
 #endif  // __HIPCC__

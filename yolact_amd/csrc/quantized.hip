@@ -114,38 +114,29 @@ struct yp_epi_scaled {
   const float *x_scale, *w_scale, *bias;
   void* out;
   int vec;
-  template <int TYPE, int BM, int BN, int WI, int WJ, int MI, int NJ, class Acc>
-  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], int ti, int tj, int, int wi, int wj, int lane) const {
-    const int ib = ti * BM + wi * (BM / 2 / WI) + (lane >> 4) * 4, jb = tj * BN + wj * (BN / 2 / WJ) + (lane & 15);
-    if (vec) put<BM, BN, true>(g, acc, ib, jb);
-    else put<BM, BN, false>(g, acc, ib, jb);
-  }
-  template <int BM, int BN, bool VEC, int MI, int NJ, class Acc>
-  __device__ __forceinline__ void put(const yp_gemm& g, Acc (&acc)[MI][NJ], int ib, int jb) const {
+  template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
+  __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], const yp_place& at) const {
+    typedef yp_shape<SHAPE> S;
+    int i0, j0;
+    yp_origin<SHAPE>(at, i0, j0);
     float sx[NJ];
 #pragma unroll
-    for (int n = 0; n < NJ; ++n) sx[n] = jb + yp_frag_at<BN, NJ>(n) < g.J ? x_scale[jb + yp_frag_at<BN, NJ>(n)] : 0.0f;
+    for (int n = 0; n < NJ; ++n) { const int j = j0 + yp_frag_at<S::BN, NJ>(n); sx[n] = j < g.J ? x_scale[j] : 0.0f; }
+    yp_f4 sw[MI], b[MI];
 #pragma unroll
-    for (int m = 0; m < MI; ++m) {
-      const int i = ib + yp_frag_at<BM, MI>(m), left = g.I - i;
-      if (left > 0) {
-        yp_f4 sw, b;
+    for (int m = 0; m < MI; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sw[r] = r < left ? w_scale[i + r] : 0.0f;
-          b[r] = bias && r < left ? bias[i + r] : 0.0f;
-        }
-#pragma unroll
-        for (int n = 0; n < NJ; ++n) {
-          if (jb + yp_frag_at<BN, NJ>(n) < g.J) {
-            yp_f4 y;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = __builtin_fmaf((float)acc[m][n][r] * sx[n], sw[r], b[r]);
-            yp_store4<OUT, VEC>(out, (int64_t)(jb + yp_frag_at<BN, NJ>(n)) * g.I + i, y, left);
-          }
-        }
+      for (int r = 0; r < 4; ++r) {
+        const int i = i0 + yp_frag_at<S::BM, MI>(m) + r;
+        sw[m][r] = i < g.I ? w_scale[i] : 0.0f;
+        b[m][r] = bias && i < g.I ? bias[i] : 0.0f;
       }
-    }
+    yp_put_tile<OUT, SHAPE, false, MI, NJ>(at, out, g.I, g.I, g.J, vec != 0, [&](int m, int n) {
+      yp_f4 y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = __builtin_fmaf((float)acc[m][n][r] * sx[n], sw[m][r], b[m][r]);
+      return y;
+    });
   }
 };
 
@@ -153,7 +144,7 @@ template <int OUT>
 static hipError_t linear_t(const yp_gemm& g, const float* x_scale, const float* w_scale, const float* bias, void* out, hipStream_t st) {
   yp_epi_scaled<OUT> e;
   e.x_scale = x_scale; e.w_scale = w_scale; e.bias = bias; e.out = out;
-  e.vec = g.I % 4 == 0 && ((uintptr_t)out & 15) == 0;
+  e.vec = (int64_t)g.I * yp_type<OUT>::bytes % 16 == 0 && ((uintptr_t)out & 15) == 0;
   return yp_launch_gemm<YP_T_I8>(yp_plan_tiles(g.I, g.J, g.steps, false), g, e, st);
 }
 
