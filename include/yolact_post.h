@@ -304,7 +304,7 @@ enum { YP_F32 = 0, YP_BF16 = 1, YP_F16 = 2, YP_INT8 = 3 };
  * value for every row (grad_stride 0); with count != NULL the values are divided by max(*count, 1) (the mean: pass
  * reduced + 2).  grad_bias is NULL without a bias.  Products accumulate in float32, gradients are rounded once; dz =
  * grad (softmax - onehot) is rounded to dtype before its products.  Fixed order of sums, no float atomics.
- * 0 <= n <= 2^20, 1 <= v <= 2^24, 1 <= d <= 65536; contiguous tensors, aligned to their elements.  All pointers on the
+ * 0 <= n <= 2^20, 1 <= v <= 2^24, n v <= 2^38, 1 <= d <= 65536; contiguous tensors, aligned to their elements.  All pointers on the
  * device; asynchronous on hip_stream; allocates nothing, may be captured. */
 int64_t yp_class_loss_workspace(int32_t n, int32_t v, int32_t d, int32_t dtype, int32_t has_bias, int32_t backward);
 int yp_class_loss(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
@@ -319,7 +319,8 @@ int yp_class_loss_backward(int32_t device_id, int32_t n, int32_t v, int32_t d, i
  *   scale[r] = max_k |x[r,k]| / 127     q[r,k] = x[r,k] / scale[r] to the nearest integer, ties to even (0 for a row of
  *   zeros)                              out[i,j] = (sum_k xq[i,k] wq[j,k]) x_scale[i] w_scale[j] + bias[j]
  * q rows are yp_quantized_row_bytes(k) bytes apart (k padded to 128), the padding is zero; 16-byte aligned.  A row that
- * holds an infinity or NaN gets the scale NaN, so its results are NaN.  1 <= k <= 131072 (the integer sums fit 32 bits).
+ * holds an infinity or NaN gets the scale NaN, so its results are NaN.  1 <= k <= 131072 (the integer sums fit 32 bits);
+ * rows v <= 2^37.
  *   yp_quantize_rows     x [rows,k] contiguous, dtype YP_F32 / YP_BF16 / YP_F16 -> q, scale [rows] float32
  *   yp_quantized_linear  x: dtype YP_INT8 (x = q rows, x_scale their scales) or a float type, x [rows,k] contiguous,
  *                        quantized on the way into workspace (yp_quantized_linear_workspace(rows, k) bytes, 256-byte
@@ -334,7 +335,7 @@ int yp_quantized_linear(int32_t device_id, int32_t rows, int32_t v, int32_t k, i
 
 /* Dropout whose mask is never stored: element i of x (count elements, contiguous) is kept if word i % 4 of
  * Philox4x32-10 (Salmon et al. 2011) under the 64-bit key state[0] at the 64-bit counter state[1] + i / 4 is
- * >= floor(p 2^32), and then y = x / (1 - p); otherwise y = 0, whatever x holds.  0 <= p <= 1.  The backward pass is the
+ * >= floor(p 2^32), and then y = x / (1 - p); otherwise y = 0, whatever x holds.  0 <= p <= 1, 0 <= count <= 2^40.  The backward pass is the
  * same call on the gradient with the same state.  state [2] int64 on the device: a captured call reads it on every
  * replay; advance state[1] by (count + 3) / 4 between uses.  y may be x.  Asynchronous on hip_stream. */
 int yp_dropout(int32_t device_id, int64_t count, int32_t dtype, double p, const int64_t* state, const void* x, void* y, void* hip_stream);

@@ -749,6 +749,7 @@ static int check_class_loss_sizes(const char* who, int n, int v, int d, int dtyp
   if (n < 0 || n > (1 << 20)) return fail(YP_EINVAL, "%s: n must be in [0, 2^20]", who);
   if (v < 1 || v > (1 << 24)) return fail(YP_EINVAL, "%s: v must be in [1, 2^24]", who);
   if (d < 1 || d > 65536) return fail(YP_EINVAL, "%s: d must be in [1, 65536]", who);
+  if ((int64_t)n * v > (1ll << 38)) return fail(YP_EINVAL, "%s: n * v must be at most 2^38", who);   // (workgroups of one launch)
   return YP_OK;
 }
 
@@ -844,7 +845,7 @@ extern "C" int yp_quantized_linear(int32_t device_id, int32_t rows, int32_t v, i
   if (dtype != YP_INT8 && !head_type(dtype)) return fail(YP_EINVAL, "yp_quantized_linear: dtype must be YP_INT8, YP_F32, YP_BF16 or YP_F16");
   if (!head_type(out_dtype)) return fail(YP_EINVAL, "yp_quantized_linear: out_dtype must be YP_F32, YP_BF16 or YP_F16");
   if (v < 1 || v > (1 << 24)) return fail(YP_EINVAL, "yp_quantized_linear: v must be in [1, 2^24]");
-  if (((int64_t)rows + 127) / 128 * (((int64_t)v + 127) / 128) >= (1ll << 30)) return fail(YP_EINVAL, "yp_quantized_linear: rows * v is too large");
+  if (((int64_t)rows + 127) / 128 * (((int64_t)v + 127) / 128) >= (1ll << 23)) return fail(YP_EINVAL, "yp_quantized_linear: rows * v is too large");
   if (rows == 0) return YP_OK;
   if (!x || !wq || !w_scale || !out || (dtype == YP_INT8 ? !x_scale : !workspace)) return fail(YP_EINVAL, "yp_quantized_linear: null argument");
   if (((uintptr_t)wq & 15) != 0 || (dtype == YP_INT8 ? ((uintptr_t)x & 15) != 0 : !elem_aligned(x, dtype)) || !elem_aligned(out, out_dtype) ||
@@ -852,21 +853,14 @@ extern "C" int yp_quantized_linear(int32_t device_id, int32_t rows, int32_t v, i
     return fail(YP_EINVAL, "yp_quantized_linear: a tensor is not aligned (8-bit rows to 16 bytes, the others to their elements)");
   if (((uintptr_t)workspace & 255) != 0) return fail(YP_EINVAL, "yp_quantized_linear: workspace must be 256-byte aligned");
   YP_ON_DEVICE(device_id);
-  const void* xq = x;
-  if (dtype != YP_INT8) {
-    xq = workspace;
-    float* const s = (float*)((char*)workspace + (int64_t)rows * yp_qrow_bytes(k));
-    YP_HIP(yp_launch_quantize_rows(rows, k, dtype, x, workspace, s, (hipStream_t)hip_stream));
-    x_scale = s;
-  }
-  YP_HIP(yp_launch_quantized_linear(rows, v, k, xq, x_scale, wq, w_scale, bias, out, out_dtype, (hipStream_t)hip_stream));
+  YP_HIP(yp_launch_quantized_linear(rows, v, k, dtype, x, x_scale, wq, w_scale, bias, workspace, out, out_dtype, (hipStream_t)hip_stream));
   return YP_OK;
 }
 
 extern "C" int yp_dropout(int32_t device_id, int64_t count, int32_t dtype, double p, const int64_t* state, const void* x, void* y, void* hip_stream) {
   if (!head_type(dtype)) return fail(YP_EINVAL, "yp_dropout: dtype must be YP_F32, YP_BF16 or YP_F16");
   if (!(p >= 0.0 && p <= 1.0)) return fail(YP_EINVAL, "yp_dropout: p must be in [0, 1]");
-  if (count < 0) return fail(YP_EINVAL, "yp_dropout: negative count");
+  if (count < 0 || count > (1ll << 40)) return fail(YP_EINVAL, "yp_dropout: count must be in [0, 2^40]");
   if (count == 0) return YP_OK;
   if (!state || !x || !y) return fail(YP_EINVAL, "yp_dropout: null argument");
   if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || ((uintptr_t)state & 7) != 0) return fail(YP_EINVAL, "yp_dropout: a tensor is not aligned to its elements");

@@ -9,7 +9,7 @@
 // A row whose label is outside [0, V) has loss NaN and no gradient.
 //
 // Forward: one product on the tile engine whose epilogue reduces a wave's part of the vocabulary to (max, sum exp) per
-// row; a second kernel joins the parts.  2 N V D operations, h and w are read, 8 bytes per row and 64 classes written.
+// row; a second kernel joins the parts.  2 N V D operations, h and w are read, 8 bytes per row and half tile of classes written.
 // Backward, per piece of the vocabulary (so that a piece of dz stays in the Infinity Cache): the product again, with an
 // epilogue that turns z into dz [row][class]; then both gradient products in one launch, which read dz, h and w as they
 // lie ("by k", gemm_tile.hpp): dw's piece is complete, dh adds up over the pieces in f32.
@@ -246,7 +246,6 @@ __device__ __forceinline__ void yp_write_reduced(float* reduced, double sum, dou
   reduced[2] = (float)count;
 }
 
-// Joins the parts of 32 rows per workgroup (8 threads a row), and the rows' losses if they are asked for.
 struct yp_join_args {
   const yp_softmax_part* part;
   int parts;
@@ -257,21 +256,41 @@ struct yp_join_args {
   float* reduced;           // [3], may be null
   double* block_part;       // [blocks][2]
 };
+// Joins the parts of the rows, and the sum of their losses if it is asked for.
+template <int RPB>   // rows per workgroup and turn; YP_CL_THREADS / RPB threads a row
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_join_kernel(const yp_join_args a) {
-  __shared__ float lm[8][32], ls[8][32];
+  constexpr int TPR = YP_CL_THREADS / RPB;
+  __shared__ float lm[TPR][RPB], ls[TPR][RPB];
   __shared__ double red[YP_CL_THREADS / 64];
-  const int x = (int)threadIdx.x & 31, y = (int)threadIdx.x >> 5;
+  const int x = (int)threadIdx.x % RPB, y = (int)threadIdx.x / RPB;
   double loss = 0.0, count = 0.0;
-  for (int n0 = (int)blockIdx.x * 32; n0 < a.N; n0 += (int)gridDim.x * 32) {
+  for (int n0 = (int)blockIdx.x * RPB; n0 < a.N; n0 += (int)gridDim.x * RPB) {
     const int n = n0 + x;
     float m = -INFINITY, s = 0.0f;
-    if (n < a.N)
-      for (int p = y; p < a.parts; p += 8) {
-        const yp_softmax_part v = a.part[(int64_t)p * a.N + n];
+    if (n < a.N) {
+      const yp_softmax_part* const col = a.part + n;
+      int p = y;
+      for (; p + 3 * TPR < a.parts; p += 4 * TPR) {     // four loads in flight
+        yp_softmax_part v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = col[(int64_t)(p + u * TPR) * a.N];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) yp_join(m, s, v[u].m, v[u].s);
+      }
+      for (; p < a.parts; p += TPR) {
+        const yp_softmax_part v = col[(int64_t)p * a.N];
         yp_join(m, s, v.m, v.s);
       }
+    }
     __syncthreads();
     lm[y][x] = m; ls[y][x] = s;
+    if constexpr (TPR > 8) {                            // 8 threads gather the others'
+      __syncthreads();
+      if (y < 8) {
+        for (int u = y + 8; u < TPR; u += 8) yp_join(m, s, lm[u][x], ls[u][x]);
+        lm[y][x] = m; ls[y][x] = s;
+      }
+    }
     __syncthreads();
     if (y == 0 && n < a.N) {
       for (int u = 1; u < 8; ++u) yp_join(m, s, lm[u][x], ls[u][x]);
@@ -323,20 +342,47 @@ __global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, int6
   }
 }
 
-// Up to three arrays, each out[e] = scale * sum over its parts, in the order of the parts
+// Up to three arrays, each out[e] = scale * sum over its parts.  64 elements and 4 waves a workgroup: wave w adds parts
+// w, w + 4, ... in their order, then the four sums are added in theirs.
 struct yp_sum_job { const float* part; int parts; int64_t stride, total; void* out; };
 struct yp_sum_args { yp_sum_job job[3]; int jobs, out_type; const float* scale; };
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_sum_args a) {
+  __shared__ float red[YP_CL_THREADS / 64][64];
+  const int x = (int)threadIdx.x & 63, y = (int)threadIdx.x >> 6;
   const float sc = a.scale ? *a.scale : 1.0f;
+  auto put = [&](void* out, int64_t e, float s) {
+    if (a.out_type == YP_F32) reinterpret_cast<float*>(out)[e] = s;
+    else if (a.out_type == YP_BF16) reinterpret_cast<__bf16*>(out)[e] = (__bf16)s;
+    else reinterpret_cast<_Float16*>(out)[e] = (_Float16)s;
+  };
   for (int j = 0; j < a.jobs; ++j) {
     const yp_sum_job& b = a.job[j];
-    for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < b.total; e += (int64_t)gridDim.x * YP_CL_THREADS) {
+    if (b.parts < 4) {   // (or none: zeros) a thread an element
+      for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < b.total; e += (int64_t)gridDim.x * YP_CL_THREADS) {
+        float s = 0.0f;
+        for (int p = 0; p < b.parts; ++p) s += b.part[(int64_t)p * b.stride + e];
+        put(b.out, e, s * sc);
+      }
+      continue;
+    }
+    for (int64_t e0 = (int64_t)blockIdx.x * 64; e0 < b.total; e0 += (int64_t)gridDim.x * 64) {
+      const int64_t e = e0 + x;
       float s = 0.0f;
-      for (int p = 0; p < b.parts; ++p) s += b.part[(int64_t)p * b.stride + e];
-      s *= sc;
-      if (a.out_type == YP_F32) reinterpret_cast<float*>(b.out)[e] = s;
-      else if (a.out_type == YP_BF16) reinterpret_cast<__bf16*>(b.out)[e] = (__bf16)s;
-      else reinterpret_cast<_Float16*>(b.out)[e] = (_Float16)s;
+      if (e < b.total) {
+        int p = y;
+        for (; p + 12 < b.parts; p += 16) {
+          float v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = b.part[(int64_t)(p + 4 * u) * b.stride + e];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s += v[u];
+        }
+        for (; p < b.parts; p += 4) s += b.part[(int64_t)p * b.stride + e];
+      }
+      __syncthreads();
+      red[y][x] = s;
+      __syncthreads();
+      if (y == 0 && e < b.total) put(b.out, e, (((red[0][x] + red[1][x]) + red[2][x]) + red[3][x]) * sc);
     }
   }
 }
@@ -348,9 +394,12 @@ static inline unsigned blocks_for(int64_t n, int per, int64_t most) { const int6
 
 static hipError_t sum_parts(const yp_sum_args& a, hipStream_t st) {
   int64_t most = 0;
-  for (int j = 0; j < a.jobs; ++j) most = a.job[j].total > most ? a.job[j].total : most;
-  if (most == 0) return hipSuccess;
-  hipLaunchKernelGGL(yp_sum_parts_kernel, dim3(blocks_for(most, YP_CL_THREADS, 8192)), dim3(YP_CL_THREADS), 0, st, a);
+  for (int j = 0; j < a.jobs; ++j) {
+    const int64_t b = (a.job[j].total + 63) / 64 / (a.job[j].parts < 4 ? 4 : 1);
+    most = b > most ? b : most;
+  }
+  if (a.jobs == 0) return hipSuccess;
+  hipLaunchKernelGGL(yp_sum_parts_kernel, dim3(blocks_for(most, 1, 8192)), dim3(YP_CL_THREADS), 0, st, a);
   return hipGetLastError();
 }
 static void add_sum(yp_sum_args& a, const float* part, int parts, int64_t stride, int64_t total, void* out) {
@@ -395,13 +444,13 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   auto take = [&](int64_t bytes) { const int64_t o = off; off = up256(off + bytes); return o; };
   if (copy_fwd) cut_pieces(V, YP_CL_PIECE_BYTES / p.kd, &p.fwd_pieces, &p.fwd_piece);
   else { p.fwd_pieces = 1; p.fwd_piece = (int)V; }
-  p.fwd = yp_plan_tiles(p.fwd_piece, N, p.kd / YP_TILE_KB, false);
-  p.parts = p.fwd.tiles_i * yp_plan_waves_i(p.fwd);
+  p.fwd = yp_plan_tiles(p.fwd_piece, N);
+  p.parts = p.fwd.tiles_i * 2;
   p.o_h = take(copy_fwd ? N * p.kd : 0);
   p.o_w = take(copy_fwd ? p.fwd_piece * p.kd : 0);
   p.o_part = take((int64_t)p.fwd_pieces * p.parts * N * sizeof(yp_softmax_part));
   p.o_picked = take(N * 4);
-  p.o_block = take((N + 31) / 32 * 16);
+  p.o_block = take((N <= 1024 ? (N + 1) / 2 : (N + 31) / 32) * 16);
   p.fwd_total = off;
 
   off = 0;
@@ -411,7 +460,7 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   if (most > YP_CL_PIECE_BYTES / p.kd) most = YP_CL_PIECE_BYTES / p.kd;
   cut_pieces(V, most, &p.pieces, &p.piece);
   p.kv = yp_pad_k(p.piece, b);
-  p.dzp = yp_plan_tiles(p.piece, p.kn, p.kd / YP_TILE_KB, false);
+  p.dzp = yp_plan_tiles(p.piece, p.kn);
   // the two gradient products share a launch and so a tile shape
   yp_plan_two(D, p.piece, p.kn / kr, D, N, p.kv / YP_TILE_KB, &p.dwp, &p.dhp);
   p.o_factor = take(8);
@@ -477,13 +526,21 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
     e.bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
     e.labels = labels; e.first = v0; e.part = part + (int64_t)parts * a.n; e.picked = (float*)(ws + p.o_picked);
     CL_TRY(yp_launch_gemm<TYPE>(tp, g, e, st));
-    parts += tp.tiles_i * yp_plan_waves_i(tp);
+    parts += tp.tiles_i * 2;
   }
   yp_join_args j;
   j.part = part; j.parts = parts; j.picked = (const float*)(ws + p.o_picked); j.labels = labels;
   j.N = a.n; j.losses = a.losses; j.lse = a.lse; j.reduced = a.reduced; j.block_part = (double*)(ws + p.o_block);
-  const int blocks = a.n <= 256 && parts <= 64 ? 1 : (a.n + 31) / 32;   // (one workgroup sums its own losses: a launch less)
-  hipLaunchKernelGGL(yp_join_kernel, dim3(blocks), dim3(YP_CL_THREADS), 0, st, j);
+  // few rows of many parts: 128 threads a row; else 8.  A few rows of few parts are one workgroup's, which sums their losses
+  // itself: a launch less.
+  int blocks;
+  if (a.n <= 1024 && parts > 64) {
+    blocks = (a.n + 1) / 2;
+    hipLaunchKernelGGL(yp_join_kernel<2>, dim3(blocks), dim3(YP_CL_THREADS), 0, st, j);
+  } else {
+    blocks = a.n <= 256 ? 1 : (a.n + 31) / 32;
+    hipLaunchKernelGGL(yp_join_kernel<32>, dim3(blocks), dim3(YP_CL_THREADS), 0, st, j);
+  }
   if (a.reduced && blocks > 1) hipLaunchKernelGGL(yp_reduce_kernel, dim3(1), dim3(YP_CL_THREADS), 0, st, (const double*)j.block_part, blocks, a.reduced);
   return hipGetLastError();
 }

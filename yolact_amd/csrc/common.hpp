@@ -306,6 +306,6 @@ hipError_t yp_launch_class_loss(const yp_class_loss_args& a, hipStream_t st);
 hipError_t yp_launch_class_loss_backward(const yp_class_loss_args& a, hipStream_t st);
 int64_t yp_qrow_bytes(int64_t k);
 hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x, void* q, float* scale, hipStream_t st);
-hipError_t yp_launch_quantized_linear(int rows, int v, int k, const void* xq, const float* x_scale, const void* wq, const float* w_scale,
-                                      const float* bias, void* out, int out_type, hipStream_t st);
+hipError_t yp_launch_quantized_linear(int rows, int v, int k, int x_type, const void* x, const float* x_scale, const void* wq, const float* w_scale,
+                                      const float* bias, void* workspace, void* out, int out_type, hipStream_t st);
 hipError_t yp_launch_dropout(int64_t count, int type, double p, const int64_t* state, const void* x, void* y, hipStream_t st);

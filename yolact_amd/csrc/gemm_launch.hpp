@@ -10,43 +10,53 @@ struct yp_tile_plan {
   int tiles_i, tiles_j, splits;
 };
 
-// L 256 x 256 (4 waves of 128 x 128: 256 rows of fragments read for 128 x 128 results, half of what M reads),
-// M 128 x 128 (4 waves of 64 x 64, two workgroups a CU), S 128 x 64 (4 waves of 32 x 64, three workgroups a CU) for few
-// rows, where only streaming A counts.  L needs about a full round of tiles; below that M's finer cut wins.
+// L 256 x 256 (4 waves of 128 x 128: 256 rows of fragments read for 128 x 128 results), M 128 x 128 (4 waves of 64 x 64,
+// two workgroups a CU), T 64 x 64 (4 waves of 32 x 32, four a CU): the larger, the faster per result once the card is
+// full - 1315, 1088 and about 600 TFLOP/s, bf16 - but a small product leaves most of the card idle with it.
 static inline yp_tile_plan yp_plan_shape(int shape, int64_t I, int64_t J) {
   yp_tile_plan p;
   p.shape = shape;
-  p.bi = shape == YP_TILE_L ? 256 : 128;
-  p.bj = shape == YP_TILE_L ? 256 : (shape == YP_TILE_M ? 128 : 64);
+  p.bi = p.bj = shape == YP_TILE_L ? 256 : shape == YP_TILE_M ? 128 : 64;
   p.tiles_i = (int)((I + p.bi - 1) / p.bi);
   p.tiles_j = (int)((J + p.bj - 1) / p.bj);
   p.splits = 1;
   return p;
 }
-// Few tiles: deal the k axis to more workgroups, up to two for each of `cus` compute units, at least 4 steps each.
-static inline void yp_plan_splits(yp_tile_plan* p, int64_t steps, int cus) {
-  const int64_t tiles = (int64_t)p->tiles_i * p->tiles_j;
-  if (tiles >= cus) return;
-  int64_t s = (2 * cus + tiles - 1) / tiles;
-  if (s > steps / 4) s = steps / 4;
+// Time of `tiles` tiles of a shape, in units of a 64 x 64 tile at the large shape's rate: rounds of what is resident at a
+// time (256 CUs), each as long as the CU's share of them takes.
+static inline int64_t yp_plan_cost(int shape, int64_t tiles) {
+  if (shape == YP_TILE_L) return (tiles + 255) / 256 * 16;
+  if (shape == YP_TILE_M) return tiles <= 256 ? 6 : (tiles + 511) / 512 * 10;
+  return tiles <= 256 ? 2 : tiles <= 512 ? 4 : (tiles + 1023) / 1024 * 8;
+}
+static inline int yp_plan_best(int64_t I1, int64_t J1, int64_t I2, int64_t J2) {   // (J2 = 0: one product)
+  int best = YP_TILE_L;
+  int64_t least = INT64_MAX;
+  for (int s = YP_TILE_L; s <= YP_TILE_T; ++s) {
+    const int64_t e = s == YP_TILE_L ? 256 : s == YP_TILE_M ? 128 : 64;
+    const int64_t c = yp_plan_cost(s, (I1 + e - 1) / e * ((J1 + e - 1) / e) + (I2 + e - 1) / e * ((J2 + e - 1) / e));
+    if (c < least) { least = c; best = s; }
+  }
+  return best;
+}
+static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J) { return yp_plan_shape(yp_plan_best(I, J, 0, 0), I, J); }
+static inline int yp_plan_waves_i(const yp_tile_plan&) { return 2; }
+
+// Few tiles: deal the k axis to more workgroups, until half of the card is busy or a workgroup has 8 steps left.
+static inline void yp_plan_splits(yp_tile_plan* p, int64_t steps) {
+  const int64_t tiles = (int64_t)p->tiles_i * p->tiles_j, fill = p->shape == YP_TILE_L ? 128 : p->shape == YP_TILE_M ? 256 : 512;
+  if (tiles >= fill) return;
+  int64_t s = fill / tiles;
+  if (s > steps / 8) s = steps / 8;
   p->splits = s < 1 ? 1 : (int)s;
 }
-static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps, bool may_split) {
-  const int64_t tl = ((I + 255) / 256) * ((J + 255) / 256);
-  yp_tile_plan p = yp_plan_shape(J <= 64 ? YP_TILE_S : tl >= 192 ? YP_TILE_L : YP_TILE_M, I, J);
-  if (may_split) yp_plan_splits(&p, steps, 256);
-  return p;
-}
-static inline int yp_plan_waves_i(const yp_tile_plan& p) { return p.shape == YP_TILE_S ? 4 : 2; }
-
-// Two products that share a launch, and so a shape: the larger one's.  Each splits for half of the card.
+// Two products that share a launch, and so a shape.
 static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I2, int64_t J2, int64_t steps2, yp_tile_plan* p1, yp_tile_plan* p2) {
-  const int64_t tl = ((I1 + 255) / 256) * ((J1 + 255) / 256) + ((I2 + 255) / 256) * ((J2 + 255) / 256);
-  const int shape = J1 <= 64 && J2 <= 64 ? YP_TILE_S : tl >= 192 ? YP_TILE_L : YP_TILE_M;
+  const int shape = yp_plan_best(I1, J1, I2, J2);
   *p1 = yp_plan_shape(shape, I1, J1);
   *p2 = yp_plan_shape(shape, I2, J2);
-  yp_plan_splits(p1, steps1, 128);
-  yp_plan_splits(p2, steps2, 128);
+  yp_plan_splits(p1, steps1);
+  yp_plan_splits(p2, steps2);
 }
 
 #ifdef __HIPCC__
@@ -59,7 +69,7 @@ static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const
   const dim3 grid((unsigned)yp_plan_workgroups(p));
   if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
   else if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
-  else hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_S, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
+  else hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_T, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
   return hipGetLastError();
 }
 
@@ -71,7 +81,7 @@ static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const
   const dim3 grid((unsigned)(n1 + yp_plan_workgroups(p2)));
   if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
   else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
-  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_S, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
+  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
   return hipGetLastError();
 }
 

@@ -23,7 +23,7 @@
 
 #include "common.hpp"
 
-enum { YP_TILE_L = 0, YP_TILE_M = 1, YP_TILE_S = 2 };
+enum { YP_TILE_L = 0, YP_TILE_M = 1, YP_TILE_T = 2 };
 enum { YP_T_F32 = YP_F32, YP_T_BF16 = YP_BF16, YP_T_F16 = YP_F16, YP_T_I8 = 3 };
 
 typedef float yp_f4 __attribute__((ext_vector_type(4)));
@@ -216,7 +216,7 @@ struct yp_side {
 template <int SHAPE> struct yp_shape;
 template <> struct yp_shape<YP_TILE_L> { static constexpr int BM = 256, BN = 256, WI = 2, WJ = 2, WPS = 1; };
 template <> struct yp_shape<YP_TILE_M> { static constexpr int BM = 128, BN = 128, WI = 2, WJ = 2, WPS = 2; };
-template <> struct yp_shape<YP_TILE_S> { static constexpr int BM = 128, BN = 64, WI = 4, WJ = 1, WPS = 3; };
+template <> struct yp_shape<YP_TILE_T> { static constexpr int BM = 64, BN = 64, WI = 2, WJ = 2, WPS = 4; };
 template <int SHAPE> constexpr int yp_lds_bytes = 2 * (yp_shape<SHAPE>::BM + yp_shape<SHAPE>::BN) * YP_TILE_KB;
 
 // What an epilogue knows about its place.
@@ -380,6 +380,7 @@ __device__ __forceinline__ void yp_put_tile(const yp_place& at, void* out, int64
   typedef yp_shape<SHAPE> S;
   typedef typename yp_type<OUT>::elem elem;
   constexpr int OB = yp_type<OUT>::bytes, E = 16 / OB, CPR = S::BM / E;      // elements per chunk, chunks per row
+  constexpr int SW = (CPR < 16 ? CPR : 16) - 1;                             // chunk c of row r sits at slot c ^ (r & SW)
   constexpr int PASSES = S::BM * S::BN * OB > yp_lds_bytes<SHAPE> ? 2 : 1;
   typedef elem e4 __attribute__((ext_vector_type(4)));
   typedef elem eE __attribute__((ext_vector_type(E)));
@@ -395,7 +396,7 @@ __device__ __forceinline__ void yp_put_tile(const yp_place& at, void* out, int64
       for (int m = 0; m < MI; ++m) {
         const int byte = (iw + yp_frag_at<S::BM, MI>(m)) * OB;
         const yp_f4 v = val(m, n);
-        *reinterpret_cast<e4*>(at.lds + jl * (S::BM * OB) + (((byte >> 4) ^ (at.lane & 15)) << 4) + (byte & 15)) =
+        *reinterpret_cast<e4*>(at.lds + jl * (S::BM * OB) + (((byte >> 4) ^ (at.lane & SW)) << 4) + (byte & 15)) =
             e4{(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
       }
     }
@@ -406,7 +407,7 @@ __device__ __forceinline__ void yp_put_tile(const yp_place& at, void* out, int64
       const int c = tid % CPR, i = i0 + c * E;
       for (int r = tid / CPR; r < ROWS && j0 + r < J; r += 256 / CPR) {
         if (i >= I) break;
-        eE v = *reinterpret_cast<const eE*>(at.lds + r * (S::BM * OB) + ((c ^ (r & 15)) << 4));
+        eE v = *reinterpret_cast<const eE*>(at.lds + r * (S::BM * OB) + ((c ^ (r & SW)) << 4));
         elem* const to = reinterpret_cast<elem*>(out) + (int64_t)(j0 + r) * ld + i;
         if (i + E <= I) {
           if (ADD) v = v + *reinterpret_cast<const eE*>(to);
@@ -420,7 +421,7 @@ __device__ __forceinline__ void yp_put_tile(const yp_place& at, void* out, int64
       const int c = tid % S::BM, i = i0 + c;
       if (i < I)
         for (int r = tid / S::BM; r < ROWS && j0 + r < J; r += 256 / S::BM) {
-          const elem v = *reinterpret_cast<const elem*>(at.lds + r * (S::BM * OB) + (((c / E) ^ (r & 15)) << 4) + (c % E) * OB);
+          const elem v = *reinterpret_cast<const elem*>(at.lds + r * (S::BM * OB) + (((c / E) ^ (r & SW)) << 4) + (c % E) * OB);
           elem* const to = reinterpret_cast<elem*>(out) + (int64_t)(j0 + r) * ld + i;
           *to = ADD ? (elem)(v + *to) : v;
         }

@@ -38,75 +38,228 @@ __device__ __forceinline__ int yp_quantize(float x, const yp_row_scale& s) {
   return (int)fminf(fmaxf(r, -127.0f), 127.0f);
 }
 
-// LANES threads per row; a thread takes 16-byte chunks of the row.
-template <int TYPE, int LANES>
-__global__ __launch_bounds__(YP_QR_THREADS) void yp_quantize_rows_kernel(const void* x, int64_t rows, int k, int kp, char* q, float* scale, int vec) {
+// A row's elements in 16-byte chunks: chunk c as floats, zeros past the end.
+template <int TYPE>
+struct yp_row_reader {
   typedef typename yp_type<TYPE>::elem elem;
-  constexpr int E = 16 / (int)sizeof(elem);
+  static constexpr int E = 16 / (int)sizeof(elem);
   typedef elem ev __attribute__((ext_vector_type(E)));
-  __shared__ uint32_t red[YP_QR_THREADS / 64];
-  const int lane = (int)threadIdx.x % LANES;
-  const int64_t row = (int64_t)blockIdx.x * (YP_QR_THREADS / LANES) + (int)threadIdx.x / LANES;
-  const bool live = row < rows;
-  const elem* const src = reinterpret_cast<const elem*>(x) + (live ? row : 0) * k;
-  auto get = [&](int c, float (&v)[E]) {
-    if (vec && c + E <= k) {
-      const ev t = *reinterpret_cast<const ev*>(src + c);
+  const elem* src;
+  int k, vec;              // vec: the row starts on 16 bytes
+  __device__ __forceinline__ ev get(int c) const {
+    const int e = c * E;
+    if (vec && e + E <= k) return *reinterpret_cast<const ev*>(src + e);
+    ev t;
 #pragma unroll
-      for (int u = 0; u < E; ++u) v[u] = (float)t[u];
-    } else {
-#pragma unroll
-      for (int u = 0; u < E; ++u) v[u] = c + u < k ? (float)src[c + u] : 0.0f;
-    }
-  };
-  uint32_t top = 0;
-  if (live)
-    for (int c = lane * E; c < k; c += LANES * E) {
-      float v[E];
-      get(c, v);
-#pragma unroll
-      for (int u = 0; u < E; ++u) top = max(top, __builtin_bit_cast(uint32_t, v[u]) & 0x7fffffffu);
-    }
-#pragma unroll
-  for (int s = (LANES < 64 ? LANES : 64) / 2; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
-  if constexpr (LANES > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < LANES / 64; ++w) top = max(top, red[(threadIdx.x / LANES) * (LANES / 64) + w]);
+    for (int u = 0; u < E; ++u) t[u] = e + u < k ? src[e + u] : (elem)0;
+    return t;
   }
-  if (!live) return;
-  const yp_row_scale s = yp_make_scale(top);
-  if (lane == 0) scale[row] = s.scale;
-  char* const dst = q + row * kp;
-  for (int c = lane * E; c < kp; c += LANES * E) {
-    float v[E];
-    get(c, v);
-    uint32_t word[E / 4];
+  static __device__ __forceinline__ uint32_t top(const ev& t, uint32_t m) {
+#pragma unroll
+    for (int u = 0; u < E; ++u) m = max(m, __builtin_bit_cast(uint32_t, (float)t[u]) & 0x7fffffffu);
+    return m;
+  }
+  static __device__ __forceinline__ void put(char* dst, int c, const ev& t, const yp_row_scale& s) {
 #pragma unroll
     for (int w = 0; w < E / 4; ++w) {
-      word[w] = 0;
+      uint32_t word = 0;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) word[w] |= ((uint32_t)yp_quantize(v[w * 4 + u], s) & 0xffu) << (8 * u);
-      reinterpret_cast<uint32_t*>(dst + c)[w] = word[w];
+      for (int u = 0; u < 4; ++u) word |= ((uint32_t)yp_quantize((float)t[w * 4 + u], s) & 0xffu) << (8 * u);
+      reinterpret_cast<uint32_t*>(dst + c * E)[w] = word;
     }
+  }
+};
+
+// LANES threads per row, a thread takes chunks LANES apart and keeps the first YP_QR_KEEP of them in registers between the
+// two passes (maximum, quotients); a longer row's are read again, out of the caches.
+#define YP_QR_KEEP 4
+template <int TYPE, int LANES>
+__global__ __launch_bounds__(YP_QR_THREADS) void yp_quantize_rows_kernel(const void* x, int64_t rows, int k, int kp, char* q, float* scale, int vec) {
+  typedef yp_row_reader<TYPE> R;
+  constexpr int PER = YP_QR_THREADS / LANES;
+  __shared__ uint32_t red[2][YP_QR_THREADS / 64];
+  const int lane = (int)threadIdx.x % LANES, chunks = kp / R::E;
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * PER; first < rows; first += (int64_t)gridDim.x * PER, turn ^= 1) {
+    const int64_t row = first + (int)threadIdx.x / LANES;
+    const bool live = row < rows;
+    const R r = {reinterpret_cast<const typename R::elem*>(x) + (live ? row : 0) * k, k, vec};
+    typename R::ev keep[YP_QR_KEEP];
+    uint32_t top = 0;
+#pragma unroll
+    for (int u = 0; u < YP_QR_KEEP; ++u) if (lane + u * LANES < chunks) keep[u] = r.get(lane + u * LANES);
+#pragma unroll
+    for (int u = 0; u < YP_QR_KEEP; ++u) if (lane + u * LANES < chunks) top = R::top(keep[u], top);
+    for (int c = lane + YP_QR_KEEP * LANES; c < chunks; c += LANES) top = R::top(r.get(c), top);
+#pragma unroll
+    for (int s = (LANES < 64 ? LANES : 64) / 2; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+    if constexpr (LANES > 64) {
+      if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < LANES / 64; ++w) top = max(top, red[turn][w]);
+    }
+    if (!live) continue;
+    const yp_row_scale s = yp_make_scale(top);
+    if (lane == 0) scale[row] = s.scale;
+    char* const dst = q + row * kp;
+#pragma unroll
+    for (int u = 0; u < YP_QR_KEEP; ++u) if (lane + u * LANES < chunks) R::put(dst, lane + u * LANES, keep[u], s);
+    for (int c = lane + YP_QR_KEEP * LANES; c < chunks; c += LANES) R::put(dst, c, r.get(c), s);
   }
 }
 
 template <int TYPE>
-static hipError_t quantize_t(int64_t rows, int k, const void* x, void* q, float* scale, hipStream_t st) {
-  const int kp = (int)yp_qrow_bytes(k);
-  const int vec = ((int64_t)k * yp_type<TYPE>::bytes) % 16 == 0 && ((uintptr_t)x & 15) == 0;
-  if (k <= 2048)
-    hipLaunchKernelGGL((yp_quantize_rows_kernel<TYPE, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(YP_QR_THREADS), 0, st, x, rows, k, kp, (char*)q, scale, vec);
-  else
-    hipLaunchKernelGGL((yp_quantize_rows_kernel<TYPE, 256>), dim3((unsigned)rows), dim3(YP_QR_THREADS), 0, st, x, rows, k, kp, (char*)q, scale, vec);
+static int row_vec(int k, const void* x) { return (int64_t)k * yp_type<TYPE>::bytes % 16 == 0 && ((uintptr_t)x & 15) == 0; }
+
+template <int TYPE, int LANES>
+static hipError_t quantize_l(int64_t rows, int k, const void* x, void* q, float* scale, hipStream_t st) {
+  const int64_t blocks = (rows * LANES + YP_QR_THREADS - 1) / YP_QR_THREADS;
+  hipLaunchKernelGGL((yp_quantize_rows_kernel<TYPE, LANES>), dim3((unsigned)(blocks < (1 << 22) ? blocks : (1 << 22))), dim3(YP_QR_THREADS), 0, st, x, rows, k,
+                     (int)yp_qrow_bytes(k), (char*)q, scale, row_vec<TYPE>(k, x));
   return hipGetLastError();
+}
+// as many threads to a row as keep it in registers
+template <int TYPE>
+static hipError_t quantize_t(int64_t rows, int k, const void* x, void* q, float* scale, hipStream_t st) {
+  const int64_t chunks = yp_qrow_bytes(k) * yp_type<TYPE>::bytes / 16;
+  return chunks <= 16 * YP_QR_KEEP ? quantize_l<TYPE, 16>(rows, k, x, q, scale, st)
+       : chunks <= 64 * YP_QR_KEEP ? quantize_l<TYPE, 64>(rows, k, x, q, scale, st) : quantize_l<TYPE, 256>(rows, k, x, q, scale, st);
 }
 
 hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x, void* q, float* scale, hipStream_t st) {
   return type == YP_F32 ? quantize_t<YP_T_F32>(rows, k, x, q, scale, st)
        : type == YP_BF16 ? quantize_t<YP_T_BF16>(rows, k, x, q, scale, st) : quantize_t<YP_T_F16>(rows, k, x, q, scale, st);
+}
+
+// ---- few rows: the weight is read once and that is all there is -----------------------------------------------------
+// A workgroup holds the (at most YP_FR_ROWS) rows of x in LDS, quantized by itself - 8 KB of x per row from L2 cost less
+// than another launch - and its waves walk over rows of the weight, YP_FR_W at a time: a lane reads 16 bytes of k of each,
+// multiplies with 4-wide dot products and the wave adds up.  YP_FR_C chunks of each are on their way at a time - 16 KB a
+// wave -, the first ones while x is quantized.
+#define YP_FR_ROWS 8
+#define YP_FR_W 4
+#define YP_FR_C 4
+#define YP_FR_LDS 61440
+
+template <int XTYPE, int OUT, int ROWS>
+__global__ __launch_bounds__(YP_QR_THREADS) void yp_few_rows_kernel(const void* x, const float* x_scale, int rows, int v, int k, int kp, const char* wq,
+                                                                    const float* w_scale, const float* bias, void* out, int vec) {
+  typedef typename yp_type<OUT>::elem oelem;
+  extern __shared__ __align__(16) char xl[];      // [rows][kp]
+  __shared__ float sx[ROWS];
+  __shared__ uint32_t red[ROWS][YP_QR_THREADS / 64];
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int wave = (int)blockIdx.x * (YP_QR_THREADS / 64) + (tid >> 6), waves = (int)gridDim.x * (YP_QR_THREADS / 64);
+  const int chunks = kp / 16;
+  yp_i4 w[YP_FR_C][YP_FR_W];
+  auto get_w = [&](int j0, int c0) {              // (zeros past the row)
+#pragma unroll
+    for (int c = 0; c < YP_FR_C; ++c)
+#pragma unroll
+      for (int u = 0; u < YP_FR_W; ++u)
+        w[c][u] = c0 + c * 64 < chunks ? *reinterpret_cast<const yp_i4*>(wq + (int64_t)min(j0 + u, v - 1) * kp + (c0 + c * 64) * 16) : yp_i4{0, 0, 0, 0};
+  };
+  int j0 = wave * YP_FR_W;
+  if (j0 < v) get_w(j0, lane);
+  if constexpr (XTYPE == YP_T_I8) {
+    for (int c = tid; c < rows * chunks; c += YP_QR_THREADS) reinterpret_cast<yp_i4*>(xl)[c] = reinterpret_cast<const yp_i4*>(x)[c];
+    if (tid < rows) sx[tid] = x_scale[tid];
+  } else {
+    typedef yp_row_reader<XTYPE> R;
+    const int ec = kp / R::E;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const R rr = {reinterpret_cast<const typename R::elem*>(x) + (int64_t)min(r, rows - 1) * k, k, vec};
+      uint32_t top = 0;
+      for (int c = tid; c < ec; c += YP_QR_THREADS) top = R::top(rr.get(c), top);
+#pragma unroll
+      for (int s = 32; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+      if (lane == 0) red[r][tid >> 6] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (r < rows) {
+        const R rr = {reinterpret_cast<const typename R::elem*>(x) + (int64_t)r * k, k, vec};
+        uint32_t top = 0;
+#pragma unroll
+        for (int u = 0; u < YP_QR_THREADS / 64; ++u) top = max(top, red[r][u]);
+        const yp_row_scale s = yp_make_scale(top);
+        if (tid == 0) sx[r] = s.scale;
+        for (int c = tid; c < ec; c += YP_QR_THREADS) R::put(xl + r * kp, c, rr.get(c), s);
+      }
+    }
+  }
+  __syncthreads();
+  for (; j0 < v; j0 += waves * YP_FR_W) {
+    int acc[YP_FR_W][ROWS];
+#pragma unroll
+    for (int u = 0; u < YP_FR_W; ++u)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) acc[u][r] = 0;
+    for (int c0 = lane; c0 - lane < chunks; c0 += YP_FR_C * 64) {
+      if (c0 != lane) get_w(j0, c0);
+#pragma unroll
+      for (int c = 0; c < YP_FR_C; ++c) {
+        if (c0 + c * 64 < chunks) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            if (r < rows) {
+              const yp_i4 xv = *reinterpret_cast<const yp_i4*>(xl + r * kp + (c0 + c * 64) * 16);
+#pragma unroll
+              for (int u = 0; u < YP_FR_W; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[u][r] = __builtin_amdgcn_sdot4(w[c][u][e], xv[e], acc[u][r], false);
+            }
+          }
+        }
+      }
+    }
+    const int here = j0;
+    if (here + waves * YP_FR_W < v) get_w(here + waves * YP_FR_W, lane);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (r < rows) {
+#pragma unroll
+        for (int u = 0; u < YP_FR_W; ++u) {
+          int t = acc[u][r];
+#pragma unroll
+          for (int s = 32; s > 0; s >>= 1) t += __shfl_xor(t, s);
+          const int j = here + u;
+          if (lane == u && j < v)
+            reinterpret_cast<oelem*>(out)[(int64_t)r * v + j] = (oelem)__builtin_fmaf((float)t * sx[r], w_scale[j], bias ? bias[j] : 0.0f);
+        }
+      }
+    }
+  }
+}
+
+template <int XTYPE, int OUT>
+static hipError_t few_rows_t(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out,
+                             hipStream_t st) {
+  const int kp = (int)yp_qrow_bytes(k);
+  const int per = YP_FR_W * (YP_QR_THREADS / 64);                 // rows of the weight per workgroup and turn
+  const int64_t turns = ((int64_t)v + per - 1) / per;
+  int64_t resident = 163840 / (rows * kp + 256);                  // workgroups a CU's LDS holds; more would only quantize x again
+  if (resident > 4) resident = 4;                                 // (and its registers: 4)
+  const unsigned blocks = (unsigned)(turns < 256 * resident ? turns : 256 * resident);
+  int vec = 0;
+  if constexpr (XTYPE != YP_T_I8) vec = row_vec<XTYPE>(k, x);
+#define YP_FR_LAUNCH(R) hipLaunchKernelGGL((yp_few_rows_kernel<XTYPE, OUT, R>), dim3(blocks), dim3(YP_QR_THREADS), (size_t)rows * kp, st, x, x_scale, rows, v, k, kp, \
+                                           (const char*)wq, w_scale, bias, out, vec)
+  if (rows == 1) YP_FR_LAUNCH(1);
+  else if (rows <= 4) YP_FR_LAUNCH(4);
+  else YP_FR_LAUNCH(YP_FR_ROWS);
+#undef YP_FR_LAUNCH
+  return hipGetLastError();
+}
+template <int XTYPE>
+static hipError_t few_rows_x(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out,
+                             int out_type, hipStream_t st) {
+  return out_type == YP_F32 ? few_rows_t<XTYPE, YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
+       : out_type == YP_BF16 ? few_rows_t<XTYPE, YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
+                             : few_rows_t<XTYPE, YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st);
 }
 
 template <int OUT>
@@ -145,15 +298,28 @@ static hipError_t linear_t(const yp_gemm& g, const float* x_scale, const float* 
   yp_epi_scaled<OUT> e;
   e.x_scale = x_scale; e.w_scale = w_scale; e.bias = bias; e.out = out;
   e.vec = (int64_t)g.I * yp_type<OUT>::bytes % 16 == 0 && ((uintptr_t)out & 15) == 0;
-  return yp_launch_gemm<YP_T_I8>(yp_plan_tiles(g.I, g.J, g.steps, false), g, e, st);
+  return yp_launch_gemm<YP_T_I8>(yp_plan_tiles(g.I, g.J), g, e, st);
 }
 
-hipError_t yp_launch_quantized_linear(int rows, int v, int k, const void* xq, const float* x_scale, const void* wq, const float* w_scale,
-                                      const float* bias, void* out, int out_type, hipStream_t st) {
+hipError_t yp_launch_quantized_linear(int rows, int v, int k, int x_type, const void* x, const float* x_scale, const void* wq, const float* w_scale,
+                                      const float* bias, void* workspace, void* out, int out_type, hipStream_t st) {
+  const int64_t kp = yp_qrow_bytes(k);
+  if (rows <= YP_FR_ROWS && rows * kp <= YP_FR_LDS)
+    return x_type == YP_INT8 ? few_rows_x<YP_T_I8>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_F32 ? few_rows_x<YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_BF16 ? few_rows_x<YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+                             : few_rows_x<YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
+  if (x_type != YP_INT8) {
+    float* const s = (float*)((char*)workspace + rows * kp);
+    const hipError_t e = yp_launch_quantize_rows(rows, k, x_type, x, workspace, s, st);
+    if (e != hipSuccess) return e;
+    x = workspace;
+    x_scale = s;
+  }
   yp_gemm g = {};
-  g.lda = g.ldb = yp_qrow_bytes(k);
-  g.a = (const char*)wq; g.b = (const char*)xq;
-  g.I = v; g.J = rows; g.steps = (int)(g.lda / YP_TILE_KB);
+  g.lda = g.ldb = kp;
+  g.a = (const char*)wq; g.b = (const char*)x;
+  g.I = v; g.J = rows; g.steps = (int)(kp / YP_TILE_KB);
   return out_type == YP_F32 ? linear_t<YP_T_F32>(g, x_scale, w_scale, bias, out, st)
        : out_type == YP_BF16 ? linear_t<YP_T_BF16>(g, x_scale, w_scale, bias, out, st) : linear_t<YP_T_F16>(g, x_scale, w_scale, bias, out, st);
 }
