@@ -78,10 +78,11 @@ template <int TYPE, class Epi>
 static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const Epi& e1, const yp_tile_plan& p2, const yp_gemm& g2, const Epi& e2, hipStream_t st) {
   const yp_gemm a = yp_with_plan(g1, p1), b = yp_with_plan(g2, p2);
   const int n1 = (int)yp_plan_workgroups(p1);
+  const int second_first = b.steps / b.splits > a.steps / a.splits;   // the longer ones first: the short ones fill up the end
   const dim3 grid((unsigned)(n1 + yp_plan_workgroups(p2)));
-  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
-  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
-  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2);
+  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
+  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
+  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
   return hipGetLastError();
 }
 

@@ -355,12 +355,15 @@ __global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_gemm_kernel(cons
   yp_gemm_tile<TYPE, SHAPE, A_BY_K, B_BY_K>(g, epi, (int)blockIdx.x, (int)gridDim.x, lds);
 }
 
-// Two independent products of one tile shape in one launch: the first `n1` workgroups are the first one's.
+// Two independent products of one tile shape in one launch, n1 workgroups the first one's; with `second_first` the second
+// one's workgroups come first.
 template <int TYPE, int SHAPE, bool A1, bool B1, bool A2, bool B2, class Epi>
-__global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_two_gemms_kernel(const yp_gemm g1, const Epi e1, int n1, const yp_gemm g2, const Epi e2) {
+__global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_two_gemms_kernel(const yp_gemm g1, const Epi e1, int n1, const yp_gemm g2, const Epi e2, int second_first) {
   __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
-  if ((int)blockIdx.x < n1) yp_gemm_tile<TYPE, SHAPE, A1, B1>(g1, e1, (int)blockIdx.x, n1, lds);
-  else yp_gemm_tile<TYPE, SHAPE, A2, B2>(g2, e2, (int)blockIdx.x - n1, (int)gridDim.x - n1, lds);
+  const int n2 = (int)gridDim.x - n1, wg = (int)blockIdx.x;
+  const bool first = second_first ? wg >= n2 : wg < n1;
+  if (first) yp_gemm_tile<TYPE, SHAPE, A1, B1>(g1, e1, second_first ? wg - n2 : wg, n1, lds);
+  else yp_gemm_tile<TYPE, SHAPE, A2, B2>(g2, e2, second_first ? wg : wg - n1, n2, lds);
 }
 
 // Where an epilogue's fragment (0, 0), element 0 lies: i and j of this lane.

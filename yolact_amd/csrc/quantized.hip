@@ -2,9 +2,10 @@
 //
 //   scale = max|x| / 127 (f32)      q = x / scale to the nearest integer, ties to even
 //
-// q is the rounding of the exact quotient: r = rint(x * (1 / scale)) is at most one off (only next to a half), and
-// x - r scale is exact in one fused multiply-add (|r| <= 127, |x - r scale| <= scale), so comparing it with half a
-// scale settles the case.  A reciprocal per row and no division per element.
+// q is the rounding of the exact quotient: r = x * (1 / scale) rounded to a whole number is at most one off, and only next
+// to a half; x - r scale is exact in one fused multiply-add (|r| <= 127, |x - r scale| <= scale), so comparing it with half
+// a scale settles the case.  A reciprocal per row and no division per element; the comparison is one maximum per element,
+// and only where some element of the thread's lies within 2^-12 of a half (1 in 2000 chunks) is each looked at.
 // The integer sums are exact (k <= 131072: 127 * 127 * k < 2^31); the only roundings are the sum's conversion to f32,
 // the two scales, the bias, and the output type.
 #include "gemm_launch.hpp"
@@ -13,29 +14,50 @@
 
 int64_t yp_qrow_bytes(int64_t k) { return yp_pad_k(k, 1); }
 
-struct yp_row_scale { float scale, unit, inv, half; float pre; };
+struct yp_row_scale { float scale, unit, inv, half, near; };
 
 // scale of a row from the bits of its largest magnitude (NaN and infinities have the largest bits of all)
 __device__ __forceinline__ yp_row_scale yp_make_scale(uint32_t top) {
   yp_row_scale r;
-  if (top >= 0x7f800000u) { r.scale = NAN; r.unit = r.inv = r.half = r.pre = 0.0f; return r; }
+  if (top >= 0x7f800000u) { r.scale = NAN; r.unit = r.inv = r.half = 0.0f; r.near = -1.0f; return r; }
   const float amax = __builtin_bit_cast(float, top);
   r.scale = amax / 127.0f;
-  r.pre = amax < 0x1p-60f ? 0x1p64f : 1.0f;          // keeps the reciprocal of a tiny scale finite; exact
-  r.unit = r.scale * r.pre;
+  const bool tiny = amax < 0x1p-60f;                // near = -1: every element the careful way, scaled up by 2^64 (exact)
+  r.unit = r.scale * (tiny ? 0x1p64f : 1.0f);
   r.inv = r.unit > 0.0f ? 1.0f / r.unit : 0.0f;
   r.half = 0.5f * r.unit;
+  r.near = tiny ? -1.0f : r.half * (1.0f - 0x1p-12f);
   return r;
 }
-__device__ __forceinline__ int yp_quantize(float x, const yp_row_scale& s) {
-  const float v = x * s.pre;
-  float r = rintf(v * s.inv);
-  r = fminf(fmaxf(r, -127.0f), 127.0f);
+static __device__ __attribute__((noinline)) uint32_t yp_quantize_carefully(float x, const yp_row_scale s) {
+  const float v = s.near < 0.0f ? x * 0x1p64f : x;
+  float r = fminf(fmaxf(rintf(v * s.inv), -127.0f), 127.0f);
   const float rem = __builtin_fmaf(-r, s.unit, v);
-  const bool odd = ((int)r & 1) != 0;
-  if (rem > s.half || (rem == s.half && odd && s.unit > 0.0f)) r += 1.0f;
-  else if (rem < -s.half || (rem == -s.half && odd && s.unit > 0.0f)) r -= 1.0f;
-  return (int)fminf(fmaxf(r, -127.0f), 127.0f);
+  const bool odd = ((int)r & 1) != 0 && s.unit > 0.0f;
+  if (rem > s.half || (rem == s.half && odd)) r += 1.0f;
+  else if (rem < -s.half || (rem == -s.half && odd)) r -= 1.0f;
+  return s.unit > 0.0f ? (uint32_t)(int)fminf(fmaxf(r, -127.0f), 127.0f) & 0xffu : 0u;
+}
+// N elements to N bytes
+template <int N>
+__device__ __forceinline__ void yp_quantize(const float (&x)[N], const yp_row_scale& s, uint32_t (&word)[N / 4]) {
+  uint32_t bits[N];
+  float far = 0.0f;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const float m = __builtin_fmaf(x[u], s.inv, 12582912.0f);        // 1.5 * 2^23: the sum's low byte is the whole number
+    far = fmaxf(far, fabsf(__builtin_fmaf(-(m - 12582912.0f), s.unit, x[u])));
+    bits[u] = __builtin_bit_cast(uint32_t, m);
+  }
+  if (far > s.near) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) bits[u] = yp_quantize_carefully(x[u], s);
+  }
+#pragma unroll
+  for (int w = 0; w < N / 4; ++w) {
+    const uint32_t lo = __builtin_amdgcn_perm(bits[w * 4 + 1], bits[w * 4], 0x0c0c0400u), hi = __builtin_amdgcn_perm(bits[w * 4 + 3], bits[w * 4 + 2], 0x0c0c0400u);
+    word[w] = lo | hi << 16;
+  }
 }
 
 // A row's elements in 16-byte chunks: chunk c as floats, zeros past the end.
@@ -59,14 +81,17 @@ struct yp_row_reader {
     for (int u = 0; u < E; ++u) m = max(m, __builtin_bit_cast(uint32_t, (float)t[u]) & 0x7fffffffu);
     return m;
   }
+  static __device__ __forceinline__ void quantize(const ev& t, const yp_row_scale& s, uint32_t (&word)[E / 4]) {
+    float x[E];
+#pragma unroll
+    for (int u = 0; u < E; ++u) x[u] = (float)t[u];
+    yp_quantize<E>(x, s, word);
+  }
   static __device__ __forceinline__ void put(char* dst, int c, const ev& t, const yp_row_scale& s) {
+    uint32_t word[E / 4];
+    quantize(t, s, word);
 #pragma unroll
-    for (int w = 0; w < E / 4; ++w) {
-      uint32_t word = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) word |= ((uint32_t)yp_quantize((float)t[w * 4 + u], s) & 0xffu) << (8 * u);
-      reinterpret_cast<uint32_t*>(dst + c * E)[w] = word;
-    }
+    for (int w = 0; w < E / 4; ++w) reinterpret_cast<uint32_t*>(dst + c * E)[w] = word[w];
   }
 };
 
@@ -262,6 +287,137 @@ static hipError_t few_rows_x(int rows, int v, int k, const void* x, const float*
                              : few_rows_t<XTYPE, YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st);
 }
 
+// ---- many rows, a small weight: the head over all anchors ------------------------------------------------------------
+// x is read once, and that is most of it.  A wave takes 16 rows and keeps them in registers in the order of the matrix
+// instruction - lane l holds row l & 15, and of every 64 k those that 16-byte loads bring to quarter l >> 4 (which k they
+// are does not matter as long as the weight has the same order: it is laid out so in LDS, once per workgroup) -, so the
+// row's maximum is two shuffles and the quotients never leave the lane.  The results go through LDS, 16 rows at a time,
+// and out as one run of 16-byte stores: 16 rows are a multiple of 16 bytes whatever v is.
+#define YP_TR_LDS 81920
+
+template <int XTYPE, int OUT, int STEPS>   // STEPS: 64 k each, at most
+__global__ __launch_bounds__(YP_QR_THREADS) void yp_tall_kernel(const void* x, const float* x_scale, int rows, int v, int k, int kp, const char* wq,
+                                                                const float* w_scale, const float* bias, void* out, int vec, int out_vec) {
+  typedef typename yp_type<OUT>::elem oelem;
+  constexpr int XB = yp_type<XTYPE>::bytes, E = 16 / XB, LOADS = 4 * XB / 4;   // loads per 64 k: 4 (f32), 2, 1
+  extern __shared__ __align__(16) char lds[];          // [v padded to 16][kp] weight | [2][v padded] scales, biases | per wave [16][v] results
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, g = lane >> 4;
+  const int vt = (v + 15) / 16, steps = kp / 64;
+  // chunk c of a weight row (16 k): its 64 k's quarter-chunks, reordered; slot exclusive-ored by the row against bank conflicts
+  for (int c = tid; c < vt * 16 * (kp / 16); c += YP_QR_THREADS) {
+    const int i = c / (kp / 16), q = c - i * (kp / 16), s = q >> 2, qg = q & 3;
+    yp_i4 w = {0, 0, 0, 0};
+    if (i < v) {
+      const char* const src = wq + (int64_t)i * kp + s * 64;
+#pragma unroll
+      for (int e = 0; e < LOADS; ++e)
+#pragma unroll
+        for (int u = 0; u < E / 4; ++u) w[e * (E / 4) + u] = *reinterpret_cast<const int*>(src + e * 4 * E + qg * E + u * 4);
+    }
+    *reinterpret_cast<yp_i4*>(lds + i * kp + ((q ^ (i & 7)) * 16)) = w;
+  }
+  float* const sw = reinterpret_cast<float*>(lds + vt * 16 * kp);
+  for (int i = tid; i < vt * 16; i += YP_QR_THREADS) { sw[i] = i < v ? w_scale[i] : 0.0f; sw[vt * 16 + i] = bias && i < v ? bias[i] : 0.0f; }
+  oelem* const stage = reinterpret_cast<oelem*>(lds + vt * 16 * (kp + 8)) + wave * 16 * v;
+  __syncthreads();
+  for (int64_t r0 = ((int64_t)blockIdx.x * 4 + wave) * 16; r0 < rows; r0 += (int64_t)gridDim.x * 64) {
+    const int64_t r = r0 + row < rows ? r0 + row : rows - 1;
+    yp_i4 f[STEPS];
+    float sx;
+    if constexpr (XTYPE == YP_T_I8) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        f[s] = s < steps ? *reinterpret_cast<const yp_i4*>(reinterpret_cast<const char*>(x) + r * kp + s * 64 + g * 16) : yp_i4{0, 0, 0, 0};
+      sx = x_scale[r];
+    } else {
+      typedef yp_row_reader<XTYPE> R;
+      const R rr = {reinterpret_cast<const typename R::elem*>(x) + r * k, k, vec};
+      typename R::ev t[STEPS][LOADS];
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (s < steps)
+#pragma unroll
+          for (int e = 0; e < LOADS; ++e) t[s][e] = rr.get(s * (64 / E) + e * 4 + g);
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (s < steps)
+#pragma unroll
+          for (int e = 0; e < LOADS; ++e) top = R::top(t[s][e], top);
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      const yp_row_scale sc = yp_make_scale(top);
+      sx = sc.scale;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        f[s] = yp_i4{0, 0, 0, 0};
+        if (s < steps)
+#pragma unroll
+          for (int e = 0; e < LOADS; ++e) {
+            uint32_t word[E / 4];
+            R::quantize(t[s][e], sc, word);
+#pragma unroll
+            for (int u = 0; u < E / 4; ++u) f[s][e * (E / 4) + u] = (int)word[u];
+          }
+      }
+    }
+    for (int it = 0; it < vt; ++it) {
+      yp_i4 acc = {0, 0, 0, 0};
+      const int i = it * 16 + row;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (s < steps) acc = yp_mma<YP_T_I8>(*reinterpret_cast<const yp_i4*>(lds + i * kp + (((s * 4 + g) ^ (i & 7)) * 16)), f[s], acc);
+      const yp_f4 ws = *reinterpret_cast<const yp_f4*>(sw + it * 16 + g * 4), b = *reinterpret_cast<const yp_f4*>(sw + vt * 16 + it * 16 + g * 4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int o = it * 16 + g * 4 + u;
+        if (o < v) stage[row * v + o] = (oelem)__builtin_fmaf((float)acc[u] * sx, ws[u], b[u]);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the wave's own rows: no other wave to wait for)
+    const int total = (int)(rows - r0 < 16 ? rows - r0 : 16) * v, per = 16 / (int)sizeof(oelem);
+    oelem* const to = reinterpret_cast<oelem*>(out) + r0 * v;
+    if (out_vec) {
+      for (int c = lane; c < total / per; c += 64) reinterpret_cast<yp_i4*>(to)[c] = reinterpret_cast<const yp_i4*>(stage)[c];
+      for (int c = total / per * per + lane; c < total; c += 64) to[c] = stage[c];
+    } else {
+      for (int c = lane; c < total; c += 64) to[c] = stage[c];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+static bool tall_fits(int rows, int v, int64_t kp, int out_bytes) {
+  return rows >= 4096 && kp <= 512 && (int64_t)(v + 15) / 16 * 16 * (kp + 8) + (int64_t)64 * v * out_bytes <= YP_TR_LDS;
+}
+template <int XTYPE, int OUT>
+static hipError_t tall_t(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, hipStream_t st) {
+  const int kp = (int)yp_qrow_bytes(k);
+  const size_t lds = (size_t)(v + 15) / 16 * 16 * (kp + 8) + (size_t)64 * v * yp_type<OUT>::bytes;
+  int64_t blocks = ((int64_t)rows + 63) / 64, resident = 256 * (163840 / (int64_t)lds < 4 ? 163840 / (int64_t)lds : 4);
+  if (blocks > resident) blocks = resident;
+  int vec = 0;
+  if constexpr (XTYPE != YP_T_I8) vec = row_vec<XTYPE>(k, x);
+  const int out_vec = ((uintptr_t)out & 15) == 0;
+  const void* const fn = kp <= 256 ? reinterpret_cast<const void*>(&yp_tall_kernel<XTYPE, OUT, 4>) : reinterpret_cast<const void*>(&yp_tall_kernel<XTYPE, OUT, 8>);
+  if (lds > 48 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, YP_TR_LDS);
+    if (e != hipSuccess) return e;
+  }
+  if (kp <= 256)
+    hipLaunchKernelGGL((yp_tall_kernel<XTYPE, OUT, 4>), dim3((unsigned)blocks), dim3(YP_QR_THREADS), lds, st, x, x_scale, rows, v, k, kp, (const char*)wq, w_scale, bias, out, vec, out_vec);
+  else
+    hipLaunchKernelGGL((yp_tall_kernel<XTYPE, OUT, 8>), dim3((unsigned)blocks), dim3(YP_QR_THREADS), lds, st, x, x_scale, rows, v, k, kp, (const char*)wq, w_scale, bias, out, vec, out_vec);
+  return hipGetLastError();
+}
+template <int XTYPE>
+static hipError_t tall_x(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, int out_type,
+                         hipStream_t st) {
+  return out_type == YP_F32 ? tall_t<XTYPE, YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
+       : out_type == YP_BF16 ? tall_t<XTYPE, YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
+                             : tall_t<XTYPE, YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st);
+}
+
 template <int OUT>
 struct yp_epi_scaled {
   const float *x_scale, *w_scale, *bias;
@@ -309,6 +465,11 @@ hipError_t yp_launch_quantized_linear(int rows, int v, int k, int x_type, const 
          : x_type == YP_F32 ? few_rows_x<YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
          : x_type == YP_BF16 ? few_rows_x<YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
                              : few_rows_x<YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
+  if (tall_fits(rows, v, kp, out_type == YP_F32 ? 4 : 2))
+    return x_type == YP_INT8 ? tall_x<YP_T_I8>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_F32 ? tall_x<YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_BF16 ? tall_x<YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+                             : tall_x<YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
   if (x_type != YP_INT8) {
     float* const s = (float*)((char*)workspace + rows * kp);
     const hipError_t e = yp_launch_quantize_rows(rows, k, x_type, x, workspace, s, st);
