@@ -16,12 +16,15 @@
 // dz is rounded to the features' type - the matrix instruction takes nothing wider beside h and w; each dz is off by
 // half a step of that type, like the gradients themselves - f16 with a power-of-two factor that brings the largest
 // |g| to [2^13, 2^14), so that probabilities down to 2^-38 of it are kept, taken out again in f32 at the end.
+// f32 of any size worth it runs on the bf16 matrix instructions, as three bf16 planes per operand (SPLIT, gemm_tile.hpp).
 // What takes no part has dz = 0, but 0 times NaN is NaN: the gradient products read a copy of h in which ignored rows are
 // zero (and of w, if a bias may mask classes).
 // All sums are f32 in a fixed order: no float atomics, the same call gives the same bits.
 #include "gemm_launch.hpp"
 
 #define YP_CL_THREADS 256
+// f32 products of as many multiplications go through bf16 planes: 200 TFLOP/s against 125; below, the copies cost more
+#define YP_CL_SPLIT_FROM (1ll << 31)
 #define YP_CL_PIECE_MAX (1 << 17)
 #define YP_CL_PIECE_BYTES (128ll << 20)   // of dz: half of the Infinity Cache
 
@@ -39,6 +42,12 @@ __device__ __forceinline__ void yp_join(float& m, float& s, float m2, float s2) 
   m = t;
 }
 
+// what is left of an f32 beside its bf16 plane: exact (nothing beside an infinity or NaN)
+__device__ __forceinline__ float yp_plane_rest(float x) {
+  const float h = (float)(__bf16)x;
+  return fabsf(h) < INFINITY ? x - h : 0.0f;
+}
+
 struct yp_labels {
   const void* labels;
   int bytes;
@@ -53,8 +62,9 @@ struct yp_labels {
 };
 
 // ---- epilogue of the forward product: i = class, j = row ----------------------------------------------------------
+template <int ELEM>
 struct yp_epi_stats {
-  const void* bias;            // elements of the features' type, may be null; of the piece
+  const void* bias;            // of the tensors' type ELEM, may be null; of the piece
   yp_labels labels;
   int first;                   // first class of the piece
   yp_softmax_part* part;       // [tiles_i * WI][N] of the piece
@@ -70,7 +80,7 @@ struct yp_epi_stats {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = ib + yp_frag_at<S::BM, MI>(m) + r;
-          const float b = i >= g.I ? -INFINITY : (bias ? yp_load_as_float(bias, i, TYPE) : 0.0f);
+          const float b = i >= g.I ? -INFINITY : (bias ? yp_load_as_float(bias, i, ELEM) : 0.0f);
 #pragma unroll
           for (int n = 0; n < NJ; ++n) acc[m][n][r] = b == -INFINITY ? -INFINITY : acc[m][n][r] + b;
         }
@@ -105,8 +115,9 @@ struct yp_epi_stats {
 };
 
 // ---- epilogue of the backward product -----------------------------------------------------------------------------
+template <int ELEM, bool SPLIT>
 struct yp_epi_dz {
-  const void* bias;            // of the piece
+  const void* bias;            // of the tensors' type ELEM; of the piece
   const float* lse;
   yp_labels labels;
   const float* grad;
@@ -114,7 +125,8 @@ struct yp_epi_dz {
   const float* count;          // null: grads are the rows' own; else divided by max(count, 1)
   const float* factor;         // f16: {2^e, 2^-e}, else null
   int first;                   // first class of the piece
-  void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv)
+  void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv); SPLIT: three planes of it, bf16
+  int64_t plane;               // bytes of one
   int kv, kn;
   void* bias_out;              // of the piece; null without bias
   float* bias_part;            // [tiles_j][bias_ld] of the piece if there is more than one tile in j, else null
@@ -122,7 +134,7 @@ struct yp_epi_dz {
   template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
   __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], const yp_place& at) const {
     typedef yp_shape<SHAPE> S;
-    typedef typename yp_type<TYPE>::elem elem;
+    typedef typename yp_type<ELEM>::elem elem;
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
     const float over = count ? 1.0f / fmaxf(*count, 1.0f) : 1.0f, up = factor ? factor[0] : 1.0f;
@@ -133,7 +145,7 @@ struct yp_epi_dz {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = ib + yp_frag_at<S::BM, MI>(m) + r;
-        b[m][r] = !edge ? 0.0f : i >= g.I ? -INFINITY : (bias ? yp_load_as_float(bias, i, TYPE) : 0.0f);
+        b[m][r] = !edge ? 0.0f : i >= g.I ? -INFINITY : (bias ? yp_load_as_float(bias, i, ELEM) : 0.0f);
       }
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
@@ -179,6 +191,17 @@ struct yp_epi_dz {
       yp_arrive<0>();
     }
     yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, dz, kv, kv, kn, true, [&](int m, int n) { return acc[m][n]; });
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int q = 1; q < 3; ++q) {
+        yp_arrive<0>();
+        yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, (char*)dz + q * plane, kv, kv, kn, true, [&](int m, int n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[m][n][r] = yp_plane_rest(acc[m][n][r]);
+          return acc[m][n];
+        });
+      }
+    }
   }
 };
 
@@ -193,6 +216,7 @@ struct yp_copy_job {
   int vec;                // rows of src are multiples of 16 bytes and so is their address
   int by_label;
   const void* bias;
+  int64_t plane;          // 0, or: f32 rows to three bf16 planes, this many bytes apart (row_bytes, kb: of a plane's row)
 };
 struct yp_copy_args {
   yp_copy_job job[2];
@@ -212,6 +236,30 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
     bool in = r < j.rows;
     if (in && j.by_label) in = a.labels.counted(r) >= 0;
     if (in && j.bias) in = yp_load_as_float(j.bias, r, a.type) != -INFINITY;
+    if (j.plane) {        // 8 elements
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = 0.0f;
+      if (in) {
+        const char* const s = j.src + (r * j.row_bytes + at) * 2;
+        if (j.vec && at + 16 <= j.row_bytes) {
+          const yp_f4 lo = reinterpret_cast<const yp_f4*>(s)[0], hi = reinterpret_cast<const yp_f4*>(s)[1];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) { x[u] = lo[u]; x[4 + u] = hi[u]; }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) if (at + 2 * u < j.row_bytes) x[u] = reinterpret_cast<const float*>(s)[u];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        yp_bf8 o;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { o[u] = (__bf16)x[u]; x[u] = yp_plane_rest(x[u]); }
+        *reinterpret_cast<yp_bf8*>(j.dst + q * j.plane + r * j.kb + at) = o;
+      }
+      continue;
+    }
     yp_i4 v = {0, 0, 0, 0};
     if (in) {
       const char* const s = j.src + r * j.row_bytes + at;
@@ -414,6 +462,8 @@ static hipError_t zero(void* out, int64_t n, int type, hipStream_t st) {   // (a
 
 // The launch plan of a call, from its sizes alone: the same for yp_class_loss_workspace and for the call.
 struct ClassLossPlan {
+  bool split;                  // f32 in three bf16 planes
+  int b, planes;               // bytes of an element and how many planes the products read
   int64_t kd;                  // bytes of a padded feature row
   int fwd_pieces, fwd_piece;   // forward: pieces of the vocabulary if w is copied, else one
   yp_tile_plan fwd;            // of a whole piece
@@ -438,16 +488,20 @@ static void cut_pieces(int64_t V, int64_t most, int* pieces, int* piece) {   // 
 
 static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, bool has_bias, bool copy_fwd) {
   ClassLossPlan p;
-  const int b = type_bytes(type);
+  p.split = type == YP_F32 && N * V >= YP_CL_SPLIT_FROM / D;
+  const int b = p.split ? 2 : type_bytes(type), planes = p.split ? 3 : 1;
+  p.b = b;
+  p.planes = planes;
+  copy_fwd = copy_fwd || p.split;
   p.kd = yp_pad_k(D, b);
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = up256(off + bytes); return o; };
-  if (copy_fwd) cut_pieces(V, YP_CL_PIECE_BYTES / p.kd, &p.fwd_pieces, &p.fwd_piece);
+  if (copy_fwd) cut_pieces(V, YP_CL_PIECE_BYTES / (p.kd * planes), &p.fwd_pieces, &p.fwd_piece);
   else { p.fwd_pieces = 1; p.fwd_piece = (int)V; }
   p.fwd = yp_plan_tiles(p.fwd_piece, N);
   p.parts = p.fwd.tiles_i * 2;
-  p.o_h = take(copy_fwd ? N * p.kd : 0);
-  p.o_w = take(copy_fwd ? p.fwd_piece * p.kd : 0);
+  p.o_h = take(copy_fwd ? N * p.kd * planes : 0);
+  p.o_w = take(copy_fwd ? p.fwd_piece * p.kd * planes : 0);
   p.o_part = take((int64_t)p.fwd_pieces * p.parts * N * sizeof(yp_softmax_part));
   p.o_picked = take(N * 4);
   p.o_block = take((N <= 1024 ? (N + 1) / 2 : (N + 31) / 32) * 16);
@@ -456,17 +510,18 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   off = 0;
   const int kr = YP_TILE_KB / b;
   p.kn = (N + kr - 1) / kr * kr;
-  int64_t most = YP_CL_PIECE_BYTES / (p.kn * b);
-  if (most > YP_CL_PIECE_BYTES / p.kd) most = YP_CL_PIECE_BYTES / p.kd;
+  int64_t most = YP_CL_PIECE_BYTES / (p.kn * b * planes);
+  if (most > YP_CL_PIECE_BYTES / (p.kd * planes)) most = YP_CL_PIECE_BYTES / (p.kd * planes);
   cut_pieces(V, most, &p.pieces, &p.piece);
   p.kv = yp_pad_k(p.piece, b);
   p.dzp = yp_plan_tiles(p.piece, p.kn);
   // the two gradient products share a launch and so a tile shape
-  yp_plan_two(D, p.piece, p.kn / kr, D, N, p.kv / YP_TILE_KB, &p.dwp, &p.dhp);
+  const int segs = p.split ? YP_SEGMENTS : 1;
+  yp_plan_two(D, p.piece, p.kn / kr * segs, D, N, p.kv / YP_TILE_KB * segs, &p.dwp, &p.dhp);
   p.o_factor = take(8);
-  p.o_hc = take(p.kn * p.kd);
-  p.o_wc = take(p.piece * p.kd);
-  p.o_dz = take(p.kn * p.kv);
+  p.o_hc = take(p.kn * p.kd * planes);
+  p.o_wc = take(p.piece * p.kd * planes);
+  p.o_dz = take(p.kn * p.kv * planes);
   p.o_bp = take(has_bias && p.dzp.tiles_j > 1 ? (int64_t)p.dzp.tiles_j * V * 4 : 0);
   p.o_dwpart = take(p.dwp.splits > 1 ? (int64_t)p.dwp.splits * p.piece * D * 4 : 0);
   p.o_dhpart = take(p.dhp.splits > 1 || p.pieces > 1 ? (int64_t)p.dhp.splits * N * D * 4 : 0);
@@ -481,10 +536,12 @@ int64_t yp_class_loss_bytes(int64_t n, int64_t v, int64_t d, int type, int has_b
   return a.fwd_total > c.fwd_total ? a.fwd_total : c.fwd_total;
 }
 
-#define CL_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
+#define CL_TRY(...) do { const hipError_t e_ = (__VA_ARGS__); if (e_ != hipSuccess) return e_; } while (0)
 
-static yp_copy_job copy_job(const void* src, char* dst, int64_t row_bytes, int64_t kb, int64_t rows, int64_t rows_out) {
+static yp_copy_job copy_job(const void* src, char* dst, int64_t d, const ClassLossPlan& p, int64_t rows, int64_t rows_out) {
+  const int64_t row_bytes = d * p.b, kb = p.kd;
   yp_copy_job j = {};
+  if (p.split) j.plane = rows_out * kb;
   j.src = (const char*)src; j.dst = dst; j.row_bytes = row_bytes; j.kb = kb; j.rows = rows; j.rows_out = rows_out;
   j.vec = row_bytes % 16 == 0 && ((uintptr_t)src & 15) == 0;
   return j;
@@ -496,12 +553,13 @@ static hipError_t copy_rows(yp_copy_args a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int TYPE>
+// TYPE: the matrix instructions'; ELEM: the tensors'.  SPLIT: f32 by three bf16 planes.
+template <int TYPE, int ELEM, bool SPLIT>
 static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
-  constexpr int b = yp_type<TYPE>::bytes;
+  constexpr int b = yp_type<ELEM>::bytes;
   const int64_t row = (int64_t)a.d * b;
-  const bool copy = row % YP_TILE_KB != 0 || (((uintptr_t)a.features | (uintptr_t)a.weight) & 15) != 0;
-  const ClassLossPlan p = plan_class_loss(a.n, a.v, a.d, TYPE, a.bias != nullptr, copy);
+  const bool copy = SPLIT || row % YP_TILE_KB != 0 || (((uintptr_t)a.features | (uintptr_t)a.weight) & 15) != 0;
+  const ClassLossPlan p = plan_class_loss(a.n, a.v, a.d, ELEM, a.bias != nullptr, copy);
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
   yp_softmax_part* const part = (yp_softmax_part*)(ws + p.o_part);
@@ -512,9 +570,10 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
     g.a = (const char*)a.weight; g.b = (const char*)a.features;
     if (copy) {
       yp_copy_args c = {};
-      c.type = TYPE;
-      c.job[0] = copy_job(g.a + v0 * row, ws + p.o_w, row, p.kd, nv, nv);
-      if (s == 0) c.job[1] = copy_job(g.b, ws + p.o_h, row, p.kd, a.n, a.n);
+      c.type = ELEM;
+      c.job[0] = copy_job(g.a + v0 * row, ws + p.o_w, a.d, p, nv, nv);
+      if (s == 0) c.job[1] = copy_job(g.b, ws + p.o_h, a.d, p, a.n, a.n);
+      g.aplane = nv * p.kd; g.bplane = a.n * p.kd;
       CL_TRY(copy_rows(c, st));
       g.a = ws + p.o_w; g.b = ws + p.o_h;
     }
@@ -522,10 +581,10 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
     g.I = nv; g.J = a.n; g.steps = (int)(p.kd / YP_TILE_KB);
     yp_tile_plan tp = p.fwd;
     tp.tiles_i = (nv + tp.bi - 1) / tp.bi;
-    yp_epi_stats e;
+    yp_epi_stats<ELEM> e;
     e.bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
     e.labels = labels; e.first = v0; e.part = part + (int64_t)parts * a.n; e.picked = (float*)(ws + p.o_picked);
-    CL_TRY(yp_launch_gemm<TYPE>(tp, g, e, st));
+    CL_TRY(yp_launch_gemm<TYPE, SPLIT>(tp, g, e, st));
     parts += tp.tiles_i * 2;
   }
   yp_join_args j;
@@ -545,12 +604,12 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int TYPE>
+template <int TYPE, int ELEM, bool SPLIT>
 static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
-  constexpr int b = yp_type<TYPE>::bytes;
+  constexpr int b = yp_type<ELEM>::bytes, tb = yp_type<TYPE>::bytes;
   const int64_t row = (int64_t)a.d * b;
-  const ClassLossPlan p = plan_class_loss(a.n, a.v, a.d, TYPE, a.bias != nullptr, false);
-  const bool copy_w = a.bias || row % YP_TILE_KB != 0 || ((uintptr_t)a.weight & 15) != 0;
+  const ClassLossPlan p = plan_class_loss(a.n, a.v, a.d, ELEM, a.bias != nullptr, false);
+  const bool copy_w = SPLIT || a.bias || row % YP_TILE_KB != 0 || ((uintptr_t)a.weight & 15) != 0;
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
   float* const factor = TYPE == YP_T_F16 ? (float*)(ws + p.o_factor) : nullptr;
@@ -563,7 +622,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   float* const biaspart = p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
   const bool dh_joined = p.dhp.splits > 1 || p.pieces > 1;
   yp_sum_args sums = {};
-  sums.out_type = TYPE;
+  sums.out_type = ELEM;
   sums.scale = back;
   for (int s = 0; s < p.pieces; ++s) {
     const int v0 = s * p.piece, nv = a.v - v0 < p.piece ? a.v - v0 : p.piece;
@@ -571,19 +630,22 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     const char* w = (const char*)a.weight + v0 * row;
     if (s == 0 || copy_w) {
       yp_copy_args c = {};
-      c.type = TYPE;
+      c.type = ELEM;
       c.labels = labels;
       int n = 0;
-      if (s == 0) { c.job[n] = copy_job(a.features, ws + p.o_hc, row, p.kd, a.n, p.kn); c.job[n++].by_label = 1; }
-      if (copy_w) { c.job[n] = copy_job(w, ws + p.o_wc, row, p.kd, nv, nv); c.job[n++].bias = bias; w = ws + p.o_wc; }
+      if (s == 0) { c.job[n] = copy_job(a.features, ws + p.o_hc, a.d, p, a.n, p.kn); c.job[n++].by_label = 1; }
+      if (copy_w) { c.job[n] = copy_job(w, ws + p.o_wc, a.d, p, nv, nv); c.job[n++].bias = bias; w = ws + p.o_wc; }
       CL_TRY(copy_rows(c, st));
     }
-    const int kv = (int)(yp_pad_k(nv, b) / b);
+    const int kv = (int)(yp_pad_k(nv, tb) / tb);
+    const int64_t hplane = p.kn * p.kd, wplane = nv * p.kd, dzplane = p.kn * kv * tb;
     // dz of the piece
     yp_gemm g = {};
     g.a = w; g.b = ws + p.o_hc; g.lda = g.ldb = p.kd;
+    g.aplane = wplane; g.bplane = hplane;
     g.I = nv; g.J = a.n; g.steps = (int)(p.kd / YP_TILE_KB);
-    yp_epi_dz e;
+    yp_epi_dz<ELEM, SPLIT> e;
+    e.plane = dzplane;
     e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad; e.grad_stride = a.grad_stride; e.count = a.count; e.factor = factor;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
     e.bias_out = a.bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
@@ -591,14 +653,14 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     e.bias_ld = a.v;
     yp_tile_plan tp = p.dzp;
     tp.tiles_i = (nv + tp.bi - 1) / tp.bi;
-    CL_TRY(yp_launch_gemm<TYPE>(tp, g, e, st));
+    CL_TRY(yp_launch_gemm<TYPE, SPLIT>(tp, g, e, st));
     // dw[v][d] = sum_n dz[n][v] h[n][d]
     yp_gemm gw = {};
-    gw.a = ws + p.o_hc; gw.lda = p.kd; gw.I = a.d;
-    gw.b = ws + p.o_dz; gw.ldb = (int64_t)kv * b; gw.J = nv;
-    gw.K = (int)p.kn; gw.steps = (int)(p.kn * b / YP_TILE_KB);
+    gw.a = ws + p.o_hc; gw.lda = p.kd; gw.I = a.d; gw.aplane = hplane; gw.bplane = dzplane;
+    gw.b = ws + p.o_dz; gw.ldb = (int64_t)kv * tb; gw.J = nv;
+    gw.K = (int)p.kn; gw.steps = (int)(p.kn * tb / YP_TILE_KB);
     char* const gwo = (char*)a.grad_weight + v0 * row;
-    yp_epi_store ew = {};
+    yp_epi_store<ELEM> ew = {};
     ew.out = gwo; ew.ld = a.d; ew.scale = back;
     ew.vec = row % 16 == 0 && ((uintptr_t)a.grad_weight & 15) == 0;
     ew.part_vec = a.d % 4 == 0;
@@ -607,16 +669,16 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     twp.tiles_j = (nv + twp.bj - 1) / twp.bj;
     // dh[n][d] (+)= sum_v dz[n][v] w[v][d]
     yp_gemm gh = {};
-    gh.a = w; gh.lda = copy_w ? p.kd : row; gh.I = a.d;
-    gh.b = ws + p.o_dz; gh.ldb = (int64_t)kv * b; gh.J = a.n;
-    gh.K = nv; gh.steps = (int)((int64_t)kv * b / YP_TILE_KB);
-    yp_epi_store eh = {};
+    gh.a = w; gh.lda = copy_w ? p.kd : row; gh.I = a.d; gh.aplane = wplane; gh.bplane = dzplane;
+    gh.b = ws + p.o_dz; gh.ldb = (int64_t)kv * tb; gh.J = a.n;
+    gh.K = nv; gh.steps = (int)((int64_t)kv * tb / YP_TILE_KB);
+    yp_epi_store<ELEM> eh = {};
     eh.out = a.grad_features; eh.ld = a.d; eh.scale = back;
     eh.vec = row % 16 == 0 && ((uintptr_t)a.grad_features & 15) == 0;
     eh.part_vec = a.d % 4 == 0;
     eh.part = dh_joined ? dhpart : nullptr;
     eh.add = s > 0;
-    CL_TRY(yp_launch_two<TYPE>(twp, gw, ew, p.dhp, gh, eh, st));
+    CL_TRY(yp_launch_two<TYPE, SPLIT>(twp, gw, ew, p.dhp, gh, eh, st));
     if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, (int64_t)nv * a.d, gwo);
     if (s == p.pieces - 1) {
       if (dh_joined) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features);
@@ -630,12 +692,16 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
 
 hipError_t yp_launch_class_loss(const yp_class_loss_args& a, hipStream_t st) {
   if (a.n == 0) return a.reduced ? zero(a.reduced, 3, YP_F32, st) : hipSuccess;
-  return a.type == YP_F32 ? forward_t<YP_T_F32>(a, st) : a.type == YP_BF16 ? forward_t<YP_T_BF16>(a, st) : forward_t<YP_T_F16>(a, st);
+  const bool split = plan_class_loss(a.n, a.v, a.d, a.type, false, false).split;
+  return a.type == YP_BF16 ? forward_t<YP_T_BF16, YP_T_BF16, false>(a, st) : a.type == YP_F16 ? forward_t<YP_T_F16, YP_T_F16, false>(a, st)
+       : split ? forward_t<YP_T_BF16, YP_T_F32, true>(a, st) : forward_t<YP_T_F32, YP_T_F32, false>(a, st);
 }
 hipError_t yp_launch_class_loss_backward(const yp_class_loss_args& a, hipStream_t st) {
   if (a.n == 0) {
     CL_TRY(zero(a.grad_weight, (int64_t)a.v * a.d, a.type, st));
     return a.bias ? zero(a.grad_bias, a.v, a.type, st) : hipSuccess;
   }
-  return a.type == YP_F32 ? backward_t<YP_T_F32>(a, st) : a.type == YP_BF16 ? backward_t<YP_T_BF16>(a, st) : backward_t<YP_T_F16>(a, st);
+  const bool split = plan_class_loss(a.n, a.v, a.d, a.type, false, false).split;
+  return a.type == YP_BF16 ? backward_t<YP_T_BF16, YP_T_BF16, false>(a, st) : a.type == YP_F16 ? backward_t<YP_T_F16, YP_T_F16, false>(a, st)
+       : split ? backward_t<YP_T_BF16, YP_T_F32, true>(a, st) : backward_t<YP_T_F32, YP_T_F32, false>(a, st);
 }

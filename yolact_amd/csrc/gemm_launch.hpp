@@ -63,26 +63,25 @@ static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I
 static inline yp_gemm yp_with_plan(yp_gemm g, const yp_tile_plan& p) { g.tiles_i = p.tiles_i; g.tiles_j = p.tiles_j; g.splits = p.splits; return g; }
 static inline int64_t yp_plan_workgroups(const yp_tile_plan& p) { return (int64_t)p.tiles_i * p.tiles_j * p.splits; }
 
-template <int TYPE, class Epi>
+template <int TYPE, bool SPLIT = false, class Epi>
 static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const Epi& epi, hipStream_t st) {
   const yp_gemm g = yp_with_plan(g0, p);
   const dim3 grid((unsigned)yp_plan_workgroups(p));
-  if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
-  else if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
-  else hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_T, false, false, Epi>), grid, dim3(256), 0, st, g, epi);
+  if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
+  else if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
+  else hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_T, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
   return hipGetLastError();
 }
 
-// the gradient products: the first reads both operands by k, the second A by k and B by rows
-template <int TYPE, class Epi>
+template <int TYPE, bool SPLIT, class Epi>
 static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const Epi& e1, const yp_tile_plan& p2, const yp_gemm& g2, const Epi& e2, hipStream_t st) {
   const yp_gemm a = yp_with_plan(g1, p1), b = yp_with_plan(g2, p2);
   const int n1 = (int)yp_plan_workgroups(p1);
   const int second_first = b.steps / b.splits > a.steps / a.splits;   // the longer ones first: the short ones fill up the end
   const dim3 grid((unsigned)(n1 + yp_plan_workgroups(p2)));
-  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
-  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
-  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, true, true, true, false, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
+  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SPLIT, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
+  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, SPLIT, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
+  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, SPLIT, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
   return hipGetLastError();
 }
 
@@ -90,22 +89,9 @@ __device__ __forceinline__ float yp_load_as_float(const void* p, int64_t i, int 
   return type == YP_F32 ? reinterpret_cast<const float*>(p)[i]
        : type == YP_BF16 ? (float)reinterpret_cast<const __bf16*>(p)[i] : (float)reinterpret_cast<const _Float16*>(p)[i];
 }
-// four consecutive values at element i of p, the first `n` of them; VEC: the address is aligned to the four of them
-template <int TYPE, bool VEC>
-__device__ __forceinline__ void yp_store4(void* p, int64_t i, const yp_f4 v, int n) {
-  typedef typename yp_type<TYPE>::elem elem;
-  typedef elem e4 __attribute__((ext_vector_type(4)));
-  elem* const at = reinterpret_cast<elem*>(p) + i;
-  if (VEC && n >= 4) {
-    *reinterpret_cast<e4*>(at) = e4{(elem)v.x, (elem)v.y, (elem)v.z, (elem)v.w};
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) if (r < n) at[r] = (elem)v[r];
-  }
-}
-
-// out[j][i] = scale * C, in the operands' type; or, with `part`, the f32 sums of this split for a later join
+// out[j][i] = scale * C, in type OUT; or, with `part`, the f32 sums of this split for a later join
 // (part[split][j][i], added to what is there if `add`).
+template <int OUT>
 struct yp_epi_store {
   void* out;
   int64_t ld;             // elements
@@ -122,7 +108,7 @@ struct yp_epi_store {
       else yp_put_tile<YP_T_F32, SHAPE, false, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
     } else {
       const float sc = scale ? *scale : 1.0f;
-      yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, out, ld, g.I, g.J, vec != 0, [&](int m, int n) { return acc[m][n] * sc; });
+      yp_put_tile<OUT, SHAPE, false, MI, NJ>(at, out, ld, g.I, g.J, vec != 0, [&](int m, int n) { return acc[m][n] * sc; });
     }
   }
 };

@@ -50,7 +50,15 @@ struct yp_gemm {
   int steps;          // steps of 128 bytes of k
   int splits;         // the steps are dealt to this many workgroups per tile (epilogues that take a split only)
   int tiles_i, tiles_j;
+  int64_t aplane, bplane;   // SPLIT: bytes between the planes
 };
+
+// SPLIT: f32 operands as the sum of three bf16 planes each (24 bits: exact), and of the nine products of planes the six
+// whose terms are not below 2^-24 of the result - the same product over a k axis six times as long.  The bf16 matrix
+// instructions are 16 times as fast as the f32 ones: 6 of them for one.  Sums are f32 as ever.  Segment by segment:
+#define YP_SEGMENTS 6
+#define YP_SEGMENT_A(s) ((0x201100 >> (4 * (s))) & 3)
+#define YP_SEGMENT_B(s) ((0x021010 >> (4 * (s))) & 3)
 
 #ifdef __HIPCC__
 template <int V> struct yp_const { static constexpr int value = V; };
@@ -185,11 +193,11 @@ struct yp_side {
       else fbase = (g * 8 + (t >> 2)) * HB + (((w * (HB / W / 16) + ((t & 3) >> 1)) ^ swizzle(g * 8 + (t >> 2))) * 16) + (t & 1) * 8;
     }
   }
-  // load u of half x of step k, into a buffer `at` bytes into the LDS
-  __device__ __forceinline__ void load(int at, int k, int x, int u) const {
+  // load u of half x of step k, which begins `from` bytes after the base, into a buffer `at` bytes into the LDS
+  __device__ __forceinline__ void load(int at, int64_t from, int k, int x, int u) const {
     const uint32_t to = lds + (uint32_t)(at + x * HALF + u * 1024);
-    if constexpr (!BY_K) yp_load_lds16(base + k * stride, off[x][u], to);
-    else yp_load_lds16(base + k * stride, min(off[x][u], (uint32_t)(min(K - k * KR, KR) - 1) * ld + colmax), to);
+    if constexpr (!BY_K) yp_load_lds16(base + from, off[x][u], to);
+    else yp_load_lds16(base + from, min(off[x][u], (uint32_t)(min(K - k * KR, KR) - 1) * ld + colmax), to);
   }
   // fragment f of half x, half step q
   __device__ __forceinline__ frag read(const char* buf, int x, int f, int q) const {
@@ -233,7 +241,7 @@ struct yp_place {
 // step s + 2 go into the buffer of step s in two groups, A0 B0 in p0 and p1 of s, B1 A1 in p2 and p3, each group a step
 // and a half before it is read.  (With the whole buffer loaded at once, half a step to a step before: 1057 TFLOP/s.  With
 // more stages of 64 bytes of k, every cache line fetched twice: 985.  This: 1257.  bf16, 16384 x 8192 x 4096.)
-template <int TYPE, int SHAPE, bool A_BY_K, bool B_BY_K, class Epi>
+template <int TYPE, int SHAPE, bool A_BY_K, bool B_BY_K, bool SPLIT, class Epi>
 __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, int wg, int nwg, char* lds) {
   typedef typename yp_type<TYPE>::frag frag;
   typedef typename yp_type<TYPE>::acc accv;
@@ -248,7 +256,8 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   yp_tile_of(g, wg, nwg, at.ti, at.tj, at.split);
   at.wi = wave % WI; at.wj = wave / WI;
   at.lds = lds;
-  const int k0 = (int)((int64_t)g.steps * at.split / g.splits), k1 = (int)((int64_t)g.steps * (at.split + 1) / g.splits);
+  const int steps = SPLIT ? g.steps * YP_SEGMENTS : g.steps;
+  const int k0 = (int)((int64_t)steps * at.split / g.splits), k1 = (int)((int64_t)steps * (at.split + 1) / g.splits);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   typedef yp_side<TYPE, BM, WAVES, WI, A_BY_K> SA;
   typedef yp_side<TYPE, BN, WAVES, WJ, B_BY_K> SB;
@@ -269,9 +278,26 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   auto read_b = [&](int buf, int x, int q) { b[x][q >> 1][q & 1] = sb.read(lds + buf * BUF + BM * YP_TILE_KB, x, q >> 1, q & 1); };
   typedef yp_const<0> E0; typedef yp_const<1> E1; typedef yp_const<2> E2;
 
+  // the step to load: k, and where it begins in a and b
+  int lk = 0, ls = 0, todo = 0;
+  int64_t from_a = 0, from_b = 0;
+  auto place = [&]() {
+    from_a = lk * sa.stride + (SPLIT ? YP_SEGMENT_A(ls) * g.aplane : 0);
+    from_b = lk * sb.stride + (SPLIT ? YP_SEGMENT_B(ls) * g.bplane : 0);
+  };
+  // past the last step the last one is loaded again: the number of loads in flight, which the waits count, is always the
+  // same
+  auto advance = [&]() {
+    if (todo > 0) {
+      --todo;
+      if (SPLIT && lk + 1 == g.steps) { lk = 0; ++ls; } else ++lk;
+      place();
+    }
+  };
+
   // products of half X of A and half Y of B; meanwhile reads half RX of A (RD = 1) or of B (RD = 2) in rbuf, and loads
-  // half LX of A (LD = 1) or of B (LD = 2) of step lk into lbuf.  2 MH groups of NH products, the reads first in each.
-  auto phase = [&](auto X, auto Y, auto RD, auto RX, int rbuf, auto LD, auto LX, int lbuf, int lk) {
+  // half LX of A (LD = 1) or of B (LD = 2) of the step to load into lbuf.  2 MH groups of NH products, the reads first in each.
+  auto phase = [&](auto X, auto Y, auto RD, auto RX, int rbuf, auto LD, auto LX, int lbuf) {
     constexpr int x = decltype(X)::value, y = decltype(Y)::value, rdk = decltype(RD)::value, rx = decltype(RX)::value;
     constexpr int ldk = decltype(LD)::value, lx = decltype(LX)::value;
     constexpr int G = 2 * MH, RN = rdk == 1 ? 2 * MH : rdk == 2 ? 2 * NH : 0, LN = ldk == 1 ? SA::P : ldk == 2 ? SB::P : 0;
@@ -286,8 +312,8 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
       }
 #pragma unroll
       for (; ld * G < (gi + 1) * LN; ++ld) {
-        if constexpr (ldk == 1) sa.load(lbuf * BUF, lk, lx, ld);
-        else if constexpr (ldk == 2) sb.load(lbuf * BUF, lk, lx, ld);
+        if constexpr (ldk == 1) sa.load(lbuf * BUF, from_a, lk, lx, ld);
+        else if constexpr (ldk == 2) sb.load(lbuf * BUF, from_b, lk, lx, ld);
       }
       if constexpr (INPLACE) {
 #pragma unroll
@@ -308,20 +334,22 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
     }
   };
   if (k0 < k1) {
-    const int last = k1 - 1;
-    // past the last step the last one is loaded again: the number of loads in flight, which the waits count, is always
-    // the same
+    ls = SPLIT ? k0 / g.steps : 0;
+    lk = SPLIT ? k0 - ls * g.steps : k0;
+    todo = k1 - 1 - k0;
+    place();
     constexpr int GROUP = SA::P + SB::P;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int u = 0; u < SA::P; ++u) sa.load(s * BUF, min(k0 + s, last), 0, u);
+      for (int u = 0; u < SA::P; ++u) sa.load(s * BUF, from_a, lk, 0, u);
 #pragma unroll
-      for (int u = 0; u < SB::P; ++u) sb.load(s * BUF, min(k0 + s, last), 0, u);
+      for (int u = 0; u < SB::P; ++u) sb.load(s * BUF, from_b, lk, 0, u);
 #pragma unroll
-      for (int u = 0; u < SB::P; ++u) sb.load(s * BUF, min(k0 + s, last), 1, u);
+      for (int u = 0; u < SB::P; ++u) sb.load(s * BUF, from_b, lk, 1, u);
 #pragma unroll
-      for (int u = 0; u < SA::P; ++u) sa.load(s * BUF, min(k0 + s, last), 1, u);
+      for (int u = 0; u < SA::P; ++u) sa.load(s * BUF, from_a, lk, 1, u);
+      advance();
     }
     yp_arrive<3 * GROUP>();
 #pragma unroll
@@ -330,40 +358,41 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
     for (int q = 0; q < 2 * NH; ++q) read_b(0, 0, q);
     yp_arrive<2 * GROUP>();
     int buf = 0;
-    for (int k = k0; k < last; ++k, buf ^= 1) {
-      const int lk = min(k + 2, last);
-      phase(E0{}, E0{}, E2{}, E1{}, buf, E1{}, E0{}, buf, lk);
-      phase(E0{}, E1{}, E1{}, E1{}, buf, E2{}, E0{}, buf, lk);
+    for (int k = k0; k < k1 - 1; ++k, buf ^= 1) {
+      phase(E0{}, E0{}, E2{}, E1{}, buf, E1{}, E0{}, buf);
+      phase(E0{}, E1{}, E1{}, E1{}, buf, E2{}, E0{}, buf);
       yp_arrive<2 * GROUP>();
-      phase(E1{}, E0{}, E1{}, E0{}, buf ^ 1, E2{}, E1{}, buf, lk);
-      phase(E1{}, E1{}, E2{}, E0{}, buf ^ 1, E1{}, E1{}, buf, lk);
+      phase(E1{}, E0{}, E1{}, E0{}, buf ^ 1, E2{}, E1{}, buf);
+      phase(E1{}, E1{}, E2{}, E0{}, buf ^ 1, E1{}, E1{}, buf);
+      advance();
       yp_arrive<2 * GROUP>();
     }
-    phase(E0{}, E0{}, E2{}, E1{}, buf, E0{}, E0{}, 0, 0);
-    phase(E0{}, E1{}, E1{}, E1{}, buf, E0{}, E0{}, 0, 0);
-    phase(E1{}, E0{}, E0{}, E0{}, 0, E0{}, E0{}, 0, 0);
-    phase(E1{}, E1{}, E0{}, E0{}, 0, E0{}, E0{}, 0, 0);
+    phase(E0{}, E0{}, E2{}, E1{}, buf, E0{}, E0{}, 0);
+    phase(E0{}, E1{}, E1{}, E1{}, buf, E0{}, E0{}, 0);
+    phase(E1{}, E0{}, E0{}, E0{}, 0, E0{}, E0{}, 0);
+    phase(E1{}, E1{}, E0{}, E0{}, 0, E0{}, E0{}, 0);
   }
   if constexpr (INPLACE) yp_settle<MI, NJ>(acc);
   yp_arrive<0>();    // the surplus loads of every wave have landed: the LDS is the epilogue's
   epi.template apply<TYPE, SHAPE, MI, NJ>(g, acc, at);
 }
 
-template <int TYPE, int SHAPE, bool A_BY_K, bool B_BY_K, class Epi>
+template <int TYPE, int SHAPE, bool SPLIT, class Epi>
 __global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_gemm_kernel(const yp_gemm g, const Epi epi) {
   __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
-  yp_gemm_tile<TYPE, SHAPE, A_BY_K, B_BY_K>(g, epi, (int)blockIdx.x, (int)gridDim.x, lds);
+  yp_gemm_tile<TYPE, SHAPE, false, false, SPLIT>(g, epi, (int)blockIdx.x, (int)gridDim.x, lds);
 }
 
-// Two independent products of one tile shape in one launch, n1 workgroups the first one's; with `second_first` the second
+// The two gradient products, of one tile shape, in one launch: the first reads both operands by k, the second A by k and B by
+// rows; n1 workgroups the first one's; with `second_first` the second
 // one's workgroups come first.
-template <int TYPE, int SHAPE, bool A1, bool B1, bool A2, bool B2, class Epi>
+template <int TYPE, int SHAPE, bool SPLIT, class Epi>
 __global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_two_gemms_kernel(const yp_gemm g1, const Epi e1, int n1, const yp_gemm g2, const Epi e2, int second_first) {
   __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
   const int n2 = (int)gridDim.x - n1, wg = (int)blockIdx.x;
   const bool first = second_first ? wg >= n2 : wg < n1;
-  if (first) yp_gemm_tile<TYPE, SHAPE, A1, B1>(g1, e1, second_first ? wg - n2 : wg, n1, lds);
-  else yp_gemm_tile<TYPE, SHAPE, A2, B2>(g2, e2, second_first ? wg : wg - n1, n2, lds);
+  if (first) yp_gemm_tile<TYPE, SHAPE, true, true, SPLIT>(g1, e1, second_first ? wg - n2 : wg, n1, lds);
+  else yp_gemm_tile<TYPE, SHAPE, true, false, SPLIT>(g2, e2, second_first ? wg : wg - n1, n2, lds);
 }
 
 // Where an epilogue's fragment (0, 0), element 0 lies: i and j of this lane.
