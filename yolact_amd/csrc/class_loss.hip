@@ -32,7 +32,8 @@ __device__ __forceinline__ int64_t yp_label_at(const void* labels, int64_t n, in
   return bytes == 8 ? reinterpret_cast<const int64_t*>(labels)[n] : (int64_t)reinterpret_cast<const int32_t*>(labels)[n];
 }
 
-__device__ __forceinline__ float yp_exp_hw(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+#define YP_LOG2E 1.44269504088896341f
+__device__ __forceinline__ float yp_exp_hw(float x) { return __builtin_amdgcn_exp2f(x * YP_LOG2E); }
 
 struct yp_softmax_part { float m, s; };
 __device__ __forceinline__ void yp_join(float& m, float& s, float m2, float s2) {
@@ -93,19 +94,26 @@ struct yp_epi_stats {
       for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[m][n][r]);
-      const float ref = top == -INFINITY ? 0.0f : top;
+      const float ref = top == -INFINITY ? 0.0f : top, c = -ref * YP_LOG2E;
 #pragma unroll
       for (int m = 0; m < MI; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += yp_exp_hw(acc[m][n][r] - ref);
-      if (j < g.J) {
-        const int64_t l = labels.at(j) - first - ib;
-        if (l >= 0 && l < S::BM) {
+        for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][r], YP_LOG2E, c));
+      const int64_t l = j < g.J ? labels.at(j) - first - ib : -1;
+      const bool mine = l >= 0 && l < S::BM;
+      if (__builtin_amdgcn_ballot_w64(mine)) {      // (mostly no lane of the wave)
+        const int at_l = mine ? (int)l : -1;
+        float z = 0.0f;
+        bool found = false;
 #pragma unroll
-          for (int m = 0; m < MI; ++m)
+        for (int m = 0; m < MI; ++m)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) if (l == yp_frag_at<S::BM, MI>(m) + r) picked[j] = acc[m][n][r];
-        }
+          for (int r = 0; r < 4; ++r) {
+            const bool is = at_l == yp_frag_at<S::BM, MI>(m) + r;
+            z = is ? acc[m][n][r] : z;
+            found |= is;
+          }
+        if (found) picked[j] = z;
       }
 #pragma unroll
       for (int x = 16; x < 64; x <<= 1) yp_join(top, sum, __shfl_xor(top, x), __shfl_xor(sum, x));
@@ -138,30 +146,40 @@ struct yp_epi_dz {
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
     const float over = count ? 1.0f / fmaxf(*count, 1.0f) : 1.0f, up = factor ? factor[0] : 1.0f;
-    const bool edge = bias || (at.ti + 1) * S::BM > g.I;
-    float b[MI][4];
-#pragma unroll
-    for (int m = 0; m < MI; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = ib + yp_frag_at<S::BM, MI>(m) + r;
-        b[m][r] = !edge ? 0.0f : i >= g.I ? -INFINITY : (bias ? yp_load_as_float(bias, i, ELEM) : 0.0f);
-      }
-#pragma unroll
-    for (int n = 0; n < NJ; ++n) {
-      const int j = jb + yp_frag_at<S::BN, NJ>(n);
-      const int label = j < g.J ? labels.counted(j) : -1;
-      const float l = label >= 0 ? lse[j] : 0.0f;
-      const float gr = label >= 0 ? grad[(int64_t)j * grad_stride] * over * up : 0.0f;
-      const int hit = label - first - ib;
+    if (bias || (at.ti + 1) * S::BM > g.I) {      // a class that takes no part, or does not exist: z = -inf
 #pragma unroll
       for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float p = l == -INFINITY ? 0.0f : yp_exp_hw(acc[m][n][r] + b[m][r] - l);
-          if (hit == yp_frag_at<S::BM, MI>(m) + r) p -= 1.0f;
-          acc[m][n][r] = label < 0 || b[m][r] == -INFINITY ? 0.0f : p * gr;
+          const int i = ib + yp_frag_at<S::BM, MI>(m) + r;
+          const float b = i >= g.I ? -INFINITY : (bias ? yp_load_as_float(bias, i, ELEM) : 0.0f);
+#pragma unroll
+          for (int n = 0; n < NJ; ++n) acc[m][n][r] = b == -INFINITY ? -INFINITY : acc[m][n][r] + b;
         }
+    }
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) {
+      const int j = jb + yp_frag_at<S::BN, NJ>(n);
+      const int label = j < g.J ? labels.counted(j) : -1;
+      const float l = label >= 0 ? lse[j] : INFINITY;
+      const float gr = label >= 0 ? grad[(int64_t)j * grad_stride] * over * up : 0.0f;
+      // exp(z - lse) = 2^(z log2e + c); a row that takes no part, or has no class left: 2^-inf = 0
+      const float c = l == -INFINITY ? -INFINITY : -l * YP_LOG2E;
+      const int hit = label < 0 ? -1 : label - first - ib;
+      if (__builtin_amdgcn_ballot_w64(hit >= 0 && hit < S::BM)) {      // (mostly no lane of the wave)
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float z = acc[m][n][r], p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, YP_LOG2E, c));
+            acc[m][n][r] = (hit == yp_frag_at<S::BM, MI>(m) + r && z != -INFINITY ? p - 1.0f : p) * gr;
+          }
+      } else {
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[m][n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][r], YP_LOG2E, c)) * gr;
+      }
     }
     if (bias_out) {   // sums over the tile's rows: 16 lanes, then the waves that share the classes
       float* const lds = reinterpret_cast<float*>(at.lds);
