@@ -137,8 +137,7 @@ struct yp_epi_dz {
   int64_t plane;               // bytes of one
   int kv, kn;
   void* bias_out;              // of the piece; null without bias
-  float* bias_part;            // [tiles_j][bias_ld] of the piece if there is more than one tile in j, else null
-  int bias_ld;
+  float* bias_part;            // [tiles_j][classes of the piece] if there is more than one tile in j, else null
   template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
   __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], const yp_place& at) const {
     typedef yp_shape<SHAPE> S;
@@ -202,7 +201,7 @@ struct yp_epi_dz {
 #pragma unroll
         for (int w = 0; w < S::WJ; ++w) col += lds[w * S::BM + t];
         if (i < g.I) {
-          if (bias_part) bias_part[(int64_t)at.tj * bias_ld + i] = col;
+          if (bias_part) bias_part[(int64_t)at.tj * g.I + i] = col;
           else reinterpret_cast<elem*>(bias_out)[i] = (elem)(col * (factor ? factor[1] : 1.0f));
         }
       }
@@ -408,10 +407,28 @@ __global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, int6
   }
 }
 
-// Up to three arrays, each out[e] = scale * sum over its parts.  64 elements and 4 waves a workgroup: wave w adds parts
+// The bias gradient: the tiles' column sums added up, a thread a class; workgroup i of those that follow the gradient products.
+struct yp_bias_sum {
+  const float* part;   // [parts][ld]
+  int parts, ld, total, type;
+  const float* scale;
+  void* out;
+  __device__ __forceinline__ void operator()(int i) const {
+    const int e = i * 256 + (int)threadIdx.x;
+    if (e >= total) return;
+    float s = 0.0f;
+    for (int p = 0; p < parts; ++p) s += part[(int64_t)p * ld + e];
+    if (scale) s *= *scale;
+    if (type == YP_F32) reinterpret_cast<float*>(out)[e] = s;
+    else if (type == YP_BF16) reinterpret_cast<__bf16*>(out)[e] = (__bf16)s;
+    else reinterpret_cast<_Float16*>(out)[e] = (_Float16)s;
+  }
+};
+
+// Up to two arrays, each out[e] = scale * sum over its parts.  64 elements and 4 waves a workgroup: wave w adds parts
 // w, w + 4, ... in their order, then the four sums are added in theirs.
 struct yp_sum_job { const float* part; int parts; int64_t stride, total; void* out; };
-struct yp_sum_args { yp_sum_job job[3]; int jobs, out_type; const float* scale; };
+struct yp_sum_args { yp_sum_job job[2]; int jobs, out_type; const float* scale; };
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_sum_args a) {
   __shared__ float red[YP_CL_THREADS / 64][64];
   const int x = (int)threadIdx.x & 63, y = (int)threadIdx.x >> 6;
@@ -540,7 +557,7 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   p.o_hc = take(p.kn * p.kd * planes);
   p.o_wc = take(p.piece * p.kd * planes);
   p.o_dz = take(p.kn * p.kv * planes);
-  p.o_bp = take(has_bias && p.dzp.tiles_j > 1 ? (int64_t)p.dzp.tiles_j * V * 4 : 0);
+  p.o_bp = take(has_bias && p.dzp.tiles_j > 1 ? (int64_t)p.dzp.tiles_j * p.piece * 4 : 0);
   p.o_dwpart = take(p.dwp.splits > 1 ? (int64_t)p.dwp.splits * p.piece * D * 4 : 0);
   p.o_dhpart = take(p.dhp.splits > 1 || p.pieces > 1 ? (int64_t)p.dhp.splits * N * D * 4 : 0);
   p.bwd_total = off;
@@ -637,7 +654,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   }
   const float* const back = factor ? factor + 1 : nullptr;
   float* const dhpart = (float*)(ws + p.o_dhpart);
-  float* const biaspart = p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
+  float* const biaspart = a.bias && p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
   const bool dh_joined = p.dhp.splits > 1 || p.pieces > 1;
   yp_sum_args sums = {};
   sums.out_type = ELEM;
@@ -667,8 +684,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad; e.grad_stride = a.grad_stride; e.count = a.count; e.factor = factor;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
     e.bias_out = a.bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
-    e.bias_part = biaspart ? biaspart + v0 : nullptr;
-    e.bias_ld = a.v;
+    e.bias_part = biaspart;
     yp_tile_plan tp = p.dzp;
     tp.tiles_i = (nv + tp.bi - 1) / tp.bi;
     CL_TRY(yp_launch_gemm<TYPE, SPLIT>(tp, g, e, st));
@@ -696,12 +712,11 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     eh.part_vec = a.d % 4 == 0;
     eh.part = dh_joined ? dhpart : nullptr;
     eh.add = s > 0;
-    CL_TRY(yp_launch_two<TYPE, SPLIT>(twp, gw, ew, p.dhp, gh, eh, st));
+    yp_bias_sum bs = {};
+    bs.part = biaspart; bs.parts = p.dzp.tiles_j; bs.ld = bs.total = nv; bs.type = ELEM; bs.scale = back; bs.out = e.bias_out;
+    CL_TRY(yp_launch_two<TYPE, SPLIT>(twp, gw, ew, p.dhp, gh, eh, bs, biaspart ? (nv + 255) / 256 : 0, st));
     if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, (int64_t)nv * a.d, gwo);
-    if (s == p.pieces - 1) {
-      if (dh_joined) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features);
-      if (a.bias && biaspart) add_sum(sums, biaspart, p.dzp.tiles_j, a.v, a.v, a.grad_bias);
-    }
+    if (s == p.pieces - 1 && dh_joined) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features);
     CL_TRY(sum_parts(sums, st));
     sums.jobs = 0;
   }

@@ -73,15 +73,16 @@ static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const
   return hipGetLastError();
 }
 
-template <int TYPE, bool SPLIT, class Epi>
-static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const Epi& e1, const yp_tile_plan& p2, const yp_gemm& g2, const Epi& e2, hipStream_t st) {
+template <int TYPE, bool SPLIT, class Epi, class Extra>
+static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const Epi& e1, const yp_tile_plan& p2, const yp_gemm& g2, const Epi& e2,
+                                const Extra& extra, int extras, hipStream_t st) {
   const yp_gemm a = yp_with_plan(g1, p1), b = yp_with_plan(g2, p2);
-  const int n1 = (int)yp_plan_workgroups(p1);
+  const int n1 = (int)yp_plan_workgroups(p1), n2 = (int)yp_plan_workgroups(p2);
   const int second_first = b.steps / b.splits > a.steps / a.splits;   // the longer ones first: the short ones fill up the end
-  const dim3 grid((unsigned)(n1 + yp_plan_workgroups(p2)));
-  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SPLIT, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
-  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, SPLIT, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
-  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, SPLIT, Epi>), grid, dim3(256), 0, st, a, e1, n1, b, e2, second_first);
+  const dim3 grid((unsigned)(n1 + n2 + extras));
+  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
   return hipGetLastError();
 }
 

@@ -69,7 +69,7 @@ def _class_loss_forward(features, weight, labels, bias, ignore_index, reduce):
     losses = torch.empty(lead, dtype=torch.float32, device=dev)
     lse = torch.empty(lead, dtype=torch.float32, device=dev)
     reduced = torch.empty((3,), dtype=torch.float32, device=dev) if reduce else None
-    _lib.check(L.yp_class_loss(dev.index, N, V, D, dt, p_h, p_w, p_b, p_y, labels.element_size(), int(ignore_index), _ptr(ws),
+    _lib.check(L.yp_class_loss(dev.index, N, V, D, dt, p_h, p_w, p_b, p_y, labels.element_size(), ignore_index, _ptr(ws),
                                losses.data_ptr(), lse.data_ptr(), _ptr(reduced), _stream(dev)))
     return losses, lse, reduced
 
@@ -81,20 +81,21 @@ def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
 
     A row labelled ``ignore_index`` takes no part (loss 0) whatever its features hold; any other label outside [0, V) has
     loss NaN.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf."""
-    losses, lse, _ = _class_loss_forward(features, weight, labels, bias, ignore_index, False)
+    losses, lse, _ = _class_loss_forward(features, weight, labels, bias, int(ignore_index), False)
     return losses, lse
 
 
-def _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad, per_row, count):
-    p_h, p_w, p_b, p_y, N, V, D, lead, dev = _class_loss_args(features, weight, labels, bias)
-    p_l = _check("lse", lse, (torch.float32,), lead, dev)
-    p_g = _check("grad_losses", grad, (torch.float32,), lead if per_row else (), dev)
+def _class_loss_backward(features, weight, labels, bias, ignore_index, lse, p_grad, per_row, p_count):
+    """The call itself, on checked tensors."""
+    V, D = weight.shape
+    N, dev = labels.numel(), weight.device
     L, dt = _lib.load(), _TYPES[weight.dtype]
     ws = _workspace(L.yp_class_loss_workspace(N, V, D, dt, bias is not None, 1), dev)
     gh, gw = torch.empty_like(features), torch.empty_like(weight)
     gb = torch.empty_like(bias) if bias is not None else None
-    _lib.check(L.yp_class_loss_backward(dev.index, N, V, D, dt, p_h, p_w, p_b, p_y, labels.element_size(), int(ignore_index), p_l,
-                                        p_g, int(per_row), _ptr(count), _ptr(ws), gh.data_ptr(), gw.data_ptr(), _ptr(gb), _stream(dev)))
+    _lib.check(L.yp_class_loss_backward(dev.index, N, V, D, dt, features.data_ptr(), weight.data_ptr(), _ptr(bias), labels.data_ptr(),
+                                        labels.element_size(), ignore_index, lse.data_ptr(), p_grad, per_row, p_count, _ptr(ws),
+                                        gh.data_ptr(), gw.data_ptr(), _ptr(gb), _stream(dev)))
     return gh, gw, gb
 
 
@@ -102,7 +103,10 @@ def class_loss_backward(features, weight, labels, lse, grad_losses, bias=None, i
     """Gradients of ``class_loss``'s losses: ``(grad_features, grad_weight, grad_bias or None)`` given ``lse`` as the forward
     returned it for the same inputs and ``grad_losses`` (float32, the shape of ``labels``).  The logits are computed again,
     in pieces of the vocabulary; sums run in float32 in a fixed order, each gradient is rounded once."""
-    return _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad_losses, True, None)
+    lead, dev = _class_loss_args(features, weight, labels, bias)[-2:]
+    _check("lse", lse, (torch.float32,), lead, dev)
+    p_grad = _check("grad_losses", grad_losses, (torch.float32,), lead, dev)
+    return _class_loss_backward(features, weight, labels, bias, int(ignore_index), lse, p_grad, 1, None)
 
 
 class ClassLoss(torch.autograd.Function):
@@ -117,18 +121,20 @@ class ClassLoss(torch.autograd.Function):
             raise ValueError(f"reduction must be one of {_REDUCTIONS}")
         features, weight, labels = features.contiguous(), weight.contiguous(), labels.contiguous()
         bias = bias.contiguous() if bias is not None else None
+        ignore_index = int(ignore_index)
         losses, lse, reduced = _class_loss_forward(features, weight, labels, bias, ignore_index, reduction != "none")
         ctx.save_for_backward(features, weight, bias, labels, lse, reduced)
-        ctx.cfg = (int(ignore_index), reduction)
-        return losses if reduction == "none" else reduced[_REDUCTIONS.index(reduction) - 1]
+        ctx.cfg = (ignore_index, reduction)
+        return losses if reduction == "none" else reduced.select(0, 0 if reduction == "sum" else 1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         features, weight, bias, labels, lse, reduced = ctx.saved_tensors
         ignore_index, reduction = ctx.cfg
-        gh, gw, gb = _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad.contiguous(), reduction == "none",
-                                          reduced[2:] if reduction == "mean" else None)
+        grad = grad.contiguous()             # (float32 and of the result's shape: autograd has seen to it)
+        gh, gw, gb = _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad.data_ptr(), int(reduction == "none"),
+                                          reduced.data_ptr() + 8 if reduction == "mean" else None)
         return gh, gw, gb, None, None, None
 
 
