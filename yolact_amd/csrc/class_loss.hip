@@ -14,8 +14,10 @@
 // epilogue that turns z into dz [row][class]; then both gradient products in one launch, which read dz, h and w as they
 // lie ("by k", gemm_tile.hpp): dw's piece is complete, dh adds up over the pieces in f32.
 // dz is rounded to the features' type - the matrix instruction takes nothing wider beside h and w; each dz is off by
-// half a step of that type, like the gradients themselves - f16 with a power-of-two factor that brings the largest
-// |g| to [2^13, 2^14), so that probabilities down to 2^-38 of it are kept, taken out again in f32 at the end.
+// half a step of that type, like the gradients themselves.  It is held relative to the largest |g| - one g for all rows
+// is taken out altogether -, which the results get back in f32: with g inside, every row's -g would be rounded the same
+// way, and sums over rows be off by as much as one of them.  f16 with 2^13 more, so that probabilities down to 2^-38 are
+// kept.
 // f32 of any size worth it runs on the bf16 matrix instructions, as three bf16 planes per operand (SPLIT, gemm_tile.hpp).
 // What takes no part has dz = 0, but 0 times NaN is NaN: the gradient products read a copy of h in which ignored rows are
 // zero (and of w, if a bias may mask classes).
@@ -128,10 +130,10 @@ struct yp_epi_dz {
   const void* bias;            // of the tensors' type ELEM; of the piece
   const float* lse;
   yp_labels labels;
-  const float* grad;
-  int grad_stride;
-  const float* count;          // null: grads are the rows' own; else divided by max(count, 1)
-  const float* factor;         // f16: {2^e, 2^-e}, else null
+  const float* grad;           // of every row, times *factor (if there is one); null: `up` for all of them
+  const float* factor;
+  float up;
+  yp_scale scale;              // what the gradients get back
   int first;                   // first class of the piece
   void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv); SPLIT: three planes of it, bf16
   int64_t plane;               // bytes of one
@@ -144,7 +146,7 @@ struct yp_epi_dz {
     typedef typename yp_type<ELEM>::elem elem;
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
-    const float over = count ? 1.0f / fmaxf(*count, 1.0f) : 1.0f, up = factor ? factor[0] : 1.0f;
+    const float by = grad && factor ? *factor : up;
     if (bias || (at.ti + 1) * S::BM > g.I) {      // a class that takes no part, or does not exist: z = -inf
 #pragma unroll
       for (int m = 0; m < MI; ++m)
@@ -161,7 +163,7 @@ struct yp_epi_dz {
       const int j = jb + yp_frag_at<S::BN, NJ>(n);
       const int label = j < g.J ? labels.counted(j) : -1;
       const float l = label >= 0 ? lse[j] : INFINITY;
-      const float gr = label >= 0 ? grad[(int64_t)j * grad_stride] * over * up : 0.0f;
+      const float gr = label < 0 ? 0.0f : grad ? grad[j] * by : by;
       // exp(z - lse) = 2^(z log2e + c); a row that takes no part, or has no class left: 2^-inf = 0
       const float c = l == -INFINITY ? -INFINITY : -l * YP_LOG2E;
       const int hit = label < 0 ? -1 : label - first - ib;
@@ -202,7 +204,7 @@ struct yp_epi_dz {
         for (int w = 0; w < S::WJ; ++w) col += lds[w * S::BM + t];
         if (i < g.I) {
           if (bias_part) bias_part[(int64_t)at.tj * g.I + i] = col;
-          else reinterpret_cast<elem*>(bias_out)[i] = (elem)(col * (factor ? factor[1] : 1.0f));
+          else reinterpret_cast<elem*>(bias_out)[i] = (elem)yp_times(col, scale.get());
         }
       }
       yp_arrive<0>();
@@ -387,23 +389,28 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_reduce_kernel(const double* 
   if (threadIdx.x == 0) yp_write_reduced(reduced, ts, tc);
 }
 
-// f16: the power of two that brings the largest |g| to [2^13, 2^14), and its inverse
-__global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, int64_t n, const float* count, float* factor) {
+// {by / largest |g|, largest |g| / by}
+__global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, int64_t n, float by, float* factor) {
   __shared__ float red[16];
   float top = 0.0f;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, fabsf(grad[i]));
+  int64_t i = threadIdx.x;
+  for (; i + 3 * 1024 < n; i += 4 * 1024) {
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = grad[i + u * 1024];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = fmaxf(top, fabsf(v[u]));
+  }
+  for (; i < n; i += 1024) top = fmaxf(top, fabsf(grad[i]));
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
-    if (count) top /= fmaxf(*count, 1.0f);
-    int e = 0;
-    if (top > 0.0f && top < INFINITY) e = 13 - ilogbf(top);
-    e = min(max(e, -100), 100);
-    factor[0] = ldexpf(1.0f, e);
-    factor[1] = ldexpf(1.0f, -e);
+    if (!(top >= 0x1p-100f && top <= 0x1p100f)) top = 1.0f;      // (nothing to go by)
+    factor[0] = by / top;
+    factor[1] = top / by;
   }
 }
 
@@ -411,14 +418,14 @@ __global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, int6
 struct yp_bias_sum {
   const float* part;   // [parts][ld]
   int parts, ld, total, type;
-  const float* scale;
+  yp_scale scale;
   void* out;
   __device__ __forceinline__ void operator()(int i) const {
     const int e = i * 256 + (int)threadIdx.x;
     if (e >= total) return;
     float s = 0.0f;
     for (int p = 0; p < parts; ++p) s += part[(int64_t)p * ld + e];
-    if (scale) s *= *scale;
+    s = yp_times(s, scale.get());
     if (type == YP_F32) reinterpret_cast<float*>(out)[e] = s;
     else if (type == YP_BF16) reinterpret_cast<__bf16*>(out)[e] = (__bf16)s;
     else reinterpret_cast<_Float16*>(out)[e] = (_Float16)s;
@@ -428,11 +435,11 @@ struct yp_bias_sum {
 // Up to two arrays, each out[e] = scale * sum over its parts.  64 elements and 4 waves a workgroup: wave w adds parts
 // w, w + 4, ... in their order, then the four sums are added in theirs.
 struct yp_sum_job { const float* part; int parts; int64_t stride, total; void* out; };
-struct yp_sum_args { yp_sum_job job[2]; int jobs, out_type; const float* scale; };
+struct yp_sum_args { yp_sum_job job[2]; int jobs, out_type; yp_scale scale; };
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_sum_args a) {
   __shared__ float red[YP_CL_THREADS / 64][64];
   const int x = (int)threadIdx.x & 63, y = (int)threadIdx.x >> 6;
-  const float sc = a.scale ? *a.scale : 1.0f;
+  const float sc = a.scale.get();
   auto put = [&](void* out, int64_t e, float s) {
     if (a.out_type == YP_F32) reinterpret_cast<float*>(out)[e] = s;
     else if (a.out_type == YP_BF16) reinterpret_cast<__bf16*>(out)[e] = (__bf16)s;
@@ -444,7 +451,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_su
       for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < b.total; e += (int64_t)gridDim.x * YP_CL_THREADS) {
         float s = 0.0f;
         for (int p = 0; p < b.parts; ++p) s += b.part[(int64_t)p * b.stride + e];
-        put(b.out, e, s * sc);
+        put(b.out, e, yp_times(s, sc));
       }
       continue;
     }
@@ -465,7 +472,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_su
       __syncthreads();
       red[y][x] = s;
       __syncthreads();
-      if (y == 0 && e < b.total) put(b.out, e, (((red[0][x] + red[1][x]) + red[2][x]) + red[3][x]) * sc);
+      if (y == 0 && e < b.total) put(b.out, e, yp_times(((red[0][x] + red[1][x]) + red[2][x]) + red[3][x], sc));
     }
   }
 }
@@ -491,6 +498,7 @@ static void add_sum(yp_sum_args& a, const float* part, int parts, int64_t stride
 static hipError_t zero(void* out, int64_t n, int type, hipStream_t st) {   // (a kernel, not a memset: the call may be captured)
   yp_sum_args a = {};
   a.out_type = type;
+  a.scale.by = 1.0f;
   add_sum(a, nullptr, 0, 0, n, out);
   return sum_parts(a, st);
 }
@@ -647,12 +655,18 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   const bool copy_w = SPLIT || a.bias || row % YP_TILE_KB != 0 || ((uintptr_t)a.weight & 15) != 0;
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
-  float* const factor = TYPE == YP_T_F16 ? (float*)(ws + p.o_factor) : nullptr;
-  if (factor) {
-    hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, a.grad_stride ? (int64_t)a.n : (int64_t)1, a.count, factor);
-    CL_TRY(hipGetLastError());
+  const float up = ELEM == YP_T_F16 ? 8192.0f : 1.0f;
+  float* factor = nullptr;
+  yp_scale back = {a.grad, a.count, 1.0f / up};             // one g for all rows
+  if (a.grad_stride) {
+    back = yp_scale{nullptr, a.count, 1.0f};
+    if (ELEM != YP_T_F32) {                                 // (f32: dz is not rounded)
+      factor = (float*)(ws + p.o_factor);
+      hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, (int64_t)a.n, up, factor);
+      CL_TRY(hipGetLastError());
+      back.a = factor + 1;
+    }
   }
-  const float* const back = factor ? factor + 1 : nullptr;
   float* const dhpart = (float*)(ws + p.o_dhpart);
   float* const biaspart = a.bias && p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
   const bool dh_joined = p.dhp.splits > 1 || p.pieces > 1;
@@ -681,7 +695,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     g.I = nv; g.J = a.n; g.steps = (int)(p.kd / YP_TILE_KB);
     yp_epi_dz<ELEM, SPLIT> e;
     e.plane = dzplane;
-    e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad; e.grad_stride = a.grad_stride; e.count = a.count; e.factor = factor;
+    e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = up; e.scale = back;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
     e.bias_out = a.bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
     e.bias_part = biaspart;

@@ -90,6 +90,16 @@ __device__ __forceinline__ float yp_load_as_float(const void* p, int64_t i, int 
   return type == YP_F32 ? reinterpret_cast<const float*>(p)[i]
        : type == YP_BF16 ? (float)reinterpret_cast<const __bf16*>(p)[i] : (float)reinterpret_cast<const _Float16*>(p)[i];
 }
+// A factor that lies on the device: by * (a ? *a : 1) / (count ? max(*count, 1) : 1).
+struct yp_scale {
+  const float* a;
+  const float* count;
+  float by;
+  __device__ __forceinline__ float get() const { return (a ? *a : 1.0f) * by / (count ? fmaxf(*count, 1.0f) : 1.0f); }
+};
+// (what is exactly zero stays so, whatever the factor)
+__device__ __forceinline__ float yp_times(float v, float scale) { return v == 0.0f ? 0.0f : v * scale; }
+
 // out[j][i] = scale * C, in type OUT; or, with `part`, the f32 sums of this split for a later join
 // (part[split][j][i], added to what is there if `add`).
 template <int OUT>
@@ -97,7 +107,7 @@ struct yp_epi_store {
   void* out;
   int64_t ld;             // elements
   int vec, part_vec;      // rows of out / of part are multiples of 16 bytes
-  const float* scale;     // device scalar, null = 1
+  yp_scale scale;
   float* part;
   int add;
   template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
@@ -108,8 +118,13 @@ struct yp_epi_store {
       if (add) yp_put_tile<YP_T_F32, SHAPE, true, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
       else yp_put_tile<YP_T_F32, SHAPE, false, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
     } else {
-      const float sc = scale ? *scale : 1.0f;
-      yp_put_tile<OUT, SHAPE, false, MI, NJ>(at, out, ld, g.I, g.J, vec != 0, [&](int m, int n) { return acc[m][n] * sc; });
+      const float sc = scale.get();
+      yp_put_tile<OUT, SHAPE, false, MI, NJ>(at, out, ld, g.I, g.J, vec != 0, [&](int m, int n) {
+        yp_f4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = yp_times(acc[m][n][r], sc);
+        return v;
+      });
     }
   }
 };
