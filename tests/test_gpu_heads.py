@@ -110,7 +110,7 @@ def test_class_loss_nothing_left():
     # no row at all
     h0, y0 = h[:0].clone().requires_grad_(), y[:0]
     loss = heads.ClassLoss.apply(h0, ww, bb, y0, -1, "mean")
-    assert float(loss) == 0.0
+    assert float(loss.detach()) == 0.0
     gs = torch.autograd.grad(loss, (h0, ww, bb))
     assert gs[0].shape == (0, 32) and not gs[1].any() and not gs[2].any()
 
@@ -155,6 +155,20 @@ def test_class_loss_autograd(dt, reduction):
     ref.within(grads[2], *want["grad_b"], "grad_bias")
     again = torch.autograd.grad(loss, (ht, wt, bt), gl)
     assert all(torch.equal(a, c) for a, c in zip(grads, again))                                # same call, same bits
+
+
+@pytest.mark.parametrize("n,v,d", [(60, 130, 40), (20, 9000, 64), (700, 90, 300)])
+def test_class_loss_gradients_that_nobody_needs(n, v, d):
+    from yolact_amd import heads
+    for dt in TYPES:
+        h, w, b, y, up = _loss_inputs(n, v, d, dt, True, 0.2)
+        _, lse = heads.class_loss(h, w, y, bias=b)
+        full = heads.class_loss_backward(h, w, y, lse, up, bias=b)
+        for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1), (1, 0, 1)):
+            leaves = [t.clone().requires_grad_(bool(k)) for t, k in zip((h, w, b), need)]
+            loss = heads.ClassLoss.apply(*leaves, y, -1, "none")
+            got = torch.autograd.grad(loss, [t for t in leaves if t.requires_grad], up)
+            assert all(torch.equal(a, c) for a, c in zip(got, [g for g, k in zip(full, need) if k]))
 
 
 def test_class_loss_gradients_against_differences():
@@ -400,6 +414,30 @@ def test_streams_and_graphs():
             other.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, c) for a, c in zip(outs2, want)), (dt, r)
+
+
+def test_first_call_in_a_graph():
+    """Shapes that no eager call has launched before: the many-row kernel with a large LDS, the few-row one, a split f32 step."""
+    from yolact_amd import heads
+    x, w = torch.randn(5000, 250, generator=_gen(1), device="cuda"), torch.randn(141, 250, generator=_gen(2), device="cuda")
+    wq = heads.quantize_rows(w)
+    h, ww, b, y, up = _loss_inputs(1300, 3001, 600, torch.float32, True, 0.1)
+
+    def step():
+        losses, lse = heads.class_loss(h, ww, y, bias=b)
+        return [heads.quantized_linear(x, wq), heads.quantized_linear(x[:3], wq), losses] + list(heads.class_loss_backward(h, ww, y, lse, up, bias=b))
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for r in range(3):
+        x.mul_(1.1)
+        h.mul_(0.9)
+        want = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(outs, want))
 
 
 def test_autograd_step_in_a_graph():

@@ -798,8 +798,8 @@ extern "C" int yp_class_loss_backward(int32_t device_id, int32_t n, int32_t v, i
   const int rc = check_class_loss("yp_class_loss_backward", a);
   if (rc != YP_OK) return rc;
   if (grad_stride != 0 && grad_stride != 1) return fail(YP_EINVAL, "yp_class_loss_backward: grad_stride must be 0 or 1");
-  if (!grad_weight || (n > 0 && (!grad || !grad_features)) || (bias != nullptr) != (grad_bias != nullptr))
-    return fail(YP_EINVAL, "yp_class_loss_backward: null argument (grad_bias goes with bias)");
+  if ((n > 0 && !grad) || (!grad_features && !grad_weight && !grad_bias)) return fail(YP_EINVAL, "yp_class_loss_backward: null argument");
+  if (grad_bias && !bias) return fail(YP_EINVAL, "yp_class_loss_backward: grad_bias without bias");
   if (!elem_aligned(grad_features, dtype) || !elem_aligned(grad_weight, dtype) || !elem_aligned(grad_bias, dtype) ||
       (((uintptr_t)grad | (uintptr_t)count) & 3) != 0)
     return fail(YP_EINVAL, "yp_class_loss_backward: a tensor is not aligned to its elements");

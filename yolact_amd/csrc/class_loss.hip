@@ -668,7 +668,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     }
   }
   float* const dhpart = (float*)(ws + p.o_dhpart);
-  float* const biaspart = a.bias && p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
+  float* const biaspart = a.grad_bias && p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
   const bool dh_joined = p.dhp.splits > 1 || p.pieces > 1;
   yp_sum_args sums = {};
   sums.out_type = ELEM;
@@ -697,7 +697,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     e.plane = dzplane;
     e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = up; e.scale = back;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
-    e.bias_out = a.bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
+    e.bias_out = a.grad_bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
     e.bias_part = biaspart;
     yp_tile_plan tp = p.dzp;
     tp.tiles_i = (nv + tp.bi - 1) / tp.bi;
@@ -707,12 +707,12 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     gw.a = ws + p.o_hc; gw.lda = p.kd; gw.I = a.d; gw.aplane = hplane; gw.bplane = dzplane;
     gw.b = ws + p.o_dz; gw.ldb = (int64_t)kv * tb; gw.J = nv;
     gw.K = (int)p.kn; gw.steps = (int)(p.kn * tb / YP_TILE_KB);
-    char* const gwo = (char*)a.grad_weight + v0 * row;
+    char* const gwo = a.grad_weight ? (char*)a.grad_weight + v0 * row : nullptr;
     yp_epi_store<ELEM> ew = {};
     ew.out = gwo; ew.ld = a.d; ew.scale = back;
     ew.vec = row % 16 == 0 && ((uintptr_t)a.grad_weight & 15) == 0;
     ew.part_vec = a.d % 4 == 0;
-    ew.part = p.dwp.splits > 1 ? (float*)(ws + p.o_dwpart) : nullptr;
+    ew.part = gwo && p.dwp.splits > 1 ? (float*)(ws + p.o_dwpart) : nullptr;
     yp_tile_plan twp = p.dwp;
     twp.tiles_j = (nv + twp.bj - 1) / twp.bj;
     // dh[n][d] (+)= sum_v dz[n][v] w[v][d]
@@ -730,7 +730,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     bs.part = biaspart; bs.parts = p.dzp.tiles_j; bs.ld = bs.total = nv; bs.type = ELEM; bs.scale = back; bs.out = e.bias_out;
     CL_TRY(yp_launch_two<TYPE, SPLIT>(twp, gw, ew, p.dhp, gh, eh, bs, biaspart ? (nv + 255) / 256 : 0, st));
     if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, (int64_t)nv * a.d, gwo);
-    if (s == p.pieces - 1 && dh_joined) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features);
+    if (s == p.pieces - 1 && dh_joined && a.grad_features) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features);
     CL_TRY(sum_parts(sums, st));
     sums.jobs = 0;
   }
@@ -745,8 +745,8 @@ hipError_t yp_launch_class_loss(const yp_class_loss_args& a, hipStream_t st) {
 }
 hipError_t yp_launch_class_loss_backward(const yp_class_loss_args& a, hipStream_t st) {
   if (a.n == 0) {
-    CL_TRY(zero(a.grad_weight, (int64_t)a.v * a.d, a.type, st));
-    return a.bias ? zero(a.grad_bias, a.v, a.type, st) : hipSuccess;
+    if (a.grad_weight) CL_TRY(zero(a.grad_weight, (int64_t)a.v * a.d, a.type, st));
+    return a.grad_bias ? zero(a.grad_bias, a.v, a.type, st) : hipSuccess;
   }
   const bool split = plan_class_loss(a.n, a.v, a.d, a.type, false, false).split;
   return a.type == YP_BF16 ? backward_t<YP_T_BF16, YP_T_BF16, false>(a, st) : a.type == YP_F16 ? backward_t<YP_T_F16, YP_T_F16, false>(a, st)

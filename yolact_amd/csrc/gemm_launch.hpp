@@ -60,12 +60,14 @@ static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I
 }
 
 #ifdef __HIPCC__
+#define YP_MAX_WORKGROUPS (1 << 24)   // of 256 threads: a launch's work items are counted in 32 bits
 static inline yp_gemm yp_with_plan(yp_gemm g, const yp_tile_plan& p) { g.tiles_i = p.tiles_i; g.tiles_j = p.tiles_j; g.splits = p.splits; return g; }
 static inline int64_t yp_plan_workgroups(const yp_tile_plan& p) { return (int64_t)p.tiles_i * p.tiles_j * p.splits; }
 
 template <int TYPE, bool SPLIT = false, class Epi>
 static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const Epi& epi, hipStream_t st) {
   const yp_gemm g = yp_with_plan(g0, p);
+  if (yp_plan_workgroups(p) >= YP_MAX_WORKGROUPS) return hipErrorInvalidValue;
   const dim3 grid((unsigned)yp_plan_workgroups(p));
   if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
   else if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
@@ -73,11 +75,14 @@ static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const
   return hipGetLastError();
 }
 
+// (either of the two may be left out: no output)
 template <int TYPE, bool SPLIT, class Epi, class Extra>
 static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const Epi& e1, const yp_tile_plan& p2, const yp_gemm& g2, const Epi& e2,
                                 const Extra& extra, int extras, hipStream_t st) {
   const yp_gemm a = yp_with_plan(g1, p1), b = yp_with_plan(g2, p2);
-  const int n1 = (int)yp_plan_workgroups(p1), n2 = (int)yp_plan_workgroups(p2);
+  if (yp_plan_workgroups(p1) + yp_plan_workgroups(p2) + extras >= YP_MAX_WORKGROUPS) return hipErrorInvalidValue;
+  const int n1 = e1.out ? (int)yp_plan_workgroups(p1) : 0, n2 = e2.out ? (int)yp_plan_workgroups(p2) : 0;
+  if (n1 + n2 + extras == 0) return hipSuccess;
   const int second_first = b.steps / b.splits > a.steps / a.splits;   // the longer ones first: the short ones fill up the end
   const dim3 grid((unsigned)(n1 + n2 + extras));
   if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);

@@ -85,17 +85,18 @@ def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
     return losses, lse
 
 
-def _class_loss_backward(features, weight, labels, bias, ignore_index, lse, p_grad, per_row, p_count):
-    """The call itself, on checked tensors."""
+def _class_loss_backward(features, weight, labels, bias, ignore_index, lse, p_grad, per_row, p_count, wanted=(True, True, True)):
+    """The call itself, on checked tensors; gradients that are not wanted are None."""
     V, D = weight.shape
     N, dev = labels.numel(), weight.device
     L, dt = _lib.load(), _TYPES[weight.dtype]
     ws = _workspace(L.yp_class_loss_workspace(N, V, D, dt, bias is not None, 1), dev)
-    gh, gw = torch.empty_like(features), torch.empty_like(weight)
-    gb = torch.empty_like(bias) if bias is not None else None
+    gh = torch.empty_like(features) if wanted[0] else None
+    gw = torch.empty_like(weight) if wanted[1] else None
+    gb = torch.empty_like(bias) if bias is not None and wanted[2] else None
     _lib.check(L.yp_class_loss_backward(dev.index, N, V, D, dt, features.data_ptr(), weight.data_ptr(), _ptr(bias), labels.data_ptr(),
                                         labels.element_size(), ignore_index, lse.data_ptr(), p_grad, per_row, p_count, _ptr(ws),
-                                        gh.data_ptr(), gw.data_ptr(), _ptr(gb), _stream(dev)))
+                                        _ptr(gh), _ptr(gw), _ptr(gb), _stream(dev)))
     return gh, gw, gb
 
 
@@ -112,7 +113,7 @@ def class_loss_backward(features, weight, labels, lse, grad_losses, bias=None, i
 class ClassLoss(torch.autograd.Function):
     """Differentiable class loss: ``ClassLoss.apply(features, weight, bias, labels, ignore_index=-1, reduction="mean")``.
     ``reduction`` "none" gives the rows' losses, "sum" and "mean" one value, "mean" over the rows that are not ignored (0 if
-    there are none).  Gradients flow to features, weight and bias (which may be None).  When forward and backward are
+    there are none).  Gradients flow to features, weight and bias (which may be None); those nobody needs are not computed.  When forward and backward are
     captured into a graph, capture both, on leaves whose eager graphs are gone."""
 
     @staticmethod
@@ -134,7 +135,7 @@ class ClassLoss(torch.autograd.Function):
         ignore_index, reduction = ctx.cfg
         grad = grad.contiguous()             # (float32 and of the result's shape: autograd has seen to it)
         gh, gw, gb = _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad.data_ptr(), int(reduction == "none"),
-                                          reduced.data_ptr() + 8 if reduction == "mean" else None)
+                                          reduced.data_ptr() + 8 if reduction == "mean" else None, ctx.needs_input_grad)
         return gh, gw, gb, None, None, None
 
 
