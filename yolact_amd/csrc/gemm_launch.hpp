@@ -2,6 +2,8 @@
 // and the epilogue that stores a plain product.
 #pragma once
 
+#include <math.h>
+
 #include "gemm_tile.hpp"
 
 struct yp_tile_plan {
@@ -11,8 +13,9 @@ struct yp_tile_plan {
 };
 
 // L 256 x 256 (4 waves of 128 x 128: 256 rows of fragments read for 128 x 128 results), M 128 x 128 (4 waves of 64 x 64,
-// two workgroups a CU), T 64 x 64 (4 waves of 32 x 32, four a CU): the larger, the faster per result once the card is
-// full - 1315, 1088 and about 600 TFLOP/s, bf16 - but a small product leaves most of the card idle with it.
+// two workgroups a CU), T 64 x 64 (4 waves of 32 x 32, five a CU): the larger, the faster per result once the card is
+// full - 1315, 1088 and 650 TFLOP/s, bf16 - but a small product leaves most of the card idle with it, and the more
+// workgroups share a CU, the better one's epilogue hides behind another's products.
 static inline yp_tile_plan yp_plan_shape(int shape, int64_t I, int64_t J) {
   yp_tile_plan p;
   p.shape = shape;
@@ -22,41 +25,45 @@ static inline yp_tile_plan yp_plan_shape(int shape, int64_t I, int64_t J) {
   p.splits = 1;
   return p;
 }
-// Time of `tiles` tiles of a shape, in units of a 64 x 64 tile at the large shape's rate: rounds of what is resident at a
-// time (256 CUs), each as long as the CU's share of them takes.
-static inline int64_t yp_plan_cost(int shape, int64_t tiles) {
-  if (shape == YP_TILE_L) return (tiles + 255) / 256 * 16;
-  if (shape == YP_TILE_M) return tiles <= 256 ? 6 : (tiles + 511) / 512 * 10;
-  return tiles <= 256 ? 2 : tiles <= 512 ? 4 : (tiles + 1023) / 1024 * 8;
+// Microseconds that `wgs` workgroups of `steps` steps each take, fitted to bf16 products from 256 x 256 to 8192 x 8192 with 4
+// to 64 steps (within 15 %); f32 and int8 steps take longer or shorter, but in the same proportions.
+static inline double yp_plan_cost(int shape, double wgs, double steps) {
+  if (shape == YP_TILE_L) return ceil(wgs / 256) * (steps * (wgs > 128 ? 1.57 : 1.2) + 12);
+  if (shape == YP_TILE_M) return wgs <= 256 ? steps * 0.49 + 5 : wgs <= 512 ? steps * 0.79 + 6 : steps * 0.93 * ceil(wgs / 256) / 2 + 6 * ceil(wgs / 512);
+  return wgs <= 256 ? steps * 0.28 + 3 : wgs <= 512 ? steps * 0.45 + 3 : wgs <= 1280 ? steps * 0.75 + 4 : steps * 0.92 * wgs / 1280 + 4 * ceil(wgs / 1280);
 }
-static inline int yp_plan_best(int64_t I1, int64_t J1, int64_t I2, int64_t J2) {   // (J2 = 0: one product)
-  int best = YP_TILE_L;
-  int64_t least = INT64_MAX;
+static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps) {
+  yp_tile_plan best = {};
+  double least = 1e30;
   for (int s = YP_TILE_L; s <= YP_TILE_T; ++s) {
-    const int64_t e = s == YP_TILE_L ? 256 : s == YP_TILE_M ? 128 : 64;
-    const int64_t c = yp_plan_cost(s, (I1 + e - 1) / e * ((J1 + e - 1) / e) + (I2 + e - 1) / e * ((J2 + e - 1) / e));
-    if (c < least) { least = c; best = s; }
+    const yp_tile_plan p = yp_plan_shape(s, I, J);
+    const double c = yp_plan_cost(s, (double)p.tiles_i * p.tiles_j, (double)steps);
+    if (c < least) { least = c; best = p; }
   }
   return best;
 }
-static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J) { return yp_plan_shape(yp_plan_best(I, J, 0, 0), I, J); }
-static inline int yp_plan_waves_i(const yp_tile_plan&) { return 2; }
-
-// Few tiles: deal the k axis to more workgroups, until half of the card is busy or a workgroup has 8 steps left.
-static inline void yp_plan_splits(yp_tile_plan* p, int64_t steps) {
-  const int64_t tiles = (int64_t)p->tiles_i * p->tiles_j, fill = p->shape == YP_TILE_L ? 128 : p->shape == YP_TILE_M ? 256 : 512;
-  if (tiles >= fill) return;
-  int64_t s = fill / tiles;
-  if (s > steps / 8) s = steps / 8;
-  p->splits = s < 1 ? 1 : (int)s;
-}
-// Two products that share a launch, and so a shape.
+// Two products that share a launch, and so a shape, each with its k axis dealt to as many workgroups as pays: their
+// f32 sums are written and read once more (5 TB/s), by another launch.  A workgroup keeps 8 steps at least.
 static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I2, int64_t J2, int64_t steps2, yp_tile_plan* p1, yp_tile_plan* p2) {
-  const int shape = yp_plan_best(I1, J1, I2, J2);
-  *p1 = yp_plan_shape(shape, I1, J1);
-  *p2 = yp_plan_shape(shape, I2, J2);
-  yp_plan_splits(p1, steps1);
-  yp_plan_splits(p2, steps2);
+  double least = 1e30;
+  for (int shape = YP_TILE_L; shape <= YP_TILE_T; ++shape) {
+    yp_tile_plan a = yp_plan_shape(shape, I1, J1), b = yp_plan_shape(shape, I2, J2);
+    const double ta = (double)a.tiles_i * a.tiles_j, tb = (double)b.tiles_i * b.tiles_j;
+    const double alone = shape == YP_TILE_L ? 1.57 : shape == YP_TILE_M ? 0.79 : 0.45;
+    for (int64_t sa = 1; sa == 1 || (sa <= steps1 / 8 && ta * sa <= 1024); sa *= 2)
+      for (int64_t sb = 1; sb == 1 || (sb <= steps2 / 8 && tb * sb <= 1024); sb *= 2) {
+        const double qa = (double)steps1 / sa, qb = (double)steps2 / sb, wgs = ta * sa + tb * sb;
+        const double longest = (qa > qb ? qa : qb) * alone + 5;
+        double c = yp_plan_cost(shape, wgs, (ta * sa * qa + tb * sb * qb) / wgs);
+        if (c < longest) c = longest;
+        if (sa > 1 || sb > 1) c += 6 + ((sa > 1 ? (double)I1 * J1 * sa : 0) + (sb > 1 ? (double)I2 * J2 * sb : 0)) * 8 / 5e6;
+        if (c < least) {
+          least = c;
+          *p1 = a; p1->splits = (int)sa;
+          *p2 = b; p2->splits = (int)sb;
+        }
+      }
+  }
 }
 
 #ifdef __HIPCC__

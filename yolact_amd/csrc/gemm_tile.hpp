@@ -384,13 +384,13 @@ __global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_gemm_kernel(cons
 }
 
 // The two gradient products, of one tile shape, in one launch: the first reads both operands by k, the second A by k and B by
-// rows; n1 and n2 workgroups, with `second_first` the second one's first.  Workgroups past them take `extra(i)`.
+// rows; n1 and n2 workgroups, with `second_first` the second one's first.  Workgroups past them take `extra(i, lds)`.
 template <int TYPE, int SHAPE, bool SPLIT, class Epi, class Extra>
 __global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_two_gemms_kernel(const yp_gemm g1, const Epi e1, int n1, const yp_gemm g2, const Epi e2, int n2,
                                                                                  int second_first, const Extra extra) {
   __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
   const int wg = (int)blockIdx.x;
-  if (wg >= n1 + n2) { extra(wg - n1 - n2); return; }
+  if (wg >= n1 + n2) { extra(wg - n1 - n2, lds); return; }
   const bool first = second_first ? wg >= n2 : wg < n1;
   if (first) yp_gemm_tile<TYPE, SHAPE, true, true, SPLIT>(g1, e1, second_first ? wg - n2 : wg, n1, lds);
   else yp_gemm_tile<TYPE, SHAPE, true, false, SPLIT>(g2, e2, second_first ? wg : wg - n1, n2, lds);
