@@ -297,12 +297,13 @@ enum { YP_F32 = 0, YP_BF16 = 1, YP_F16 = 2, YP_INT8 = 3 };
  *                gradient, counted.
  *   bias         a class whose bias is -inf takes no part: probability 0, no gradient, whatever its weights hold; as a
  *                label its loss is +inf.
- *   losses, lse  [n] float32          reduced [3] float32, may be NULL: the rows' sum, their mean over the rows that are
- *                not ignored (0 without one), and how many those are
+ *   losses, lse  [n] float32; losses may be NULL
+ *   sum, mean, count   one float32 each, may be NULL: the rows' losses added up, their mean over the rows that are not ignored
+ *                (0 without one), and how many those are
  *   workspace    yp_class_loss_workspace(n, v, d, dtype, has_bias, backward) bytes, 256-byte aligned
  * The backward pass takes the forward's inputs and its lse, and grad = dL/dlosses: [n] float32 (grad_stride 1) or one
- * value for every row (grad_stride 0); with count != NULL the values are divided by max(*count, 1) (the mean: pass
- * reduced + 2).  Gradients that are NULL are not computed.  Products accumulate in float32, gradients are rounded once; dz =
+ * value for every row (grad_stride 0); with count != NULL the values are divided by max(*count, 1) (the mean: pass the
+ * forward's count).  Gradients that are NULL are not computed.  Products accumulate in float32, gradients are rounded once; dz =
  * grad (softmax - onehot) is rounded to dtype before its products, relative to the largest |grad|.  Fixed order of sums,
  * no float atomics.
  * 0 <= n <= 2^20, 1 <= v <= 2^24, n v <= 2^38, 1 <= d <= 65536; contiguous tensors, aligned to their elements.  All pointers on the
@@ -310,7 +311,7 @@ enum { YP_F32 = 0, YP_BF16 = 1, YP_F16 = 2, YP_INT8 = 3 };
 int64_t yp_class_loss_workspace(int32_t n, int32_t v, int32_t d, int32_t dtype, int32_t has_bias, int32_t backward);
 int yp_class_loss(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
                   const void* bias, const void* labels, int32_t label_bytes, int64_t ignore_index, void* workspace,
-                  float* losses, float* lse, float* reduced, void* hip_stream);
+                  float* losses, float* lse, float* sum, float* mean, float* count, void* hip_stream);
 int yp_class_loss_backward(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
                            const void* bias, const void* labels, int32_t label_bytes, int64_t ignore_index, const float* lse,
                            const float* grad, int32_t grad_stride, const float* count, void* workspace,

@@ -153,6 +153,7 @@ def test_class_loss_autograd(dt, reduction):
     ref.within(grads[0].reshape(60, 40), *want["grad_h"], "grad_features")
     ref.within(grads[1], *want["grad_w"], "grad_weight")
     ref.within(grads[2], *want["grad_b"], "grad_bias")
+    loss += 1.0                                                # the result is the caller's to change
     again = torch.autograd.grad(loss, (ht, wt, bt), gl)
     assert all(torch.equal(a, c) for a, c in zip(grads, again))                                # same call, same bits
 

@@ -67,7 +67,7 @@ def _refused(rc, needle):
     (dict(n=-1), "n must"), (dict(n=(1 << 20) + 1), "n must"), (dict(v=0), "v must"), (dict(v=(1 << 24) + 1), "v must"),
     (dict(d=0), "d must"), (dict(d=65537), "d must"), (dict(dtype=3), "dtype"), (dict(label_bytes=2), "label_bytes"),
     (dict(features=None), "null"), (dict(weight=None), "null"), (dict(labels=None), "null"), (dict(ws=None), "null"),
-    (dict(losses=None), "null"), (dict(lse=None), "null"), (dict(features=ctypes.c_void_p(4097)), "aligned"),
+    (dict(lse=None), "null"), (dict(losses=ctypes.c_void_p(4097)), "aligned"), (dict(features=ctypes.c_void_p(4097)), "aligned"),
     (dict(bias=ctypes.c_void_p(4097)), "aligned"), (dict(labels=ctypes.c_void_p(4100)), "aligned"),
     (dict(ws=ctypes.c_void_p(4096 + 16)), "256-byte"),
 ])
@@ -75,7 +75,7 @@ def test_class_loss_refuses(change, needle):
     a = dict(n=4, v=9, d=8, dtype=1, features=P, weight=P, bias=None, labels=P, label_bytes=8, ws=P, losses=P, lse=P)
     a.update(change)
     _refused(_lib.load().yp_class_loss(0, a["n"], a["v"], a["d"], a["dtype"], a["features"], a["weight"], a["bias"], a["labels"],
-                                       a["label_bytes"], -1, a["ws"], a["losses"], a["lse"], None, None), needle)
+                                       a["label_bytes"], -1, a["ws"], a["losses"], a["lse"], None, None, None, None), needle)
 
 
 @pytest.mark.parametrize("change,needle", [

@@ -118,7 +118,7 @@ def load():
     L.yp_class_loss_workspace.restype = i64
     L.yp_class_loss_workspace.argtypes = [i32] * 6
     L.yp_class_loss.restype = ctypes.c_int
-    L.yp_class_loss.argtypes = [i32] * 5 + [vp] * 4 + [i32, i64] + [vp] * 4 + [vp]
+    L.yp_class_loss.argtypes = [i32] * 5 + [vp] * 4 + [i32, i64] + [vp] * 6 + [vp]
     L.yp_class_loss_backward.restype = ctypes.c_int
     L.yp_class_loss_backward.argtypes = [i32] * 5 + [vp] * 4 + [i32, i64, vp, vp, i32] + [vp] * 5 + [vp]
     L.yp_quantized_row_bytes.restype = i64

@@ -773,14 +773,13 @@ static int check_class_loss(const char* who, const yp_class_loss_args& a) {
 
 extern "C" int yp_class_loss(int32_t device_id, int32_t n, int32_t v, int32_t d, int32_t dtype, const void* features, const void* weight,
                              const void* bias, const void* labels, int32_t label_bytes, int64_t ignore_index, void* workspace,
-                             float* losses, float* lse, float* reduced, void* hip_stream) {
+                             float* losses, float* lse, float* sum, float* mean, float* count, void* hip_stream) {
   yp_class_loss_args a = {};
   a.n = n; a.v = v; a.d = d; a.type = dtype; a.features = features; a.weight = weight; a.bias = bias; a.labels = labels;
-  a.label_bytes = label_bytes; a.ignore_index = ignore_index; a.workspace = workspace; a.losses = losses; a.lse = lse; a.reduced = reduced;
+  a.label_bytes = label_bytes; a.ignore_index = ignore_index; a.workspace = workspace; a.losses = losses; a.lse = lse; a.sum = sum; a.mean = mean; a.counted = count;
   const int rc = check_class_loss("yp_class_loss", a);
   if (rc != YP_OK) return rc;
-  if (n > 0 && !losses) return fail(YP_EINVAL, "yp_class_loss: null argument");
-  if ((((uintptr_t)losses | (uintptr_t)reduced) & 3) != 0) return fail(YP_EINVAL, "yp_class_loss: a tensor is not aligned to its elements");
+  if ((((uintptr_t)losses | (uintptr_t)sum | (uintptr_t)mean | (uintptr_t)count) & 3) != 0) return fail(YP_EINVAL, "yp_class_loss: a tensor is not aligned to its elements");
   YP_ON_DEVICE(device_id);
   YP_HIP(yp_launch_class_loss(a, (hipStream_t)hip_stream));
   return YP_OK;

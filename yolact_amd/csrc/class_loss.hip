@@ -307,11 +307,15 @@ __device__ __forceinline__ double yp_block_sum(double v, double* lds) {   // fix
   return t;
 }
 
-__device__ __forceinline__ void yp_write_reduced(float* reduced, double sum, double count) {
-  reduced[0] = (float)sum;
-  reduced[1] = count > 0.0 ? (float)(sum / count) : 0.0f;
-  reduced[2] = (float)count;
-}
+struct yp_reduced {
+  float *sum, *mean, *count;     // any may be null
+  __host__ __device__ bool wanted() const { return sum || mean || count; }
+  __device__ __forceinline__ void put(double s, double c) const {
+    if (sum) *sum = (float)s;
+    if (mean) *mean = c > 0.0 ? (float)(s / c) : 0.0f;
+    if (count) *count = (float)c;
+  }
+};
 
 struct yp_join_args {
   const yp_softmax_part* part;
@@ -320,7 +324,7 @@ struct yp_join_args {
   yp_labels labels;
   int N;
   float *losses, *lse;
-  float* reduced;           // [3], may be null
+  yp_reduced reduced;
   double* block_part;       // [blocks][2]
 };
 // Joins the parts of the rows, and the sum of their losses if it is asked for.
@@ -371,22 +375,22 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_join_kernel(const yp_join_ar
         count += 1.0;
       }
       a.lse[n] = l;
-      a.losses[n] = v;
+      if (a.losses) a.losses[n] = v;
     }
   }
-  if (!a.reduced) return;
+  if (!a.reduced.wanted()) return;
   const double ts = yp_block_sum(loss, red), tc = yp_block_sum(count, red);
   if (threadIdx.x == 0) {
-    if (gridDim.x == 1) yp_write_reduced(a.reduced, ts, tc);
+    if (gridDim.x == 1) a.reduced.put(ts, tc);
     else { a.block_part[2 * blockIdx.x] = ts; a.block_part[2 * blockIdx.x + 1] = tc; }
   }
 }
-__global__ __launch_bounds__(YP_CL_THREADS) void yp_reduce_kernel(const double* block_part, int blocks, float* reduced) {
+__global__ __launch_bounds__(YP_CL_THREADS) void yp_reduce_kernel(const double* block_part, int blocks, const yp_reduced reduced) {
   __shared__ double red[YP_CL_THREADS / 64];
   double s = 0.0, c = 0.0;
   for (int i = (int)threadIdx.x; i < blocks; i += YP_CL_THREADS) { s += block_part[2 * i]; c += block_part[2 * i + 1]; }
   const double ts = yp_block_sum(s, red), tc = yp_block_sum(c, red);
-  if (threadIdx.x == 0) yp_write_reduced(reduced, ts, tc);
+  if (threadIdx.x == 0) reduced.put(ts, tc);
 }
 
 // {by / largest |g|, largest |g| / by}
@@ -651,7 +655,7 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   }
   yp_join_args j;
   j.part = part; j.parts = parts; j.picked = (const float*)(ws + p.o_picked); j.labels = labels;
-  j.N = a.n; j.losses = a.losses; j.lse = a.lse; j.reduced = a.reduced; j.block_part = (double*)(ws + p.o_block);
+  j.N = a.n; j.losses = a.losses; j.lse = a.lse; j.reduced = yp_reduced{a.sum, a.mean, a.counted}; j.block_part = (double*)(ws + p.o_block);
   // few rows of many parts: 128 threads a row; else 8.  A few rows of few parts are one workgroup's, which sums their losses
   // itself: a launch less.
   int blocks;
@@ -662,7 +666,7 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
     blocks = a.n <= 256 ? 1 : (a.n + 31) / 32;
     hipLaunchKernelGGL(yp_join_kernel<32>, dim3(blocks), dim3(YP_CL_THREADS), 0, st, j);
   }
-  if (a.reduced && blocks > 1) hipLaunchKernelGGL(yp_reduce_kernel, dim3(1), dim3(YP_CL_THREADS), 0, st, (const double*)j.block_part, blocks, a.reduced);
+  if (j.reduced.wanted() && blocks > 1) hipLaunchKernelGGL(yp_reduce_kernel, dim3(1), dim3(YP_CL_THREADS), 0, st, (const double*)j.block_part, blocks, j.reduced);
   return hipGetLastError();
 }
 
@@ -757,7 +761,10 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
 }
 
 hipError_t yp_launch_class_loss(const yp_class_loss_args& a, hipStream_t st) {
-  if (a.n == 0) return a.reduced ? zero(a.reduced, 3, YP_F32, st) : hipSuccess;
+  if (a.n == 0) {
+    for (float* one : {a.sum, a.mean, a.counted}) if (one) CL_TRY(zero(one, 1, YP_F32, st));
+    return hipSuccess;
+  }
   const bool split = plan_class_loss(a.n, a.v, a.d, a.type, false, false).split;
   return a.type == YP_BF16 ? forward_t<YP_T_BF16, YP_T_BF16, false>(a, st) : a.type == YP_F16 ? forward_t<YP_T_F16, YP_T_F16, false>(a, st)
        : split ? forward_t<YP_T_BF16, YP_T_F32, true>(a, st) : forward_t<YP_T_F32, YP_T_F32, false>(a, st);

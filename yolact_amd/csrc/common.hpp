@@ -295,7 +295,8 @@ struct yp_class_loss_args {
   int label_bytes;                         // 4 or 8
   int64_t ignore_index;
   void* workspace;
-  float *losses, *lse, *reduced;           // forward results (lse is an input of the backward); reduced may be null
+  float *losses, *lse;                     // forward results (lse is an input of the backward); losses may be null
+  float *sum, *mean, *counted;             // likewise, one value each; may be null
   const float* grad;                       // backward: dL/dloss of every row (stride 1) or of all of them (stride 0)
   int grad_stride;
   const float* count;                      // null, or the grads are divided by max(*count, 1)

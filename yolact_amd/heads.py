@@ -62,16 +62,12 @@ def _class_loss_args(features, weight, labels, bias):
     return p_h, p_w, p_b, p_y, labels.numel(), V, D, lead, dev
 
 
-def _class_loss_forward(features, weight, labels, bias, ignore_index, reduce):
-    p_h, p_w, p_b, p_y, N, V, D, lead, dev = _class_loss_args(features, weight, labels, bias)
-    L, dt = _lib.load(), _TYPES[weight.dtype]
-    ws = _workspace(L.yp_class_loss_workspace(N, V, D, dt, bias is not None, 0), dev)
-    losses = torch.empty(lead, dtype=torch.float32, device=dev)
-    lse = torch.empty(lead, dtype=torch.float32, device=dev)
-    reduced = torch.empty((3,), dtype=torch.float32, device=dev) if reduce else None
-    _lib.check(L.yp_class_loss(dev.index, N, V, D, dt, p_h, p_w, p_b, p_y, labels.element_size(), ignore_index, _ptr(ws),
-                               losses.data_ptr(), lse.data_ptr(), _ptr(reduced), _stream(dev)))
-    return losses, lse, reduced
+def _class_loss_forward(args, label_bytes, type_, ignore_index, p_losses, p_lse, p_sum=None, p_mean=None, p_count=None):
+    p_h, p_w, p_b, p_y, N, V, D, _, dev = args
+    L = _lib.load()
+    ws = _workspace(L.yp_class_loss_workspace(N, V, D, type_, p_b is not None, 0), dev)
+    _lib.check(L.yp_class_loss(dev.index, N, V, D, type_, p_h, p_w, p_b, p_y, label_bytes, ignore_index, _ptr(ws),
+                               p_losses, p_lse, p_sum, p_mean, p_count, _stream(dev)))
 
 
 def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
@@ -81,11 +77,15 @@ def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
 
     A row labelled ``ignore_index`` takes no part (loss 0) whatever its features hold; any other label outside [0, V) has
     loss NaN.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf."""
-    losses, lse, _ = _class_loss_forward(features, weight, labels, bias, int(ignore_index), False)
+    args = _class_loss_args(features, weight, labels, bias)
+    lead, dev = args[-2:]
+    losses = torch.empty(lead, dtype=torch.float32, device=dev)
+    lse = torch.empty(lead, dtype=torch.float32, device=dev)
+    _class_loss_forward(args, labels.element_size(), _TYPES[weight.dtype], int(ignore_index), losses.data_ptr(), lse.data_ptr())
     return losses, lse
 
 
-def _class_loss_backward(features, weight, labels, bias, ignore_index, lse, p_grad, per_row, p_count, wanted=(True, True, True)):
+def _class_loss_backward(features, weight, labels, bias, ignore_index, p_lse, p_grad, per_row, p_count, wanted=(True, True, True)):
     """The call itself, on checked tensors; gradients that are not wanted are None."""
     V, D = weight.shape
     N, dev = labels.numel(), weight.device
@@ -95,7 +95,7 @@ def _class_loss_backward(features, weight, labels, bias, ignore_index, lse, p_gr
     gw = torch.empty_like(weight) if wanted[1] else None
     gb = torch.empty_like(bias) if bias is not None and wanted[2] else None
     _lib.check(L.yp_class_loss_backward(dev.index, N, V, D, dt, features.data_ptr(), weight.data_ptr(), _ptr(bias), labels.data_ptr(),
-                                        labels.element_size(), ignore_index, lse.data_ptr(), p_grad, per_row, p_count, _ptr(ws),
+                                        labels.element_size(), ignore_index, p_lse, p_grad, per_row, p_count, _ptr(ws),
                                         _ptr(gh), _ptr(gw), _ptr(gb), _stream(dev)))
     return gh, gw, gb
 
@@ -107,7 +107,7 @@ def class_loss_backward(features, weight, labels, lse, grad_losses, bias=None, i
     lead, dev = _class_loss_args(features, weight, labels, bias)[-2:]
     _check("lse", lse, (torch.float32,), lead, dev)
     p_grad = _check("grad_losses", grad_losses, (torch.float32,), lead, dev)
-    return _class_loss_backward(features, weight, labels, bias, int(ignore_index), lse, p_grad, 1, None)
+    return _class_loss_backward(features, weight, labels, bias, int(ignore_index), lse.data_ptr(), p_grad, 1, None)
 
 
 class ClassLoss(torch.autograd.Function):
@@ -123,19 +123,27 @@ class ClassLoss(torch.autograd.Function):
         features, weight, labels = features.contiguous(), weight.contiguous(), labels.contiguous()
         bias = bias.contiguous() if bias is not None else None
         ignore_index = int(ignore_index)
-        losses, lse, reduced = _class_loss_forward(features, weight, labels, bias, ignore_index, reduction != "none")
-        ctx.save_for_backward(features, weight, bias, labels, lse, reduced)
+        args = _class_loss_args(features, weight, labels, bias)
+        N, lead, dev = args[4], args[-2], args[-1]
+        kept = torch.empty((N + 1,), dtype=torch.float32, device=dev)          # lse of the rows, and how many count
+        p_lse = kept.data_ptr()
+        loss = torch.empty(lead if reduction == "none" else (), dtype=torch.float32, device=dev)
+        p_loss = loss.data_ptr()
+        _class_loss_forward(args, labels.element_size(), _TYPES[weight.dtype], ignore_index, p_loss if reduction == "none" else None, p_lse,
+                            p_loss if reduction == "sum" else None, p_loss if reduction == "mean" else None, p_lse + 4 * N)
+        ctx.save_for_backward(features, weight, bias, labels, kept)
         ctx.cfg = (ignore_index, reduction)
-        return losses if reduction == "none" else reduced.select(0, 0 if reduction == "sum" else 1)
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        features, weight, bias, labels, lse, reduced = ctx.saved_tensors
+        features, weight, bias, labels, kept = ctx.saved_tensors
         ignore_index, reduction = ctx.cfg
         grad = grad.contiguous()             # (float32 and of the result's shape: autograd has seen to it)
-        gh, gw, gb = _class_loss_backward(features, weight, labels, bias, ignore_index, lse, grad.data_ptr(), int(reduction == "none"),
-                                          reduced.data_ptr() + 8 if reduction == "mean" else None, ctx.needs_input_grad)
+        p_lse = kept.data_ptr()
+        gh, gw, gb = _class_loss_backward(features, weight, labels, bias, ignore_index, p_lse, grad.data_ptr(), int(reduction == "none"),
+                                          p_lse + 4 * (kept.shape[0] - 1) if reduction == "mean" else None, ctx.needs_input_grad)
         return gh, gw, gb, None, None, None
 
 
