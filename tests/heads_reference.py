@@ -21,7 +21,9 @@ def class_loss(h, w, b, labels, grad, ignore=-1):
     So lse is off by e + (4 + 64 + V/64) F + 4 F max|z| + F |lse| and a probability, relatively, by e + lse's error +
     (4 + 4 max|z|) F.  dz = g (p - onehot): g is off by 2 F (a division and a factor), the difference by F, and dz is
     rounded to the type (u; f16: or to the step of its subnormals, 2^-38 of the largest g).  A product of K such terms
-    adds K F, its rounding u."""
+    adds K F, its rounding u.
+    (Large float32 products run as three products of f16 planes: 3 K sums and 2^-24 more per product at worst, each a third
+    of them far smaller than the first; the bound of the direct product is kept for them too.)"""
     dt = h.dtype
     u = HALF[dt]
     N, D = h.shape

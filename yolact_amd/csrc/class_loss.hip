@@ -18,14 +18,14 @@
 // is taken out altogether -, which the results get back in f32: with g inside, every row's -g would be rounded the same
 // way, and sums over rows be off by as much as one of them.  f16 with 2^13 more, so that probabilities down to 2^-38 are
 // kept.
-// f32 of any size worth it runs on the bf16 matrix instructions, as three bf16 planes per operand (SPLIT, gemm_tile.hpp).
+// f32 of any size worth it runs on the f16 matrix instructions, as two f16 planes per operand (SPLIT, gemm_tile.hpp).
 // What takes no part has dz = 0, but 0 times NaN is NaN: the gradient products read a copy of h in which ignored rows are
 // zero (and of w, if a bias may mask classes).
 // All sums are f32 in a fixed order: no float atomics, the same call gives the same bits.
 #include "gemm_launch.hpp"
 
 #define YP_CL_THREADS 256
-// f32 products of as many multiplications go through bf16 planes: 200 TFLOP/s against 125; below, the copies cost more
+// f32 products of as many multiplications go through f16 planes; below, the scales and copies cost more
 #define YP_CL_SPLIT_FROM (1ll << 31)
 #define YP_CL_PIECE_MAX (1 << 17)
 #define YP_CL_PIECE_BYTES (128ll << 20)   // of dz: half of the Infinity Cache
@@ -45,9 +45,9 @@ __device__ __forceinline__ void yp_join(float& m, float& s, float m2, float s2) 
   m = t;
 }
 
-// what is left of an f32 beside its bf16 plane: exact (nothing beside an infinity or NaN)
+// what is left of an f32 beside its f16 plane: exact (nothing beside an infinity or NaN)
 __device__ __forceinline__ float yp_plane_rest(float x) {
-  const float h = (float)(__bf16)x;
+  const float h = (float)(_Float16)x;
   return fabsf(h) < INFINITY ? x - h : 0.0f;
 }
 
@@ -65,18 +65,26 @@ struct yp_labels {
 };
 
 // ---- epilogue of the forward product: i = class, j = row ----------------------------------------------------------
-template <int ELEM>
+template <int ELEM, bool SPLIT>
 struct yp_epi_stats {
   const void* bias;            // of the tensors' type ELEM, may be null; of the piece
   yp_labels labels;
   int first;                   // first class of the piece
   yp_softmax_part* part;       // [tiles_i * WI][N] of the piece
   float* picked;               // [N] z of the label
+  yp_scale zscale;             // SPLIT
   template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
   __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], const yp_place& at) const {
     typedef yp_shape<SHAPE> S;
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
+    if constexpr (SPLIT) {
+      const float zs = zscale.get();
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) acc[m][n] = acc[m][n] * zs;
+    }
     if (bias || (at.ti + 1) * S::BM > g.I) {
 #pragma unroll
       for (int m = 0; m < MI; ++m)
@@ -133,9 +141,10 @@ struct yp_epi_dz {
   const float* grad;           // of every row, times *factor (if there is one); null: `up` for all of them
   const float* factor;
   float up;
-  yp_scale scale;              // what the gradients get back
+  yp_scale scale;              // what the bias gradient gets back
+  yp_scale zscale;             // SPLIT
   int first;                   // first class of the piece
-  void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv); SPLIT: three planes of it, bf16
+  void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv); SPLIT: two planes of it, f16
   int64_t plane;               // bytes of one
   int kv, kn;
   void* bias_out;              // of the piece; null without bias
@@ -147,6 +156,13 @@ struct yp_epi_dz {
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
     const float by = grad && factor ? *factor : up;
+    if constexpr (SPLIT) {
+      const float zs = zscale.get();
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) acc[m][n] = acc[m][n] * zs;
+    }
     if (bias || (at.ti + 1) * S::BM > g.I) {      // a class that takes no part, or does not exist: z = -inf
 #pragma unroll
       for (int m = 0; m < MI; ++m)
@@ -211,15 +227,13 @@ struct yp_epi_dz {
     }
     yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, dz, kv, kv, kn, true, [&](int m, int n) { return acc[m][n]; });
     if constexpr (SPLIT) {
+      yp_arrive<0>();
+      yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, (char*)dz + plane, kv, kv, kn, true, [&](int m, int n) {
+        yp_f4 v;
 #pragma unroll
-      for (int q = 1; q < 3; ++q) {
-        yp_arrive<0>();
-        yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, (char*)dz + q * plane, kv, kv, kn, true, [&](int m, int n) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[m][n][r] = yp_plane_rest(acc[m][n][r]);
-          return acc[m][n];
-        });
-      }
+        for (int r = 0; r < 4; ++r) v[r] = yp_plane_rest(acc[m][n][r]);
+        return v;
+      });
     }
   }
 };
@@ -235,7 +249,8 @@ struct yp_copy_job {
   int vec;                // rows of src are multiples of 16 bytes and so is their address
   int by_label;
   const void* bias;
-  int64_t plane;          // 0, or: f32 rows to three bf16 planes, this many bytes apart (row_bytes, kb: of a plane's row)
+  int64_t plane;          // 0, or: f32 rows times *scale to two f16 planes, this many bytes apart (row_bytes, kb: of a plane's row)
+  const float* scale;
 };
 struct yp_copy_args {
   yp_copy_job job[2];
@@ -256,6 +271,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
     if (in && j.by_label) in = a.labels.counted(r) >= 0;
     if (in && j.bias) in = yp_load_as_float(j.bias, r, a.type) != -INFINITY;
     if (j.plane) {        // 8 elements
+      const float sc = *j.scale;
       float x[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) x[u] = 0.0f;
@@ -271,11 +287,13 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
         }
       }
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        yp_bf8 o;
+      for (int u = 0; u < 8; ++u) x[u] *= sc;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) { o[u] = (__bf16)x[u]; x[u] = yp_plane_rest(x[u]); }
-        *reinterpret_cast<yp_bf8*>(j.dst + q * j.plane + r * j.kb + at) = o;
+      for (int q = 0; q < 2; ++q) {
+        yp_h8 o;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { o[u] = (_Float16)x[u]; x[u] = yp_plane_rest(x[u]); }
+        *reinterpret_cast<yp_h8*>(j.dst + q * j.plane + r * j.kb + at) = o;
       }
       continue;
     }
@@ -294,6 +312,56 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
     }
     *reinterpret_cast<yp_i4*>(j.dst + r * j.kb + at) = v;
   }
+}
+
+// The largest magnitudes of features and weight among the rows that take part - a wave a row -, a part per workgroup; and
+// the powers of two that bring them to [2^14, 2^15), scales[0] and [1].
+struct yp_peak_args {
+  const float* src[2];
+  int64_t rows[2];
+  int d, vec;
+  yp_labels labels;            // of the first
+  const float* bias;           // of the second, may be null
+  float* part;                 // [2][YP_PEAK_BLOCKS]
+};
+#define YP_PEAK_BLOCKS 512
+__global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_args a) {
+  __shared__ float red[YP_CL_THREADS / 64];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float top = 0.0f;
+    for (int64_t r = (int64_t)blockIdx.x * (YP_CL_THREADS / 64) + wave; r < a.rows[j]; r += YP_PEAK_BLOCKS * (YP_CL_THREADS / 64)) {
+      if (j == 0 ? a.labels.counted(r) < 0 : a.bias && a.bias[r] == -INFINITY) continue;
+      const float* const p = a.src[j] + r * a.d;
+      if (a.vec) {
+        for (int c = lane; c < a.d / 4; c += 64) {
+          const yp_f4 v = reinterpret_cast<const yp_f4*>(p)[c];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) top = fmaxf(top, fabsf(v[u]));
+        }
+      } else {
+        for (int c = lane; c < a.d; c += 64) top = fmaxf(top, fabsf(p[c]));
+      }
+    }
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    __syncthreads();
+    if (lane == 0) red[wave] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < YP_CL_THREADS / 64; ++w) top = fmaxf(top, red[w]);
+      a.part[j * YP_PEAK_BLOCKS + blockIdx.x] = top;
+    }
+  }
+}
+__global__ __launch_bounds__(128) void yp_scales_kernel(const float* part, float* scales) {   // a wave each
+  const int lane = (int)threadIdx.x & 63, j = (int)threadIdx.x >> 6;
+  float top = 0.0f;
+  for (int i = lane; i < YP_PEAK_BLOCKS; i += 64) top = fmaxf(top, part[j * YP_PEAK_BLOCKS + i]);
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  if (lane == 0) scales[j] = top > 0.0f && top < INFINITY ? ldexpf(1.0f, min(max(14 - ilogbf(top), -100), 100)) : 1.0f;
 }
 
 __device__ __forceinline__ double yp_block_sum(double v, double* lds) {   // fixed order; result in thread 0
@@ -453,14 +521,13 @@ struct yp_bias_sum {
   }
 };
 
-// Up to two arrays, each out[e] = scale * sum over its parts.  64 elements and 4 waves a workgroup: wave w adds parts
+// Up to two arrays, each out[e] = its scale * sum over its parts.  64 elements and 4 waves a workgroup: wave w adds parts
 // w, w + 4, ... in their order, then the four sums are added in theirs.
-struct yp_sum_job { const float* part; int parts; int64_t stride, total; void* out; };
-struct yp_sum_args { yp_sum_job job[2]; int jobs, out_type; yp_scale scale; };
+struct yp_sum_job { const float* part; int parts; int64_t stride, total; void* out; yp_scale scale; };
+struct yp_sum_args { yp_sum_job job[2]; int jobs, out_type; };
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_sum_args a) {
   __shared__ float red[YP_CL_THREADS / 64][64];
   const int x = (int)threadIdx.x & 63, y = (int)threadIdx.x >> 6;
-  const float sc = a.scale.get();
   auto put = [&](void* out, int64_t e, float s) {
     if (a.out_type == YP_F32) reinterpret_cast<float*>(out)[e] = s;
     else if (a.out_type == YP_BF16) reinterpret_cast<__bf16*>(out)[e] = (__bf16)s;
@@ -468,6 +535,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_su
   };
   for (int j = 0; j < a.jobs; ++j) {
     const yp_sum_job& b = a.job[j];
+    const float sc = b.scale.get();
     if (b.parts < 4) {   // (or none: zeros) a thread an element
       for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < b.total; e += (int64_t)gridDim.x * YP_CL_THREADS) {
         float s = 0.0f;
@@ -513,20 +581,19 @@ static hipError_t sum_parts(const yp_sum_args& a, hipStream_t st) {
   hipLaunchKernelGGL(yp_sum_parts_kernel, dim3(blocks_for(most, 1, 8192)), dim3(YP_CL_THREADS), 0, st, a);
   return hipGetLastError();
 }
-static void add_sum(yp_sum_args& a, const float* part, int parts, int64_t stride, int64_t total, void* out) {
-  a.job[a.jobs++] = yp_sum_job{part, parts, stride, total, out};
+static void add_sum(yp_sum_args& a, const float* part, int parts, int64_t stride, int64_t total, void* out, const yp_scale& scale) {
+  a.job[a.jobs++] = yp_sum_job{part, parts, stride, total, out, scale};
 }
 static hipError_t zero(void* out, int64_t n, int type, hipStream_t st) {   // (a kernel, not a memset: the call may be captured)
   yp_sum_args a = {};
   a.out_type = type;
-  a.scale.by = 1.0f;
-  add_sum(a, nullptr, 0, 0, n, out);
+  add_sum(a, nullptr, 0, 0, n, out, yp_scale{nullptr, nullptr, 1.0f, {}});
   return sum_parts(a, st);
 }
 
 // The launch plan of a call, from its sizes alone: the same for yp_class_loss_workspace and for the call.
 struct ClassLossPlan {
-  bool split;                  // f32 in three bf16 planes
+  bool split;                  // f32 in two f16 planes
   int b, planes;               // bytes of an element and how many planes the products read
   int64_t kd;                  // bytes of a padded feature row
   int fwd_pieces, fwd_piece;   // forward: pieces of the vocabulary if w is copied, else one
@@ -536,6 +603,7 @@ struct ClassLossPlan {
   int64_t kn, kv;              // rows of dz padded to a step, elements; bytes of a row
   yp_tile_plan dzp, dwp, dhp;
   // workspace offsets
+  int64_t o_scales, o_peaks;   // both passes
   int64_t o_h, o_w, o_part, o_picked, o_block, fwd_total;
   int64_t o_factor, o_hc, o_wc, o_dz, o_bp, o_dwpart, o_dhpart, bwd_total;
 };
@@ -553,13 +621,16 @@ static void cut_pieces(int64_t V, int64_t most, int* pieces, int* piece) {   // 
 static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, bool has_bias, bool copy_fwd) {
   ClassLossPlan p;
   p.split = type == YP_F32 && N * V >= YP_CL_SPLIT_FROM / D;
-  const int b = p.split ? 2 : type_bytes(type), planes = p.split ? 3 : 1;
+  const int b = p.split ? 2 : type_bytes(type), planes = p.split ? 2 : 1;
   p.b = b;
   p.planes = planes;
   copy_fwd = copy_fwd || p.split;
   p.kd = yp_pad_k(D, b);
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = up256(off + bytes); return o; };
+  p.o_scales = take(p.split ? 8 : 0);
+  p.o_peaks = take(p.split ? 2 * YP_PEAK_BLOCKS * 4 : 0);
+  const int64_t both = off;
   if (copy_fwd) cut_pieces(V, YP_CL_PIECE_BYTES / (p.kd * planes), &p.fwd_pieces, &p.fwd_piece);
   else { p.fwd_pieces = 1; p.fwd_piece = (int)V; }
   const int segs = p.split ? YP_SEGMENTS : 1;
@@ -573,14 +644,14 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   p.o_block = take((N <= 1024 ? (N + 1) / 2 : (N + 31) / 32) * 16);
   p.fwd_total = off;
 
-  off = 0;
+  off = both;
   const int kr = YP_TILE_KB / b;
   p.kn = (N + kr - 1) / kr * kr;
   int64_t most = YP_CL_PIECE_BYTES / (p.kn * b * planes);
   if (most > YP_CL_PIECE_BYTES / (p.kd * planes)) most = YP_CL_PIECE_BYTES / (p.kd * planes);
   cut_pieces(V, most, &p.pieces, &p.piece);
   p.kv = yp_pad_k(p.piece, b);
-  // (three planes of dz to write: M's epilogues hide better - 215 us against L's 253, 2048 x 8192 x 1024)
+  // (two planes of dz to write: M's epilogues hide better)
   p.dzp = p.split ? yp_plan_shape(YP_TILE_M, p.piece, p.kn) : yp_plan_tiles(p.piece, p.kn, dsteps);
   // the two gradient products share a launch and so a tile shape
   yp_plan_two(D, p.piece, p.kn / kr * segs, D, N, p.kv / YP_TILE_KB * segs, &p.dwp, &p.dhp);
@@ -612,6 +683,17 @@ static yp_copy_job copy_job(const void* src, char* dst, int64_t d, const ClassLo
   j.vec = row_bytes % 16 == 0 && ((uintptr_t)src & 15) == 0;
   return j;
 }
+// scales[0], [1]: of the features and of the weight
+static hipError_t find_scales(const yp_class_loss_args& a, const yp_labels& labels, char* ws, const ClassLossPlan& p, hipStream_t st) {
+  yp_peak_args k;
+  k.src[0] = (const float*)a.features; k.src[1] = (const float*)a.weight;
+  k.rows[0] = a.n; k.rows[1] = a.v; k.d = a.d;
+  k.vec = a.d % 4 == 0 && (((uintptr_t)a.features | (uintptr_t)a.weight) & 15) == 0;
+  k.labels = labels; k.bias = (const float*)a.bias; k.part = (float*)(ws + p.o_peaks);
+  hipLaunchKernelGGL(yp_peak_kernel, dim3(YP_PEAK_BLOCKS), dim3(YP_CL_THREADS), 0, st, k);
+  hipLaunchKernelGGL(yp_scales_kernel, dim3(1), dim3(128), 0, st, (const float*)k.part, (float*)(ws + p.o_scales));
+  return hipGetLastError();
+}
 static hipError_t copy_rows(yp_copy_args a, hipStream_t st) {
   a.chunks0 = a.job[0].rows_out * (a.job[0].kb / 16);
   a.chunks = a.chunks0 + (a.job[1].src ? a.job[1].rows_out * (a.job[1].kb / 16) : 0);
@@ -628,6 +710,8 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   const ClassLossPlan p = plan_class_loss(a.n, a.v, a.d, ELEM, a.bias != nullptr, copy);
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
+  float* const scales = SPLIT ? (float*)(ws + p.o_scales) : nullptr;
+  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, st));
   yp_softmax_part* const part = (yp_softmax_part*)(ws + p.o_part);
   int parts = 0;
   for (int s = 0; s < p.fwd_pieces; ++s) {
@@ -639,6 +723,11 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
       c.type = ELEM;
       c.job[0] = copy_job(g.a + v0 * row, ws + p.o_w, a.d, p, nv, nv);
       if (s == 0) c.job[1] = copy_job(g.b, ws + p.o_h, a.d, p, a.n, a.n);
+      c.labels = labels;
+      if (SPLIT) {       // (a row that takes no part may hold anything, beyond f16 too)
+        c.job[0].scale = scales + 1; c.job[0].bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
+        c.job[1].scale = scales; c.job[1].by_label = 1;
+      }
       g.aplane = nv * p.kd; g.bplane = a.n * p.kd;
       CL_TRY(copy_rows(c, st));
       g.a = ws + p.o_w; g.b = ws + p.o_h;
@@ -647,7 +736,8 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
     g.I = nv; g.J = a.n; g.steps = (int)(p.kd / YP_TILE_KB);
     yp_tile_plan tp = p.fwd;
     tp.tiles_i = (nv + tp.bi - 1) / tp.bi;
-    yp_epi_stats<ELEM> e;
+    yp_epi_stats<ELEM, SPLIT> e;
+    e.zscale = yp_scale{nullptr, nullptr, 1.0f, {scales, SPLIT ? scales + 1 : nullptr}};
     e.bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
     e.labels = labels; e.first = v0; e.part = part + (int64_t)parts * a.n; e.picked = (float*)(ws + p.o_picked);
     CL_TRY(yp_launch_gemm<TYPE, SPLIT>(tp, g, e, st));
@@ -678,12 +768,14 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   const bool copy_w = SPLIT || a.bias || row % YP_TILE_KB != 0 || ((uintptr_t)a.weight & 15) != 0;
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
-  const float up = ELEM == YP_T_F16 ? 8192.0f : 1.0f;
+  float* const scales = SPLIT ? (float*)(ws + p.o_scales) : nullptr;
+  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, st));
+  const float up = TYPE == YP_T_F16 ? 8192.0f : 1.0f;
   float* factor = nullptr;
-  yp_scale back = {a.grad, a.count, 1.0f / up};             // one g for all rows
+  yp_scale back = {a.grad, a.count, 1.0f / up, {}};         // one g for all rows
   if (a.grad_stride) {
-    back = yp_scale{nullptr, a.count, 1.0f};
-    if (ELEM != YP_T_F32) {                                 // (f32: dz is not rounded)
+    back = yp_scale{nullptr, a.count, 1.0f, {}};
+    if (TYPE != YP_T_F32) {                                 // (f32 as it is: dz is not rounded)
       factor = (float*)(ws + p.o_factor);
       hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, (int64_t)a.n, up, factor);
       CL_TRY(hipGetLastError());
@@ -693,9 +785,10 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   float* const dhpart = (float*)(ws + p.o_dhpart);
   float* const biaspart = a.grad_bias && p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
   const bool dh_joined = p.dhp.splits > 1 || p.pieces > 1;
+  yp_scale back_w = back, back_h = back;                    // of grad_weight, which has the features' scale, and the other way round
+  if (SPLIT) { back_w.over[0] = scales; back_h.over[0] = scales + 1; }
   yp_sum_args sums = {};
   sums.out_type = ELEM;
-  sums.scale = back;
   for (int s = 0; s < p.pieces; ++s) {
     const int v0 = s * p.piece, nv = a.v - v0 < p.piece ? a.v - v0 : p.piece;
     const char* const bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
@@ -705,8 +798,8 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
       c.type = ELEM;
       c.labels = labels;
       int n = 0;
-      if (s == 0) { c.job[n] = copy_job(a.features, ws + p.o_hc, a.d, p, a.n, p.kn); c.job[n++].by_label = 1; }
-      if (copy_w) { c.job[n] = copy_job(w, ws + p.o_wc, a.d, p, nv, nv); c.job[n++].bias = bias; w = ws + p.o_wc; }
+      if (s == 0) { c.job[n] = copy_job(a.features, ws + p.o_hc, a.d, p, a.n, p.kn); c.job[n].scale = scales; c.job[n++].by_label = 1; }
+      if (copy_w) { c.job[n] = copy_job(w, ws + p.o_wc, a.d, p, nv, nv); c.job[n].scale = scales ? scales + 1 : nullptr; c.job[n++].bias = bias; w = ws + p.o_wc; }
       CL_TRY(copy_rows(c, st));
     }
     const int kv = (int)(yp_pad_k(nv, tb) / tb);
@@ -718,6 +811,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     g.I = nv; g.J = a.n; g.steps = (int)(p.kd / YP_TILE_KB);
     yp_epi_dz<ELEM, SPLIT> e;
     e.plane = dzplane;
+    e.zscale = yp_scale{nullptr, nullptr, 1.0f, {scales, SPLIT ? scales + 1 : nullptr}};
     e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = up; e.scale = back;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
     e.bias_out = a.grad_bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
@@ -732,7 +826,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     gw.K = (int)p.kn; gw.steps = (int)(p.kn * tb / YP_TILE_KB);
     char* const gwo = a.grad_weight ? (char*)a.grad_weight + v0 * row : nullptr;
     yp_epi_store<ELEM> ew = {};
-    ew.out = gwo; ew.ld = a.d; ew.scale = back;
+    ew.out = gwo; ew.ld = a.d; ew.scale = back_w;
     ew.vec = row % 16 == 0 && ((uintptr_t)a.grad_weight & 15) == 0;
     ew.part_vec = a.d % 4 == 0;
     ew.part = gwo && p.dwp.splits > 1 ? (float*)(ws + p.o_dwpart) : nullptr;
@@ -744,7 +838,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     gh.b = ws + p.o_dz; gh.ldb = (int64_t)kv * tb; gh.J = a.n;
     gh.K = nv; gh.steps = (int)((int64_t)kv * tb / YP_TILE_KB);
     yp_epi_store<ELEM> eh = {};
-    eh.out = a.grad_features; eh.ld = a.d; eh.scale = back;
+    eh.out = a.grad_features; eh.ld = a.d; eh.scale = back_h;
     eh.vec = row % 16 == 0 && ((uintptr_t)a.grad_features & 15) == 0;
     eh.part_vec = a.d % 4 == 0;
     eh.part = dh_joined ? dhpart : nullptr;
@@ -752,8 +846,8 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     yp_bias_sum bs = {};
     bs.part = biaspart; bs.parts = p.dzp.tiles_j; bs.total = nv; bs.type = ELEM; bs.scale = back; bs.out = e.bias_out;
     CL_TRY(yp_launch_two<TYPE, SPLIT>(twp, gw, ew, p.dhp, gh, eh, bs, biaspart ? (nv + yp_bias_sum::CLASSES - 1) / yp_bias_sum::CLASSES : 0, st));
-    if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, (int64_t)nv * a.d, gwo);
-    if (s == p.pieces - 1 && dh_joined && a.grad_features) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features);
+    if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, (int64_t)nv * a.d, gwo, back_w);
+    if (s == p.pieces - 1 && dh_joined && a.grad_features) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features, back_h);
     CL_TRY(sum_parts(sums, st));
     sums.jobs = 0;
   }
@@ -767,7 +861,7 @@ hipError_t yp_launch_class_loss(const yp_class_loss_args& a, hipStream_t st) {
   }
   const bool split = plan_class_loss(a.n, a.v, a.d, a.type, false, false).split;
   return a.type == YP_BF16 ? forward_t<YP_T_BF16, YP_T_BF16, false>(a, st) : a.type == YP_F16 ? forward_t<YP_T_F16, YP_T_F16, false>(a, st)
-       : split ? forward_t<YP_T_BF16, YP_T_F32, true>(a, st) : forward_t<YP_T_F32, YP_T_F32, false>(a, st);
+       : split ? forward_t<YP_T_F16, YP_T_F32, true>(a, st) : forward_t<YP_T_F32, YP_T_F32, false>(a, st);
 }
 hipError_t yp_launch_class_loss_backward(const yp_class_loss_args& a, hipStream_t st) {
   if (a.n == 0) {
@@ -776,5 +870,5 @@ hipError_t yp_launch_class_loss_backward(const yp_class_loss_args& a, hipStream_
   }
   const bool split = plan_class_loss(a.n, a.v, a.d, a.type, false, false).split;
   return a.type == YP_BF16 ? backward_t<YP_T_BF16, YP_T_BF16, false>(a, st) : a.type == YP_F16 ? backward_t<YP_T_F16, YP_T_F16, false>(a, st)
-       : split ? backward_t<YP_T_BF16, YP_T_F32, true>(a, st) : backward_t<YP_T_F32, YP_T_F32, false>(a, st);
+       : split ? backward_t<YP_T_F16, YP_T_F32, true>(a, st) : backward_t<YP_T_F32, YP_T_F32, false>(a, st);
 }

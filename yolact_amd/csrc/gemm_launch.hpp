@@ -102,12 +102,18 @@ __device__ __forceinline__ float yp_load_as_float(const void* p, int64_t i, int 
   return type == YP_F32 ? reinterpret_cast<const float*>(p)[i]
        : type == YP_BF16 ? (float)reinterpret_cast<const __bf16*>(p)[i] : (float)reinterpret_cast<const _Float16*>(p)[i];
 }
-// A factor that lies on the device: by * (a ? *a : 1) / (count ? max(*count, 1) : 1).
+// A factor that lies on the device: by * (a ? *a : 1) / (count ? max(*count, 1) : 1) / (over[i] ? *over[i] : 1).
 struct yp_scale {
   const float* a;
   const float* count;
   float by;
-  __device__ __forceinline__ float get() const { return (a ? *a : 1.0f) * by / (count ? fmaxf(*count, 1.0f) : 1.0f); }
+  const float* over[2];
+  __device__ __forceinline__ float get() const {
+    float v = (a ? *a : 1.0f) * by / (count ? fmaxf(*count, 1.0f) : 1.0f);
+    if (over[0]) v /= *over[0];
+    if (over[1]) v /= *over[1];
+    return v;
+  }
 };
 // (what is exactly zero stays so, whatever the factor)
 __device__ __forceinline__ float yp_times(float v, float scale) { return v == 0.0f ? 0.0f : v * scale; }

@@ -53,12 +53,13 @@ struct yp_gemm {
   int64_t aplane, bplane;   // SPLIT: bytes between the planes
 };
 
-// SPLIT: f32 operands as the sum of three bf16 planes each (24 bits: exact), and of the nine products of planes the six
-// whose terms are not below 2^-24 of the result - the same product over a k axis six times as long.  The bf16 matrix
-// instructions are 16 times as fast as the f32 ones: 6 of them for one.  Sums are f32 as ever.  Segment by segment:
-#define YP_SEGMENTS 6
-#define YP_SEGMENT_A(s) ((0x201100 >> (4 * (s))) & 3)
-#define YP_SEGMENT_B(s) ((0x021010 >> (4 * (s))) & 3)
+// SPLIT: f32 operands, scaled by a power of two, as the sum of two f16 planes each (22 bits, to 2^-40 of the largest
+// element), and of the four products of planes the three whose terms are not below 2^-24 of the result - the same product
+// over a k axis three times as long.  The f16 matrix instructions are 16 times as fast as the f32 ones: three of them for
+// one.  Sums are f32 as ever.  Plane of either operand, segment by segment:
+#define YP_SEGMENTS 3
+#define YP_SEGMENT_A(s) ((s) == 2)
+#define YP_SEGMENT_B(s) ((s) == 1)
 
 #ifdef __HIPCC__
 template <int V> struct yp_const { static constexpr int value = V; };
@@ -96,6 +97,11 @@ __device__ __forceinline__ void yp_settle(Acc (&acc)[MI][NJ]) {
 #pragma unroll
     for (int n = 0; n < NJ; ++n) asm volatile("" : "+a"(acc[m][n]));
   __builtin_amdgcn_sched_barrier(0);
+}
+
+// (the compiler does not always see that a value is the same in all lanes)
+__device__ __forceinline__ int64_t yp_uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 
 // 64 lanes x 16 bytes from base + off (per lane) to LDS at `lds` (uniform) + lane * 16.  Written as assembly because the
@@ -282,8 +288,12 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   int lk = 0, ls = 0, todo = 0;
   int64_t from_a = 0, from_b = 0;
   auto place = [&]() {
-    from_a = lk * sa.stride + (SPLIT ? YP_SEGMENT_A(ls) * g.aplane : 0);
-    from_b = lk * sb.stride + (SPLIT ? YP_SEGMENT_B(ls) * g.bplane : 0);
+    from_a = lk * sa.stride;
+    from_b = lk * sb.stride;
+    if (SPLIT) {
+      from_a = yp_uniform(from_a + (YP_SEGMENT_A(ls) ? g.aplane : 0));
+      from_b = yp_uniform(from_b + (YP_SEGMENT_B(ls) ? g.bplane : 0));
+    }
   };
   // past the last step the last one is loaded again: the number of loads in flight, which the waits count, is always the
   // same
