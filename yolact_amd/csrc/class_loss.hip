@@ -633,9 +633,9 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   const int64_t both = off;
   if (copy_fwd) cut_pieces(V, YP_CL_PIECE_BYTES / (p.kd * planes), &p.fwd_pieces, &p.fwd_piece);
   else { p.fwd_pieces = 1; p.fwd_piece = (int)V; }
-  const int segs = p.split ? YP_SEGMENTS : 1;
+  const int segs = p.split ? YP_SEGMENTS : 1, largest = type == YP_F32 && !p.split ? YP_TILE_M : YP_TILE_L;
   const int64_t dsteps = p.kd / YP_TILE_KB * segs;
-  p.fwd = yp_plan_tiles(p.fwd_piece, N, dsteps);
+  p.fwd = yp_plan_tiles(p.fwd_piece, N, dsteps, largest);
   p.parts = p.fwd.tiles_i * 2;
   p.o_h = take(copy_fwd ? N * p.kd * planes : 0);
   p.o_w = take(copy_fwd ? p.fwd_piece * p.kd * planes : 0);
@@ -652,9 +652,9 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   cut_pieces(V, most, &p.pieces, &p.piece);
   p.kv = yp_pad_k(p.piece, b);
   // (two planes of dz to write: M's epilogues hide better)
-  p.dzp = p.split ? yp_plan_shape(YP_TILE_M, p.piece, p.kn) : yp_plan_tiles(p.piece, p.kn, dsteps);
+  p.dzp = p.split ? yp_plan_shape(YP_TILE_M, p.piece, p.kn) : yp_plan_tiles(p.piece, p.kn, dsteps, largest);
   // the two gradient products share a launch and so a tile shape
-  yp_plan_two(D, p.piece, p.kn / kr * segs, D, N, p.kv / YP_TILE_KB * segs, &p.dwp, &p.dhp);
+  yp_plan_two(D, p.piece, p.kn / kr * segs, D, N, p.kv / YP_TILE_KB * segs, largest, &p.dwp, &p.dhp);
   p.o_factor = take(8);
   p.o_hc = take(p.kn * p.kd * planes);
   p.o_wc = take(p.piece * p.kd * planes);

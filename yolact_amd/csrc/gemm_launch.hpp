@@ -32,10 +32,11 @@ static inline double yp_plan_cost(int shape, double wgs, double steps) {
   if (shape == YP_TILE_M) return wgs <= 256 ? steps * 0.49 + 5 : wgs <= 512 ? steps * 0.79 + 6 : steps * 0.93 * ceil(wgs / 256) / 2 + 6 * ceil(wgs / 512);
   return wgs <= 256 ? steps * 0.28 + 3 : wgs <= 512 ? steps * 0.45 + 3 : wgs <= 1280 ? steps * 0.75 + 4 : steps * 0.92 * wgs / 1280 + 4 * ceil(wgs / 1280);
 }
-static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps) {
+// `largest`: YP_TILE_M for f32 as it is, else YP_TILE_L
+static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps, int largest) {
   yp_tile_plan best = {};
   double least = 1e30;
-  for (int s = YP_TILE_L; s <= YP_TILE_T; ++s) {
+  for (int s = largest; s <= YP_TILE_T; ++s) {
     const yp_tile_plan p = yp_plan_shape(s, I, J);
     const double c = yp_plan_cost(s, (double)p.tiles_i * p.tiles_j, (double)steps);
     if (c < least) { least = c; best = p; }
@@ -44,9 +45,9 @@ static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps) {
 }
 // Two products that share a launch, and so a shape, each with its k axis dealt to as many workgroups as pays: their
 // f32 sums are written and read once more (5 TB/s), by another launch.  A workgroup keeps 8 steps at least.
-static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I2, int64_t J2, int64_t steps2, yp_tile_plan* p1, yp_tile_plan* p2) {
+static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I2, int64_t J2, int64_t steps2, int largest, yp_tile_plan* p1, yp_tile_plan* p2) {
   double least = 1e30;
-  for (int shape = YP_TILE_L; shape <= YP_TILE_T; ++shape) {
+  for (int shape = largest; shape <= YP_TILE_T; ++shape) {
     yp_tile_plan a = yp_plan_shape(shape, I1, J1), b = yp_plan_shape(shape, I2, J2);
     const double ta = (double)a.tiles_i * a.tiles_j, tb = (double)b.tiles_i * b.tiles_j;
     const double alone = shape == YP_TILE_L ? 1.57 : shape == YP_TILE_M ? 0.79 : 0.45;
@@ -76,9 +77,11 @@ static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const
   const yp_gemm g = yp_with_plan(g0, p);
   if (yp_plan_workgroups(p) >= YP_MAX_WORKGROUPS) return hipErrorInvalidValue;
   const dim3 grid((unsigned)yp_plan_workgroups(p));
-  if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
-  else if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
-  else hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_T, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
+  if constexpr (TYPE != YP_T_F32) {
+    if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
+  }
+  if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
+  if (p.shape == YP_TILE_T) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_T, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
   return hipGetLastError();
 }
 
@@ -92,9 +95,11 @@ static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const
   if (n1 + n2 + extras == 0) return hipSuccess;
   const int second_first = b.steps / b.splits > a.steps / a.splits;   // the longer ones first: the short ones fill up the end
   const dim3 grid((unsigned)(n1 + n2 + extras));
-  if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
-  else if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
-  else hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+  if constexpr (TYPE != YP_T_F32) {
+    if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+  }
+  if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+  if (p1.shape == YP_TILE_T) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
   return hipGetLastError();
 }
 

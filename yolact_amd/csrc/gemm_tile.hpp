@@ -80,12 +80,11 @@ __device__ __forceinline__ typename yp_type<TYPE>::acc yp_mma(const typename yp_
 // The same in place, for the tile whose accumulators fill all 256 accumulation registers: given the builtin, the register
 // allocator has no room to turn and moves every accumulator once per step (873 against 1 3xx TFLOP/s).  The compiler
 // does not know that this is a matrix instruction: yp_settle stands between these and any other use of the result.
-template <int TYPE, int U>
+template <int TYPE>
 __device__ __forceinline__ void yp_mma_inplace(const typename yp_type<TYPE>::frag& a, const typename yp_type<TYPE>::frag& b, typename yp_type<TYPE>::acc& c) {
   if constexpr (TYPE == YP_T_BF16) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   else if constexpr (TYPE == YP_T_F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  else if constexpr (TYPE == YP_T_I8) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  else asm volatile("v_mfma_f32_16x16x4_f32 %0, %1, %2, %0" : "+a"(c) : "v"(a[U]), "v"(b[U]));
+  else asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 // Nothing passes this: the accumulators are written by vector instructions before it and by matrix instructions after it,
 // or the other way round, and the longest of either (16 passes) has finished.
@@ -256,6 +255,7 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   constexpr int MI = BM / WI / 16, NJ = BN / WJ / 16, MH = MI / 2, NH = NJ / 2;
   constexpr int BUF = (BM + BN) * YP_TILE_KB;
   constexpr bool INPLACE = MI * NJ * 4 == 256;
+  static_assert(!(INPLACE && TYPE == YP_T_F32), "f32 as it is runs on the smaller tiles: it keeps two sums");
   yp_place at;
   at.lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -278,6 +278,15 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
 #pragma unroll
     for (int n = 0; n < NJ; ++n) acc[m][n] = accv{0, 0, 0, 0};
   if constexpr (INPLACE) yp_settle<MI, NJ>(acc);
+  // the f32 matrix instruction rounds after every k: sums of 256 are added up apart, or thousands of roundings in a row show
+  constexpr bool CHUNKS = TYPE == YP_T_F32;
+  accv total[MI][NJ];
+  if constexpr (CHUNKS) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) total[m][n] = accv{0, 0, 0, 0};
+  }
 
   frag a[2][MH][2], b[2][NH][2];          // [half][fragment][half step]
   auto read_a = [&](int buf, int x, int q) { a[x][q >> 1][q & 1] = sa.read(lds + buf * BUF, x, q >> 1, q & 1); };
@@ -327,15 +336,7 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
       }
       if constexpr (INPLACE) {
 #pragma unroll
-        for (int n = 0; n < NH; ++n) yp_mma_inplace<TYPE, 0>(a[x][m][q], b[y][n][q], acc[x * MH + m][y * NH + n]);
-        if constexpr (TYPE == YP_T_F32) {      // (the same accumulator again after NH others)
-#pragma unroll
-          for (int n = 0; n < NH; ++n) yp_mma_inplace<TYPE, 1>(a[x][m][q], b[y][n][q], acc[x * MH + m][y * NH + n]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) yp_mma_inplace<TYPE, 2>(a[x][m][q], b[y][n][q], acc[x * MH + m][y * NH + n]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) yp_mma_inplace<TYPE, 3>(a[x][m][q], b[y][n][q], acc[x * MH + m][y * NH + n]);
-        }
+        for (int n = 0; n < NH; ++n) yp_mma_inplace<TYPE>(a[x][m][q], b[y][n][q], acc[x * MH + m][y * NH + n]);
       } else {
 #pragma unroll
         for (int n = 0; n < NH; ++n) acc[x * MH + m][y * NH + n] = yp_mma<TYPE>(a[x][m][q], b[y][n][q], acc[x * MH + m][y * NH + n]);
@@ -369,6 +370,12 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
     yp_arrive<2 * GROUP>();
     int buf = 0;
     for (int k = k0; k < k1 - 1; ++k, buf ^= 1) {
+      if (CHUNKS && k > k0 && ((k - k0) & 7) == 0) {
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+          for (int n = 0; n < NJ; ++n) { total[m][n] = total[m][n] + acc[m][n]; acc[m][n] = accv{0, 0, 0, 0}; }
+      }
       phase(E0{}, E0{}, E2{}, E1{}, buf, E1{}, E0{}, buf);
       phase(E0{}, E1{}, E1{}, E1{}, buf, E2{}, E0{}, buf);
       yp_arrive<2 * GROUP>();
@@ -383,6 +390,12 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
     phase(E1{}, E1{}, E0{}, E0{}, 0, E0{}, E0{}, 0);
   }
   if constexpr (INPLACE) yp_settle<MI, NJ>(acc);
+  if constexpr (CHUNKS) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) acc[m][n] = total[m][n] + acc[m][n];
+  }
   yp_arrive<0>();    // the surplus loads of every wave have landed: the LDS is the epilogue's
   epi.template apply<TYPE, SHAPE, MI, NJ>(g, acc, at);
 }

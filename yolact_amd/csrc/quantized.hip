@@ -454,7 +454,7 @@ static hipError_t linear_t(const yp_gemm& g, const float* x_scale, const float* 
   yp_epi_scaled<OUT> e;
   e.x_scale = x_scale; e.w_scale = w_scale; e.bias = bias; e.out = out;
   e.vec = (int64_t)g.I * yp_type<OUT>::bytes % 16 == 0 && ((uintptr_t)out & 15) == 0;
-  return yp_launch_gemm<YP_T_I8>(yp_plan_tiles(g.I, g.J, g.steps), g, e, st);
+  return yp_launch_gemm<YP_T_I8>(yp_plan_tiles(g.I, g.J, g.steps, YP_TILE_L), g, e, st);
 }
 
 hipError_t yp_launch_quantized_linear(int rows, int v, int k, int x_type, const void* x, const float* x_scale, const void* wq, const float* w_scale,
