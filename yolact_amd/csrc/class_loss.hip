@@ -17,8 +17,8 @@
 // half a step of that type, like the gradients themselves.  It is held relative to the largest |g| - one g for all rows
 // is taken out altogether -, which the results get back in f32: with g inside, every row's -g would be rounded the same
 // way, and sums over rows be off by as much as one of them.  f16 with 2^13 more, so that probabilities down to 2^-38 are
-// kept.
-// f32 of any size worth it runs on the f16 matrix instructions, as two f16 planes per operand (SPLIT, gemm_tile.hpp).
+// kept.  Where rows are few, their roundings do not average out, and dz has two planes (twice the precision).
+// f32 of any size worth it runs on the f16 matrix instructions, as two f16 planes per operand (SPLIT; gemm_tile.hpp).
 // What takes no part has dz = 0, but 0 times NaN is NaN: the gradient products read a copy of h in which ignored rows are
 // zero (and of w, if a bias may mask classes).
 // All sums are f32 in a fixed order: no float atomics, the same call gives the same bits.
@@ -27,6 +27,10 @@
 #define YP_CL_THREADS 256
 // f32 products of as many multiplications go through f16 planes; below, the scales and copies cost more
 #define YP_CL_SPLIT_FROM (1ll << 31)
+// up to as many rows, or as many multiplications, dz has two planes: 12 instead of 8 N V D operations where reading w,
+// writing dw or the launches are what takes time
+#define YP_CL_FINE_ROWS 512
+#define YP_CL_FINE_WORK (1ll << 30)
 #define YP_CL_PIECE_MAX (1 << 17)
 #define YP_CL_PIECE_BYTES (128ll << 20)   // of dz: half of the Infinity Cache
 
@@ -45,9 +49,10 @@ __device__ __forceinline__ void yp_join(float& m, float& s, float m2, float s2) 
   m = t;
 }
 
-// what is left of an f32 beside its f16 plane: exact (nothing beside an infinity or NaN)
+// what is left of an f32 beside its first plane: exact (nothing beside an infinity or NaN)
+template <class E>
 __device__ __forceinline__ float yp_plane_rest(float x) {
-  const float h = (float)(_Float16)x;
+  const float h = (float)(E)x;
   return fabsf(h) < INFINITY ? x - h : 0.0f;
 }
 
@@ -133,7 +138,7 @@ struct yp_epi_stats {
 };
 
 // ---- epilogue of the backward product -----------------------------------------------------------------------------
-template <int ELEM, bool SPLIT>
+template <int ELEM, bool SPLIT, int PLANES>
 struct yp_epi_dz {
   const void* bias;            // of the tensors' type ELEM; of the piece
   const float* lse;
@@ -144,7 +149,7 @@ struct yp_epi_dz {
   yp_scale scale;              // what the bias gradient gets back
   yp_scale zscale;             // SPLIT
   int first;                   // first class of the piece
-  void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv); SPLIT: two planes of it, f16
+  void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv); or PLANES of it
   int64_t plane;               // bytes of one
   int kv, kn;
   void* bias_out;              // of the piece; null without bias
@@ -226,12 +231,12 @@ struct yp_epi_dz {
       yp_arrive<0>();
     }
     yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, dz, kv, kv, kn, true, [&](int m, int n) { return acc[m][n]; });
-    if constexpr (SPLIT) {
+    if constexpr (PLANES == 2) {
       yp_arrive<0>();
       yp_put_tile<TYPE, SHAPE, false, MI, NJ>(at, (char*)dz + plane, kv, kv, kn, true, [&](int m, int n) {
         yp_f4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = yp_plane_rest(acc[m][n][r]);
+        for (int r = 0; r < 4; ++r) v[r] = yp_plane_rest<typename yp_type<TYPE>::elem>(acc[m][n][r]);
         return v;
       });
     }
@@ -292,7 +297,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
       for (int q = 0; q < 2; ++q) {
         yp_h8 o;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) { o[u] = (_Float16)x[u]; x[u] = yp_plane_rest(x[u]); }
+        for (int u = 0; u < 8; ++u) { o[u] = (_Float16)x[u]; x[u] = yp_plane_rest<_Float16>(x[u]); }
         *reinterpret_cast<yp_h8*>(j.dst + q * j.plane + r * j.kb + at) = o;
       }
       continue;
@@ -594,7 +599,8 @@ static hipError_t zero(void* out, int64_t n, int type, hipStream_t st) {   // (a
 // The launch plan of a call, from its sizes alone: the same for yp_class_loss_workspace and for the call.
 struct ClassLossPlan {
   bool split;                  // f32 in two f16 planes
-  int b, planes;               // bytes of an element and how many planes the products read
+  int b, planes;               // bytes of an element of what the products read, and its planes
+  int dzplanes, segs;          // planes of dz, segments of the gradient products
   int64_t kd;                  // bytes of a padded feature row
   int fwd_pieces, fwd_piece;   // forward: pieces of the vocabulary if w is copied, else one
   yp_tile_plan fwd;            // of a whole piece
@@ -624,6 +630,8 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   const int b = p.split ? 2 : type_bytes(type), planes = p.split ? 2 : 1;
   p.b = b;
   p.planes = planes;
+  p.dzplanes = p.split || (type != YP_F32 && (N <= YP_CL_FINE_ROWS || N * V <= YP_CL_FINE_WORK / D)) ? 2 : 1;
+  p.segs = p.split ? 3 : p.dzplanes;
   copy_fwd = copy_fwd || p.split;
   p.kd = yp_pad_k(D, b);
   int64_t off = 0;
@@ -633,8 +641,8 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   const int64_t both = off;
   if (copy_fwd) cut_pieces(V, YP_CL_PIECE_BYTES / (p.kd * planes), &p.fwd_pieces, &p.fwd_piece);
   else { p.fwd_pieces = 1; p.fwd_piece = (int)V; }
-  const int segs = p.split ? YP_SEGMENTS : 1, largest = type == YP_F32 && !p.split ? YP_TILE_M : YP_TILE_L;
-  const int64_t dsteps = p.kd / YP_TILE_KB * segs;
+  const int largest = type == YP_F32 && !p.split ? YP_TILE_M : YP_TILE_L;
+  const int64_t dsteps = p.kd / YP_TILE_KB * (p.split ? 3 : 1);
   p.fwd = yp_plan_tiles(p.fwd_piece, N, dsteps, largest);
   p.parts = p.fwd.tiles_i * 2;
   p.o_h = take(copy_fwd ? N * p.kd * planes : 0);
@@ -647,18 +655,18 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   off = both;
   const int kr = YP_TILE_KB / b;
   p.kn = (N + kr - 1) / kr * kr;
-  int64_t most = YP_CL_PIECE_BYTES / (p.kn * b * planes);
+  int64_t most = YP_CL_PIECE_BYTES / (p.kn * b * p.dzplanes);
   if (most > YP_CL_PIECE_BYTES / (p.kd * planes)) most = YP_CL_PIECE_BYTES / (p.kd * planes);
   cut_pieces(V, most, &p.pieces, &p.piece);
   p.kv = yp_pad_k(p.piece, b);
   // (two planes of dz to write: M's epilogues hide better)
   p.dzp = p.split ? yp_plan_shape(YP_TILE_M, p.piece, p.kn) : yp_plan_tiles(p.piece, p.kn, dsteps, largest);
   // the two gradient products share a launch and so a tile shape
-  yp_plan_two(D, p.piece, p.kn / kr * segs, D, N, p.kv / YP_TILE_KB * segs, largest, &p.dwp, &p.dhp);
+  yp_plan_two(D, p.piece, p.kn / kr * p.segs, D, N, p.kv / YP_TILE_KB * p.segs, largest, &p.dwp, &p.dhp);
   p.o_factor = take(8);
   p.o_hc = take(p.kn * p.kd * planes);
   p.o_wc = take(p.piece * p.kd * planes);
-  p.o_dz = take(p.kn * p.kv * planes);
+  p.o_dz = take(p.kn * p.kv * p.dzplanes);
   p.o_bp = take(has_bias && p.dzp.tiles_j > 1 ? (int64_t)p.dzp.tiles_j * p.piece * 4 : 0);
   p.o_dwpart = take(p.dwp.splits > 1 ? (int64_t)p.dwp.splits * p.piece * D * 4 : 0);
   p.o_dhpart = take(p.dhp.splits > 1 || p.pieces > 1 ? (int64_t)p.dhp.splits * N * D * 4 : 0);
@@ -740,7 +748,7 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
     e.zscale = yp_scale{nullptr, nullptr, 1.0f, {scales, SPLIT ? scales + 1 : nullptr}};
     e.bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
     e.labels = labels; e.first = v0; e.part = part + (int64_t)parts * a.n; e.picked = (float*)(ws + p.o_picked);
-    CL_TRY(yp_launch_gemm<TYPE, SPLIT>(tp, g, e, st));
+    CL_TRY(yp_launch_gemm<TYPE, SPLIT ? 3 : 1>(tp, g, e, st));
     parts += tp.tiles_i * 2;
   }
   yp_join_args j;
@@ -760,7 +768,7 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int TYPE, int ELEM, bool SPLIT>
+template <int TYPE, int ELEM, bool SPLIT, int PLANES>
 static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   constexpr int b = yp_type<ELEM>::bytes, tb = yp_type<TYPE>::bytes;
   const int64_t row = (int64_t)a.d * b;
@@ -809,7 +817,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     g.a = w; g.b = ws + p.o_hc; g.lda = g.ldb = p.kd;
     g.aplane = wplane; g.bplane = hplane;
     g.I = nv; g.J = a.n; g.steps = (int)(p.kd / YP_TILE_KB);
-    yp_epi_dz<ELEM, SPLIT> e;
+    yp_epi_dz<ELEM, SPLIT, PLANES> e;
     e.plane = dzplane;
     e.zscale = yp_scale{nullptr, nullptr, 1.0f, {scales, SPLIT ? scales + 1 : nullptr}};
     e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = up; e.scale = back;
@@ -818,7 +826,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     e.bias_part = biaspart;
     yp_tile_plan tp = p.dzp;
     tp.tiles_i = (nv + tp.bi - 1) / tp.bi;
-    CL_TRY(yp_launch_gemm<TYPE, SPLIT>(tp, g, e, st));
+    CL_TRY(yp_launch_gemm<TYPE, SPLIT ? 3 : 1>(tp, g, e, st));
     // dw[v][d] = sum_n dz[n][v] h[n][d]
     yp_gemm gw = {};
     gw.a = ws + p.o_hc; gw.lda = p.kd; gw.I = a.d; gw.aplane = hplane; gw.bplane = dzplane;
@@ -845,7 +853,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     eh.add = s > 0;
     yp_bias_sum bs = {};
     bs.part = biaspart; bs.parts = p.dzp.tiles_j; bs.total = nv; bs.type = ELEM; bs.scale = back; bs.out = e.bias_out;
-    CL_TRY(yp_launch_two<TYPE, SPLIT>(twp, gw, ew, p.dhp, gh, eh, bs, biaspart ? (nv + yp_bias_sum::CLASSES - 1) / yp_bias_sum::CLASSES : 0, st));
+    CL_TRY(yp_launch_two<TYPE, SPLIT ? 3 : PLANES>(twp, gw, ew, p.dhp, gh, eh, bs, biaspart ? (nv + yp_bias_sum::CLASSES - 1) / yp_bias_sum::CLASSES : 0, st));
     if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, (int64_t)nv * a.d, gwo, back_w);
     if (s == p.pieces - 1 && dh_joined && a.grad_features) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features, back_h);
     CL_TRY(sum_parts(sums, st));
@@ -868,7 +876,8 @@ hipError_t yp_launch_class_loss_backward(const yp_class_loss_args& a, hipStream_
     if (a.grad_weight) CL_TRY(zero(a.grad_weight, (int64_t)a.v * a.d, a.type, st));
     return a.grad_bias ? zero(a.grad_bias, a.v, a.type, st) : hipSuccess;
   }
-  const bool split = plan_class_loss(a.n, a.v, a.d, a.type, false, false).split;
-  return a.type == YP_BF16 ? backward_t<YP_T_BF16, YP_T_BF16, false>(a, st) : a.type == YP_F16 ? backward_t<YP_T_F16, YP_T_F16, false>(a, st)
-       : split ? backward_t<YP_T_F16, YP_T_F32, true>(a, st) : backward_t<YP_T_F32, YP_T_F32, false>(a, st);
+  const ClassLossPlan p = plan_class_loss(a.n, a.v, a.d, a.type, false, false);
+  if (a.type == YP_F32) return p.split ? backward_t<YP_T_F16, YP_T_F32, true, 2>(a, st) : backward_t<YP_T_F32, YP_T_F32, false, 1>(a, st);
+  if (a.type == YP_BF16) return p.dzplanes == 2 ? backward_t<YP_T_BF16, YP_T_BF16, false, 2>(a, st) : backward_t<YP_T_BF16, YP_T_BF16, false, 1>(a, st);
+  return p.dzplanes == 2 ? backward_t<YP_T_F16, YP_T_F16, false, 2>(a, st) : backward_t<YP_T_F16, YP_T_F16, false, 1>(a, st);
 }

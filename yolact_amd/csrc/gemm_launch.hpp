@@ -72,21 +72,21 @@ static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I
 static inline yp_gemm yp_with_plan(yp_gemm g, const yp_tile_plan& p) { g.tiles_i = p.tiles_i; g.tiles_j = p.tiles_j; g.splits = p.splits; return g; }
 static inline int64_t yp_plan_workgroups(const yp_tile_plan& p) { return (int64_t)p.tiles_i * p.tiles_j * p.splits; }
 
-template <int TYPE, bool SPLIT = false, class Epi>
+template <int TYPE, int SEGS = 1, class Epi>
 static hipError_t yp_launch_gemm(const yp_tile_plan& p, const yp_gemm& g0, const Epi& epi, hipStream_t st) {
   const yp_gemm g = yp_with_plan(g0, p);
   if (yp_plan_workgroups(p) >= YP_MAX_WORKGROUPS) return hipErrorInvalidValue;
   const dim3 grid((unsigned)yp_plan_workgroups(p));
   if constexpr (TYPE != YP_T_F32) {
-    if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
+    if (p.shape == YP_TILE_L) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_L, SEGS, Epi>), grid, dim3(256), 0, st, g, epi);
   }
-  if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
-  if (p.shape == YP_TILE_T) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_T, SPLIT, Epi>), grid, dim3(256), 0, st, g, epi);
+  if (p.shape == YP_TILE_M) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_M, SEGS, Epi>), grid, dim3(256), 0, st, g, epi);
+  if (p.shape == YP_TILE_T) hipLaunchKernelGGL((yp_gemm_kernel<TYPE, YP_TILE_T, SEGS, Epi>), grid, dim3(256), 0, st, g, epi);
   return hipGetLastError();
 }
 
 // (either of the two may be left out: no output)
-template <int TYPE, bool SPLIT, class Epi, class Extra>
+template <int TYPE, int SEGS, class Epi, class Extra>
 static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const Epi& e1, const yp_tile_plan& p2, const yp_gemm& g2, const Epi& e2,
                                 const Extra& extra, int extras, hipStream_t st) {
   const yp_gemm a = yp_with_plan(g1, p1), b = yp_with_plan(g2, p2);
@@ -96,10 +96,10 @@ static hipError_t yp_launch_two(const yp_tile_plan& p1, const yp_gemm& g1, const
   const int second_first = b.steps / b.splits > a.steps / a.splits;   // the longer ones first: the short ones fill up the end
   const dim3 grid((unsigned)(n1 + n2 + extras));
   if constexpr (TYPE != YP_T_F32) {
-    if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+    if (p1.shape == YP_TILE_L) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_L, SEGS, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
   }
-  if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
-  if (p1.shape == YP_TILE_T) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, SPLIT, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+  if (p1.shape == YP_TILE_M) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_M, SEGS, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
+  if (p1.shape == YP_TILE_T) hipLaunchKernelGGL((yp_two_gemms_kernel<TYPE, YP_TILE_T, SEGS, Epi, Extra>), grid, dim3(256), 0, st, a, e1, n1, b, e2, n2, second_first, extra);
   return hipGetLastError();
 }
 

@@ -50,14 +50,15 @@ struct yp_gemm {
   int steps;          // steps of 128 bytes of k
   int splits;         // the steps are dealt to this many workgroups per tile (epilogues that take a split only)
   int tiles_i, tiles_j;
-  int64_t aplane, bplane;   // SPLIT: bytes between the planes
+  int64_t aplane, bplane;   // bytes between the planes
 };
 
-// SPLIT: f32 operands, scaled by a power of two, as the sum of two f16 planes each (22 bits, to 2^-40 of the largest
-// element), and of the four products of planes the three whose terms are not below 2^-24 of the result - the same product
-// over a k axis three times as long.  The f16 matrix instructions are 16 times as fast as the f32 ones: three of them for
-// one.  Sums are f32 as ever.  Plane of either operand, segment by segment:
-#define YP_SEGMENTS 3
+// SEGS > 1: operands as the sum of two planes of their type, and the products of planes one after the other along a k
+// axis SEGS times as long:
+//   2  B has two planes: twice its precision
+//   3  f32 operands, scaled by a power of two, as two f16 planes each (22 bits, to 2^-40 of the largest element); of the
+//      four products of planes the three whose terms are not below 2^-24 of the result.  The f16 matrix instructions are
+//      16 times as fast as the f32 ones: three of them for one.  Sums are f32 as ever.
 #define YP_SEGMENT_A(s) ((s) == 2)
 #define YP_SEGMENT_B(s) ((s) == 1)
 
@@ -246,7 +247,7 @@ struct yp_place {
 // step s + 2 go into the buffer of step s in two groups, A0 B0 in p0 and p1 of s, B1 A1 in p2 and p3, each group a step
 // and a half before it is read.  (With the whole buffer loaded at once, half a step to a step before: 1057 TFLOP/s.  With
 // more stages of 64 bytes of k, every cache line fetched twice: 985.  This: 1257.  bf16, 16384 x 8192 x 4096.)
-template <int TYPE, int SHAPE, bool A_BY_K, bool B_BY_K, bool SPLIT, class Epi>
+template <int TYPE, int SHAPE, bool A_BY_K, bool B_BY_K, int SEGS, class Epi>
 __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, int wg, int nwg, char* lds) {
   typedef typename yp_type<TYPE>::frag frag;
   typedef typename yp_type<TYPE>::acc accv;
@@ -262,7 +263,7 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   yp_tile_of(g, wg, nwg, at.ti, at.tj, at.split);
   at.wi = wave % WI; at.wj = wave / WI;
   at.lds = lds;
-  const int steps = SPLIT ? g.steps * YP_SEGMENTS : g.steps;
+  const int steps = g.steps * SEGS;
   const int k0 = (int)((int64_t)steps * at.split / g.splits), k1 = (int)((int64_t)steps * (at.split + 1) / g.splits);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   typedef yp_side<TYPE, BM, WAVES, WI, A_BY_K> SA;
@@ -299,7 +300,7 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   auto place = [&]() {
     from_a = lk * sa.stride;
     from_b = lk * sb.stride;
-    if (SPLIT) {
+    if (SEGS > 1) {
       from_a = yp_uniform(from_a + (YP_SEGMENT_A(ls) ? g.aplane : 0));
       from_b = yp_uniform(from_b + (YP_SEGMENT_B(ls) ? g.bplane : 0));
     }
@@ -309,7 +310,7 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   auto advance = [&]() {
     if (todo > 0) {
       --todo;
-      if (SPLIT && lk + 1 == g.steps) { lk = 0; ++ls; } else ++lk;
+      if (SEGS > 1 && lk + 1 == g.steps) { lk = 0; ++ls; } else ++lk;
       place();
     }
   };
@@ -345,8 +346,8 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
     }
   };
   if (k0 < k1) {
-    ls = SPLIT ? k0 / g.steps : 0;
-    lk = SPLIT ? k0 - ls * g.steps : k0;
+    ls = SEGS > 1 ? k0 / g.steps : 0;
+    lk = k0 - ls * g.steps;
     todo = k1 - 1 - k0;
     place();
     constexpr int GROUP = SA::P + SB::P;
@@ -400,23 +401,23 @@ __device__ __forceinline__ void yp_gemm_tile(const yp_gemm& g, const Epi& epi, i
   epi.template apply<TYPE, SHAPE, MI, NJ>(g, acc, at);
 }
 
-template <int TYPE, int SHAPE, bool SPLIT, class Epi>
+template <int TYPE, int SHAPE, int SEGS, class Epi>
 __global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_gemm_kernel(const yp_gemm g, const Epi epi) {
   __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
-  yp_gemm_tile<TYPE, SHAPE, false, false, SPLIT>(g, epi, (int)blockIdx.x, (int)gridDim.x, lds);
+  yp_gemm_tile<TYPE, SHAPE, false, false, SEGS>(g, epi, (int)blockIdx.x, (int)gridDim.x, lds);
 }
 
 // The two gradient products, of one tile shape, in one launch: the first reads both operands by k, the second A by k and B by
 // rows; n1 and n2 workgroups, with `second_first` the second one's first.  Workgroups past them take `extra(i, lds)`.
-template <int TYPE, int SHAPE, bool SPLIT, class Epi, class Extra>
+template <int TYPE, int SHAPE, int SEGS, class Epi, class Extra>
 __global__ __launch_bounds__(256, yp_shape<SHAPE>::WPS) void yp_two_gemms_kernel(const yp_gemm g1, const Epi e1, int n1, const yp_gemm g2, const Epi e2, int n2,
                                                                                  int second_first, const Extra extra) {
   __shared__ __align__(1024) char lds[yp_lds_bytes<SHAPE>];
   const int wg = (int)blockIdx.x;
   if (wg >= n1 + n2) { extra(wg - n1 - n2, lds); return; }
   const bool first = second_first ? wg >= n2 : wg < n1;
-  if (first) yp_gemm_tile<TYPE, SHAPE, true, true, SPLIT>(g1, e1, second_first ? wg - n2 : wg, n1, lds);
-  else yp_gemm_tile<TYPE, SHAPE, true, false, SPLIT>(g2, e2, second_first ? wg : wg - n1, n2, lds);
+  if (first) yp_gemm_tile<TYPE, SHAPE, true, true, SEGS>(g1, e1, second_first ? wg - n2 : wg, n1, lds);
+  else yp_gemm_tile<TYPE, SHAPE, true, false, SEGS>(g2, e2, second_first ? wg : wg - n1, n2, lds);
 }
 
 // Where an epilogue's fragment (0, 0), element 0 lies: i and j of this lane.
