@@ -122,7 +122,7 @@ __global__ __launch_bounds__(YP_QR_THREADS) void yp_quantize_rows_kernel(const v
       if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = top;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < LANES / 64; ++w) top = max(top, red[turn][w]);
+      for (int w = 0; w < LANES / 64; ++w) top = max(top, red[turn][(int)threadIdx.x / LANES * (LANES / 64) + w]);
     }
     if (!live) continue;
     const yp_row_scale s = yp_make_scale(top);
@@ -149,7 +149,8 @@ template <int TYPE>
 static hipError_t quantize_t(int64_t rows, int k, const void* x, void* q, float* scale, hipStream_t st) {
   const int64_t chunks = yp_qrow_bytes(k) * yp_type<TYPE>::bytes / 16;
   return chunks <= 16 * YP_QR_KEEP ? quantize_l<TYPE, 16>(rows, k, x, q, scale, st)
-       : chunks <= 64 * YP_QR_KEEP ? quantize_l<TYPE, 64>(rows, k, x, q, scale, st) : quantize_l<TYPE, 256>(rows, k, x, q, scale, st);
+       : chunks <= 64 * YP_QR_KEEP ? quantize_l<TYPE, 64>(rows, k, x, q, scale, st)
+       : chunks <= 128 * YP_QR_KEEP ? quantize_l<TYPE, 128>(rows, k, x, q, scale, st) : quantize_l<TYPE, 256>(rows, k, x, q, scale, st);
 }
 
 hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x, void* q, float* scale, hipStream_t st) {
