@@ -79,7 +79,7 @@ __device__ __forceinline__ typename yp_type<TYPE>::acc yp_mma(const typename yp_
 }
 
 // The same in place, for the tile whose accumulators fill all 256 accumulation registers: given the builtin, the register
-// allocator has no room to turn and moves every accumulator once per step (873 against 1 3xx TFLOP/s).  The compiler
+// allocator has no room to turn and moves every accumulator once per step (883 TFLOP/s against 1057, bf16, 16384 x 8192 x 4096).  The compiler
 // does not know that this is a matrix instruction: yp_settle stands between these and any other use of the result.
 template <int TYPE>
 __device__ __forceinline__ void yp_mma_inplace(const typename yp_type<TYPE>::frag& a, const typename yp_type<TYPE>::frag& b, typename yp_type<TYPE>::acc& c) {

@@ -158,134 +158,101 @@ hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x,
        : type == YP_BF16 ? quantize_t<YP_T_BF16>(rows, k, x, q, scale, st) : quantize_t<YP_T_F16>(rows, k, x, q, scale, st);
 }
 
-// ---- few rows: the weight is read once and that is all there is -----------------------------------------------------
-// A workgroup holds the (at most YP_FR_ROWS) rows of x in LDS, quantized by itself - 8 KB of x per row from L2 cost less
-// than another launch - and its waves walk over rows of the weight, YP_FR_W at a time: a lane reads 16 bytes of k of each,
-// multiplies with 4-wide dot products and the wave adds up.  YP_FR_C chunks of each are on their way at a time - 16 KB a
-// wave -, the first ones while x is quantized.
-#define YP_FR_ROWS 8
-#define YP_FR_W 4
-#define YP_FR_C 4
-#define YP_FR_LDS 61440
+// ---- one row: the weight is read once and that is all there is -----------------------------------------------------
+// A workgroup holds the row in LDS, quantized by itself - 8 KB from L2 cost less than another launch - and its waves walk
+// over rows of the weight, YP_OR_W at a time: a lane reads 16 bytes of k of each, multiplies with 4-wide dot products and
+// the wave adds up.  YP_OR_C chunks of each are on their way at a time - 16 KB a wave -, the first ones while x is
+// quantized.  26.6 us for 32000 x 4096 (131 MB: 4.9 TB/s); from two rows on the matrix cores are faster (30 us, where this
+// took 43 for two and 100 for eight).
+#define YP_OR_W 4
+#define YP_OR_C 4
+#define YP_OR_LDS 61440
 
-template <int XTYPE, int OUT, int ROWS>
-__global__ __launch_bounds__(YP_QR_THREADS) void yp_few_rows_kernel(const void* x, const float* x_scale, int rows, int v, int k, int kp, const char* wq,
-                                                                    const float* w_scale, const float* bias, void* out, int vec) {
+template <int XTYPE, int OUT>
+__global__ __launch_bounds__(YP_QR_THREADS) void yp_one_row_kernel(const void* x, const float* x_scale, int v, int k, int kp, const char* wq, const float* w_scale,
+                                                                   const float* bias, void* out, int vec) {
   typedef typename yp_type<OUT>::elem oelem;
-  extern __shared__ __align__(16) char xl[];      // [rows][kp]
-  __shared__ float sx[ROWS];
-  __shared__ uint32_t red[ROWS][YP_QR_THREADS / 64];
+  extern __shared__ __align__(16) char xl[];      // [kp]
+  __shared__ uint32_t red[YP_QR_THREADS / 64];
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = (int)blockIdx.x * (YP_QR_THREADS / 64) + (tid >> 6), waves = (int)gridDim.x * (YP_QR_THREADS / 64);
   const int chunks = kp / 16;
-  yp_i4 w[YP_FR_C][YP_FR_W];
+  yp_i4 w[YP_OR_C][YP_OR_W];
   auto get_w = [&](int j0, int c0) {              // (zeros past the row)
 #pragma unroll
-    for (int c = 0; c < YP_FR_C; ++c)
+    for (int c = 0; c < YP_OR_C; ++c)
 #pragma unroll
-      for (int u = 0; u < YP_FR_W; ++u)
+      for (int u = 0; u < YP_OR_W; ++u)
         w[c][u] = c0 + c * 64 < chunks ? *reinterpret_cast<const yp_i4*>(wq + (int64_t)min(j0 + u, v - 1) * kp + (c0 + c * 64) * 16) : yp_i4{0, 0, 0, 0};
   };
-  int j0 = wave * YP_FR_W;
-  if (j0 < v) get_w(j0, lane);
+  int64_t j0 = (int64_t)wave * YP_OR_W;
+  if (j0 < v) get_w((int)j0, lane);
+  float sx;
   if constexpr (XTYPE == YP_T_I8) {
-    for (int c = tid; c < rows * chunks; c += YP_QR_THREADS) reinterpret_cast<yp_i4*>(xl)[c] = reinterpret_cast<const yp_i4*>(x)[c];
-    if (tid < rows) sx[tid] = x_scale[tid];
+    for (int c = tid; c < chunks; c += YP_QR_THREADS) reinterpret_cast<yp_i4*>(xl)[c] = reinterpret_cast<const yp_i4*>(x)[c];
+    sx = x_scale[0];
   } else {
     typedef yp_row_reader<XTYPE> R;
     const int ec = kp / R::E;
+    const R rr = {reinterpret_cast<const typename R::elem*>(x), k, vec};
+    uint32_t top = 0;
+    for (int c = tid; c < ec; c += YP_QR_THREADS) top = R::top(rr.get(c), top);
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      const R rr = {reinterpret_cast<const typename R::elem*>(x) + (int64_t)min(r, rows - 1) * k, k, vec};
-      uint32_t top = 0;
-      for (int c = tid; c < ec; c += YP_QR_THREADS) top = R::top(rr.get(c), top);
-#pragma unroll
-      for (int s = 32; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
-      if (lane == 0) red[r][tid >> 6] = top;
-    }
+    for (int s = 32; s > 0; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+    if (lane == 0) red[tid >> 6] = top;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (r < rows) {
-        const R rr = {reinterpret_cast<const typename R::elem*>(x) + (int64_t)r * k, k, vec};
-        uint32_t top = 0;
-#pragma unroll
-        for (int u = 0; u < YP_QR_THREADS / 64; ++u) top = max(top, red[r][u]);
-        const yp_row_scale s = yp_make_scale(top);
-        if (tid == 0) sx[r] = s.scale;
-        for (int c = tid; c < ec; c += YP_QR_THREADS) R::put(xl + r * kp, c, rr.get(c), s);
-      }
-    }
+    for (int u = 0; u < YP_QR_THREADS / 64; ++u) top = max(top, red[u]);
+    const yp_row_scale s = yp_make_scale(top);
+    sx = s.scale;
+    for (int c = tid; c < ec; c += YP_QR_THREADS) R::put(xl, c, rr.get(c), s);
   }
   __syncthreads();
-  for (; j0 < v; j0 += waves * YP_FR_W) {
-    int acc[YP_FR_W][ROWS];
+  for (; j0 < v; j0 += (int64_t)waves * YP_OR_W) {
+    int acc[YP_OR_W] = {0, 0, 0, 0};
+    for (int c0 = lane; c0 - lane < chunks; c0 += YP_OR_C * 64) {
+      if (c0 != lane) get_w((int)j0, c0);
 #pragma unroll
-    for (int u = 0; u < YP_FR_W; ++u)
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) acc[u][r] = 0;
-    for (int c0 = lane; c0 - lane < chunks; c0 += YP_FR_C * 64) {
-      if (c0 != lane) get_w(j0, c0);
-#pragma unroll
-      for (int c = 0; c < YP_FR_C; ++c) {
+      for (int c = 0; c < YP_OR_C; ++c) {
         if (c0 + c * 64 < chunks) {
+          const yp_i4 xv = *reinterpret_cast<const yp_i4*>(xl + (c0 + c * 64) * 16);
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            if (r < rows) {
-              const yp_i4 xv = *reinterpret_cast<const yp_i4*>(xl + r * kp + (c0 + c * 64) * 16);
+          for (int u = 0; u < YP_OR_W; ++u)
 #pragma unroll
-              for (int u = 0; u < YP_FR_W; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[u][r] = __builtin_amdgcn_sdot4(w[c][u][e], xv[e], acc[u][r], false);
-            }
-          }
+            for (int e = 0; e < 4; ++e) acc[u] = __builtin_amdgcn_sdot4(w[c][u][e], xv[e], acc[u], false);
         }
       }
     }
-    const int here = j0;
-    if (here + waves * YP_FR_W < v) get_w(here + waves * YP_FR_W, lane);
+    if (j0 + (int64_t)waves * YP_OR_W < v) get_w((int)j0 + waves * YP_OR_W, lane);
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (r < rows) {
+    for (int u = 0; u < YP_OR_W; ++u) {
+      int t = acc[u];
 #pragma unroll
-        for (int u = 0; u < YP_FR_W; ++u) {
-          int t = acc[u][r];
-#pragma unroll
-          for (int s = 32; s > 0; s >>= 1) t += __shfl_xor(t, s);
-          const int j = here + u;
-          if (lane == u && j < v)
-            reinterpret_cast<oelem*>(out)[(int64_t)r * v + j] = (oelem)__builtin_fmaf((float)t * sx[r], w_scale[j], bias ? bias[j] : 0.0f);
-        }
-      }
+      for (int s = 32; s > 0; s >>= 1) t += __shfl_xor(t, s);
+      const int64_t j = j0 + u;
+      if (lane == u && j < v) reinterpret_cast<oelem*>(out)[j] = (oelem)__builtin_fmaf((float)t * sx, w_scale[j], bias ? bias[j] : 0.0f);
     }
   }
 }
 
 template <int XTYPE, int OUT>
-static hipError_t few_rows_t(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out,
-                             hipStream_t st) {
+static hipError_t one_row_t(int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, hipStream_t st) {
   const int kp = (int)yp_qrow_bytes(k);
-  const int per = YP_FR_W * (YP_QR_THREADS / 64);                 // rows of the weight per workgroup and turn
+  const int per = YP_OR_W * (YP_QR_THREADS / 64);                 // rows of the weight per workgroup and turn
   const int64_t turns = ((int64_t)v + per - 1) / per;
-  int64_t resident = 163840 / (rows * kp + 256);                  // workgroups a CU's LDS holds; more would only quantize x again
+  int64_t resident = 163840 / (kp + 256);                         // workgroups a CU's LDS holds; more would only quantize x again
   if (resident > 4) resident = 4;                                 // (and its registers: 4)
   const unsigned blocks = (unsigned)(turns < 256 * resident ? turns : 256 * resident);
   int vec = 0;
   if constexpr (XTYPE != YP_T_I8) vec = row_vec<XTYPE>(k, x);
-#define YP_FR_LAUNCH(R) hipLaunchKernelGGL((yp_few_rows_kernel<XTYPE, OUT, R>), dim3(blocks), dim3(YP_QR_THREADS), (size_t)rows * kp, st, x, x_scale, rows, v, k, kp, \
-                                           (const char*)wq, w_scale, bias, out, vec)
-  if (rows == 1) YP_FR_LAUNCH(1);
-  else if (rows <= 4) YP_FR_LAUNCH(4);
-  else YP_FR_LAUNCH(YP_FR_ROWS);
-#undef YP_FR_LAUNCH
+  hipLaunchKernelGGL((yp_one_row_kernel<XTYPE, OUT>), dim3(blocks), dim3(YP_QR_THREADS), (size_t)kp, st, x, x_scale, v, k, kp, (const char*)wq, w_scale, bias, out, vec);
   return hipGetLastError();
 }
 template <int XTYPE>
-static hipError_t few_rows_x(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out,
-                             int out_type, hipStream_t st) {
-  return out_type == YP_F32 ? few_rows_t<XTYPE, YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
-       : out_type == YP_BF16 ? few_rows_t<XTYPE, YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
-                             : few_rows_t<XTYPE, YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st);
+static hipError_t one_row_x(int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, int out_type, hipStream_t st) {
+  return out_type == YP_F32 ? one_row_t<XTYPE, YP_T_F32>(v, k, x, x_scale, wq, w_scale, bias, out, st)
+       : out_type == YP_BF16 ? one_row_t<XTYPE, YP_T_BF16>(v, k, x, x_scale, wq, w_scale, bias, out, st)
+                             : one_row_t<XTYPE, YP_T_F16>(v, k, x, x_scale, wq, w_scale, bias, out, st);
 }
 
 // ---- many rows, a small weight: the head over all anchors ------------------------------------------------------------
@@ -461,11 +428,11 @@ static hipError_t linear_t(const yp_gemm& g, const float* x_scale, const float* 
 hipError_t yp_launch_quantized_linear(int rows, int v, int k, int x_type, const void* x, const float* x_scale, const void* wq, const float* w_scale,
                                       const float* bias, void* workspace, void* out, int out_type, hipStream_t st) {
   const int64_t kp = yp_qrow_bytes(k);
-  if (rows <= YP_FR_ROWS && rows * kp <= YP_FR_LDS)
-    return x_type == YP_INT8 ? few_rows_x<YP_T_I8>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
-         : x_type == YP_F32 ? few_rows_x<YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
-         : x_type == YP_BF16 ? few_rows_x<YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
-                             : few_rows_x<YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
+  if (rows == 1 && kp <= YP_OR_LDS)
+    return x_type == YP_INT8 ? one_row_x<YP_T_I8>(v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_F32 ? one_row_x<YP_T_F32>(v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_BF16 ? one_row_x<YP_T_BF16>(v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+                             : one_row_x<YP_T_F16>(v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
   if (tall_fits(rows, v, kp, out_type == YP_F32 ? 4 : 2))
     return x_type == YP_INT8 ? tall_x<YP_T_I8>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
          : x_type == YP_F32 ? tall_x<YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
