@@ -255,16 +255,18 @@ static hipError_t one_row_x(int v, int k, const void* x, const float* x_scale, c
                              : one_row_t<XTYPE, YP_T_F16>(v, k, x, x_scale, wq, w_scale, bias, out, st);
 }
 
-// ---- many rows, a small weight: the head over all anchors ------------------------------------------------------------
-// x is read once, and that is most of it.  A wave takes 16 rows and keeps them in registers in the order of the matrix
+// ---- a small weight: the head over anchors ---------------------------------------------------------------------------
+// x is read once, and that is most of it: 25.4 us for 76992 x 256 float32 against 81 rows (105 MB: 4.1 TB/s; quantizing
+// and the tile engine apart 52 us).  From two rows on: the device takes 0 to 2 us longer below 4096 than with the two
+// kernels, a caller launches one less (9.7 us a call against 11.5).  A wave takes 16 rows and keeps them in registers in the order of the matrix
 // instruction - lane l holds row l & 15, and of every 64 k those that 16-byte loads bring to quarter l >> 4 (which k they
 // are does not matter as long as the weight has the same order: it is laid out so in LDS, once per workgroup) -, so the
 // row's maximum is two shuffles and the quotients never leave the lane.  The results go through LDS, 16 rows at a time,
 // and out as one run of 16-byte stores: 16 rows are a multiple of 16 bytes whatever v is.
-#define YP_TR_LDS 81920
+#define YP_SW_LDS 81920
 
 template <int XTYPE, int OUT, int STEPS>   // STEPS: 64 k each, at most
-__global__ __launch_bounds__(YP_QR_THREADS) void yp_tall_kernel(const void* x, const float* x_scale, int rows, int v, int k, int kp, const char* wq,
+__global__ __launch_bounds__(YP_QR_THREADS) void yp_small_weight_kernel(const void* x, const float* x_scale, int rows, int v, int k, int kp, const char* wq,
                                                                 const float* w_scale, const float* bias, void* out, int vec, int out_vec) {
   typedef typename yp_type<OUT>::elem oelem;
   constexpr int XB = yp_type<XTYPE>::bytes, E = 16 / XB, LOADS = 4 * XB / 4;   // loads per 64 k: 4 (f32), 2, 1
@@ -355,11 +357,11 @@ __global__ __launch_bounds__(YP_QR_THREADS) void yp_tall_kernel(const void* x, c
   }
 }
 
-static bool tall_fits(int rows, int v, int64_t kp, int out_bytes) {
-  return rows >= 4096 && kp <= 512 && (int64_t)(v + 15) / 16 * 16 * (kp + 8) + (int64_t)64 * v * out_bytes <= YP_TR_LDS;
+static bool small_weight(int v, int64_t kp, int out_bytes) {
+  return kp <= 512 && (int64_t)(v + 15) / 16 * 16 * (kp + 8) + (int64_t)64 * v * out_bytes <= YP_SW_LDS;
 }
 template <int XTYPE, int OUT>
-static hipError_t tall_t(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, hipStream_t st) {
+static hipError_t small_weight_t(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, hipStream_t st) {
   const int kp = (int)yp_qrow_bytes(k);
   const size_t lds = (size_t)(v + 15) / 16 * 16 * (kp + 8) + (size_t)64 * v * yp_type<OUT>::bytes;
   int64_t blocks = ((int64_t)rows + 63) / 64, resident = 256 * (163840 / (int64_t)lds < 4 ? 163840 / (int64_t)lds : 4);
@@ -367,23 +369,23 @@ static hipError_t tall_t(int rows, int v, int k, const void* x, const float* x_s
   int vec = 0;
   if constexpr (XTYPE != YP_T_I8) vec = row_vec<XTYPE>(k, x);
   const int out_vec = ((uintptr_t)out & 15) == 0;
-  const void* const fn = kp <= 256 ? reinterpret_cast<const void*>(&yp_tall_kernel<XTYPE, OUT, 4>) : reinterpret_cast<const void*>(&yp_tall_kernel<XTYPE, OUT, 8>);
+  const void* const fn = kp <= 256 ? reinterpret_cast<const void*>(&yp_small_weight_kernel<XTYPE, OUT, 4>) : reinterpret_cast<const void*>(&yp_small_weight_kernel<XTYPE, OUT, 8>);
   if (lds > 48 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, YP_TR_LDS);
+    const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, YP_SW_LDS);
     if (e != hipSuccess) return e;
   }
   if (kp <= 256)
-    hipLaunchKernelGGL((yp_tall_kernel<XTYPE, OUT, 4>), dim3((unsigned)blocks), dim3(YP_QR_THREADS), lds, st, x, x_scale, rows, v, k, kp, (const char*)wq, w_scale, bias, out, vec, out_vec);
+    hipLaunchKernelGGL((yp_small_weight_kernel<XTYPE, OUT, 4>), dim3((unsigned)blocks), dim3(YP_QR_THREADS), lds, st, x, x_scale, rows, v, k, kp, (const char*)wq, w_scale, bias, out, vec, out_vec);
   else
-    hipLaunchKernelGGL((yp_tall_kernel<XTYPE, OUT, 8>), dim3((unsigned)blocks), dim3(YP_QR_THREADS), lds, st, x, x_scale, rows, v, k, kp, (const char*)wq, w_scale, bias, out, vec, out_vec);
+    hipLaunchKernelGGL((yp_small_weight_kernel<XTYPE, OUT, 8>), dim3((unsigned)blocks), dim3(YP_QR_THREADS), lds, st, x, x_scale, rows, v, k, kp, (const char*)wq, w_scale, bias, out, vec, out_vec);
   return hipGetLastError();
 }
 template <int XTYPE>
-static hipError_t tall_x(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, int out_type,
+static hipError_t small_weight_x(int rows, int v, int k, const void* x, const float* x_scale, const void* wq, const float* w_scale, const float* bias, void* out, int out_type,
                          hipStream_t st) {
-  return out_type == YP_F32 ? tall_t<XTYPE, YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
-       : out_type == YP_BF16 ? tall_t<XTYPE, YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
-                             : tall_t<XTYPE, YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st);
+  return out_type == YP_F32 ? small_weight_t<XTYPE, YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
+       : out_type == YP_BF16 ? small_weight_t<XTYPE, YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st)
+                             : small_weight_t<XTYPE, YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, st);
 }
 
 template <int OUT>
@@ -433,11 +435,11 @@ hipError_t yp_launch_quantized_linear(int rows, int v, int k, int x_type, const 
          : x_type == YP_F32 ? one_row_x<YP_T_F32>(v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
          : x_type == YP_BF16 ? one_row_x<YP_T_BF16>(v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
                              : one_row_x<YP_T_F16>(v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
-  if (tall_fits(rows, v, kp, out_type == YP_F32 ? 4 : 2))
-    return x_type == YP_INT8 ? tall_x<YP_T_I8>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
-         : x_type == YP_F32 ? tall_x<YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
-         : x_type == YP_BF16 ? tall_x<YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
-                             : tall_x<YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
+  if (small_weight(v, kp, out_type == YP_F32 ? 4 : 2))
+    return x_type == YP_INT8 ? small_weight_x<YP_T_I8>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_F32 ? small_weight_x<YP_T_F32>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+         : x_type == YP_BF16 ? small_weight_x<YP_T_BF16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st)
+                             : small_weight_x<YP_T_F16>(rows, v, k, x, x_scale, wq, w_scale, bias, out, out_type, st);
   if (x_type != YP_INT8) {
     float* const s = (float*)((char*)workspace + rows * kp);
     const hipError_t e = yp_launch_quantize_rows(rows, k, x_type, x, workspace, s, st);
