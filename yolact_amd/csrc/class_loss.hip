@@ -329,7 +329,7 @@ struct yp_peak_args {
   const float* bias;           // of the second, may be null
   float* part;                 // [2][YP_PEAK_BLOCKS]
 };
-#define YP_PEAK_BLOCKS 512
+#define YP_PEAK_BLOCKS 2048
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_args a) {
   __shared__ float red[YP_CL_THREADS / 64];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
@@ -339,14 +339,31 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
     for (int64_t r = (int64_t)blockIdx.x * (YP_CL_THREADS / 64) + wave; r < a.rows[j]; r += YP_PEAK_BLOCKS * (YP_CL_THREADS / 64)) {
       if (j == 0 ? a.labels.counted(r) < 0 : a.bias && a.bias[r] == -INFINITY) continue;
       const float* const p = a.src[j] + r * a.d;
+      int c = lane * 4;
       if (a.vec) {
-        for (int c = lane; c < a.d / 4; c += 64) {
-          const yp_f4 v = reinterpret_cast<const yp_f4*>(p)[c];
+        for (; c + 768 < a.d; c += 1024) {      // four loads in flight
+          yp_f4 v[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) top = fmaxf(top, fabsf(v[u]));
+          for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const yp_f4*>(p + c + u * 256);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[u][e]));
+        }
+        for (; c < a.d; c += 256) {
+          const yp_f4 v = *reinterpret_cast<const yp_f4*>(p + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[e]));
         }
       } else {
-        for (int c = lane; c < a.d; c += 64) top = fmaxf(top, fabsf(p[c]));
+        for (c = lane; c + 448 < a.d; c += 512) {
+          float v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) v[u] = p[c + u * 64];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(v[u]));
+        }
+        for (; c < a.d; c += 64) top = fmaxf(top, fabsf(p[c]));
       }
     }
 #pragma unroll

@@ -55,7 +55,8 @@ static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I
       for (int64_t sb = 1; sb == 1 || (sb <= steps2 / 8 && tb * sb <= 1024); sb *= 2) {
         const double qa = (double)steps1 / sa, qb = (double)steps2 / sb, wgs = ta * sa + tb * sb;
         const double longest = (qa > qb ? qa : qb) * alone + 5;
-        double c = yp_plan_cost(shape, wgs, (ta * sa * qa + tb * sb * qb) / wgs);
+        // (by k, T reads LDS twice as often as it can: 310 TFLOP/s with the card full)
+        double c = (shape == YP_TILE_T && wgs > 512 ? 2.0 : 1.0) * yp_plan_cost(shape, wgs, (ta * sa * qa + tb * sb * qb) / wgs);
         if (c < longest) c = longest;
         if (sa > 1 || sb > 1) c += 6 + ((sa > 1 ? (double)I1 * J1 * sa : 0) + (sb > 1 ? (double)I2 * J2 * sb : 0)) * 8 / 5e6;
         if (c < least) {
