@@ -32,7 +32,7 @@
 #define YP_CL_FINE_ROWS 512
 #define YP_CL_FINE_WORK (1ll << 30)
 #define YP_CL_PIECE_MAX (1 << 17)
-#define YP_CL_PIECE_BYTES (128ll << 20)   // of dz: half of the Infinity Cache
+#define YP_CL_PIECE_BYTES (256ll << 20)   // of dz: the Infinity Cache (128 MB and 512 MB: up to 10 % slower)
 
 __device__ __forceinline__ int64_t yp_label_at(const void* labels, int64_t n, int bytes) {
   return bytes == 8 ? reinterpret_cast<const int64_t*>(labels)[n] : (int64_t)reinterpret_cast<const int32_t*>(labels)[n];
