@@ -61,6 +61,13 @@ def test_class_loss_large_tiles_and_pieces(n, v, d, bias, dt):
     _check_loss(*_loss_inputs(n, v, d, dt, bias=bias, ignored=0.1))
 
 
+@pytest.mark.parametrize("n,v,d,dt,bias", [(1 << 18, 3, 8, torch.bfloat16, True), (1 << 18, 40, 16, torch.float32, False), (2, 1 << 21, 8, torch.float16, True),
+                                           (1, 1 << 21, 4, torch.float32, False), (3, 5, 65536, torch.bfloat16, True), (70, 90, 65536, torch.float32, True),
+                                           (100000, 513, 40, torch.float16, True), (513, 4000, 2048, torch.bfloat16, True)])
+def test_class_loss_long_axes(n, v, d, dt, bias):
+    _check_loss(*_loss_inputs(n, v, d, dt, bias, 0.1))
+
+
 @pytest.mark.parametrize("dt", TYPES, ids=str)
 @pytest.mark.parametrize("n,v,d", [(200, 333, 64), (1500, 2900, 500)])
 def test_class_loss_ignored_rows_and_masked_classes_may_hold_anything(n, v, d, dt):
@@ -305,6 +312,16 @@ def test_quantized_linear_largest_sums():
     y = _check_quantized(x, w, None, torch.float32)
     assert float(y[0, 0]) > 0 and float(y[0, 1]) < 0
     assert abs(float(y[0, 0]) - k) < 1
+
+
+def test_dropout_past_32_bits_of_elements():
+    """2^32 + 5 elements: the mask of the last ones."""
+    from yolact_amd import heads
+    n = (1 << 32) + 5
+    y = heads.dropout(torch.ones(n, dtype=torch.bfloat16, device="cuda"), 0.5, _state(5, 7))
+    tail = (y[-4101:] != 0).cpu().numpy()
+    first = n - 4101
+    assert np.array_equal(tail, ref.keep_mask(4104, 0.5, 5, 7 + first // 4)[first % 4:][:4101])
 
 
 def test_quantized_linear_empty_and_unaligned():

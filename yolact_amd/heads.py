@@ -76,7 +76,8 @@ def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
     int32), with ``lse = log sum exp`` of the logits and ``losses = lse - logit[label]``.
 
     A row labelled ``ignore_index`` takes no part (loss 0) whatever its features hold; any other label outside [0, V) has
-    loss NaN.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf."""
+    loss NaN.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf.
+    No gradient is recorded here: ``ClassLoss`` is the differentiable form."""
     args = _class_loss_args(features, weight, labels, bias)
     lead, dev = args[-2:]
     losses = torch.empty(lead, dtype=torch.float32, device=dev)
@@ -153,7 +154,8 @@ def dropout(x, p: float, state, out=None):
     0 (also where x is not finite).  ``state`` is an int64 CUDA tensor [2]: the key and the first counter; element i uses
     word i % 4 of Philox4x32-10 at counter ``state[1] + i // 4``.  The same state gives the same mask - which is how the
     backward pass has it - so advance ``state[1]`` by ``(x.numel() + 3) // 4`` before the next use, and not before the
-    backward of this one.  It is read on the device: a captured call follows it on every replay.  ``out`` may be x."""
+    backward of this one.  It is read on the device: a captured call follows it on every replay.  ``out`` may be x.
+    No gradient is recorded here: ``Dropout`` is the differentiable form."""
     p_x = _check("x", x, _TYPES)
     dev = x.device
     p_s = _check("state", state, (torch.int64,), (2,), dev)
@@ -231,7 +233,8 @@ def quantize_rows(x) -> QuantizedRows:
 def quantized_linear(x, weight: QuantizedRows, bias=None, out_dtype=torch.float32):
     """``x @ weight^T + bias`` with 8-bit integer products: ``x`` [..., k] float32 / bfloat16 / float16 (quantized row by row
     on the way) or ``QuantizedRows``; ``weight`` = ``quantize_rows`` of a [v, k] matrix; ``bias`` float32 [v].  Returns
-    [..., v] of ``out_dtype``: integer sums are exact, scales and bias are applied in float32, one rounding to the type."""
+    [..., v] of ``out_dtype``: integer sums are exact, scales and bias are applied in float32, one rounding to the type.
+    For answering: no gradient is recorded."""
     if not isinstance(weight, QuantizedRows) or len(weight.lead) != 1 or weight.lead[0] < 1:
         raise ValueError("weight must be quantize_rows of a [v, k] matrix")
     if out_dtype not in _TYPES:
