@@ -61,6 +61,13 @@ def test_class_loss_large_tiles_and_pieces(n, v, d, bias, dt):
     _check_loss(*_loss_inputs(n, v, d, dt, bias=bias, ignored=0.1))
 
 
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(9000, 18011, 68), (9001, 18011, 1031), (500, 140001, 41), (257, 150000, 1024)])
+def test_class_loss_over_pieces_of_the_backward_pass(n, v, d, dt):
+    """The gradient of the features adds up over pieces of the vocabulary, with and without a split of that axis."""
+    _check_loss(*_loss_inputs(n, v, d, dt, True, 0.1))
+
+
 @pytest.mark.parametrize("n,v,d,dt,bias", [(1 << 18, 3, 8, torch.bfloat16, True), (1 << 18, 40, 16, torch.float32, False), (2, 1 << 21, 8, torch.float16, True),
                                            (1, 1 << 21, 4, torch.float32, False), (3, 5, 65536, torch.bfloat16, True), (70, 90, 65536, torch.float32, True),
                                            (100000, 513, 40, torch.float16, True), (513, 4000, 2048, torch.bfloat16, True)])

@@ -124,7 +124,7 @@ struct yp_scale {
 // (what is exactly zero stays so, whatever the factor)
 __device__ __forceinline__ float yp_times(float v, float scale) { return v == 0.0f ? 0.0f : v * scale; }
 
-// out[j][i] = scale * C, in type OUT; or, with `part`, the f32 sums of this split for a later join
+// out[j][i] = scale * (C + before[j][i]), in type OUT; or, with `part`, the f32 sums of this split for a later join
 // (part[split][j][i], added to what is there if `add`).
 template <int OUT>
 struct yp_epi_store {
@@ -132,6 +132,7 @@ struct yp_epi_store {
   int64_t ld;             // elements
   int vec, part_vec;      // rows of out / of part are multiples of 16 bytes
   yp_scale scale;
+  const float* before;    // null: nothing (16-bit types only: those of f32 lose more to the registers it takes)
   float* part;
   int add;
   template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
@@ -143,6 +144,24 @@ struct yp_epi_store {
       else yp_put_tile<YP_T_F32, SHAPE, false, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
     } else {
       const float sc = scale.get();
+      if (OUT != YP_T_F32 && before) {
+        typedef yp_shape<SHAPE> S;
+        int i0, j0;
+        yp_origin<SHAPE>(at, i0, j0);
+#pragma unroll
+        for (int n = 0; n < NJ; ++n)
+#pragma unroll
+          for (int m = 0; m < MI; ++m) {
+            const int i = i0 + yp_frag_at<S::BM, MI>(m), j = j0 + yp_frag_at<S::BN, NJ>(n);
+            if (j < g.J && i < g.I) {
+              const float* const b = before + (int64_t)j * g.I + i;
+              if (part_vec) acc[m][n] = acc[m][n] + *reinterpret_cast<const yp_f4*>(b);      // (I is a multiple of four)
+              else
+#pragma unroll
+                for (int r = 0; r < 4; ++r) if (i + r < g.I) acc[m][n][r] += b[r];
+            }
+          }
+      }
       yp_put_tile<OUT, SHAPE, false, MI, NJ>(at, out, ld, g.I, g.J, vec != 0, [&](int m, int n) {
         yp_f4 v;
 #pragma unroll
