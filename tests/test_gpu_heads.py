@@ -93,6 +93,33 @@ def test_class_loss_ignored_rows_and_masked_classes_may_hold_anything(n, v, d, d
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(100, 333, 64), (2048, 8192, 128)])
+@pytest.mark.parametrize("what", [1e30, -math.inf, NAN], ids=str)
+def test_class_loss_gradients_of_ignored_rows_may_hold_anything(n, v, d, dt, what):
+    h, w, b, y, up = _loss_inputs(n, v, d, dt, True, 0.3)
+    up[y == -1] = what
+    _check_loss(h, w, b, y, up)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(100, 333, 64), (2048, 8192, 128)])
+@pytest.mark.parametrize("what", [math.inf, NAN], ids=str)
+def test_class_loss_a_gradient_that_is_not_finite_stays_with_its_row(n, v, d, dt, what):
+    from yolact_amd import heads
+    h, w, b, y, up = _loss_inputs(n, v, d, dt, True, 0.0)
+    up *= 2.0 ** -30
+    _, lse = heads.class_loss(h, w, y, bias=b)
+    bad = up.clone()
+    bad[5] = what
+    gh, gw, _ = heads.class_loss_backward(h, w, y, lse, bad, bias=b)
+    up[5] = 0.0
+    value, bound = ref.class_loss(h, w, b, y, up)["grad_h"]
+    rest = torch.arange(n, device="cuda") != 5
+    ref.within(gh[rest], value[rest], bound[rest], "grad_features")
+    assert not torch.isfinite(gh[5]).any() and not torch.isfinite(gw).any()
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
 def test_class_loss_labels_that_cannot_be(dt):
     """A masked class as label: +inf.  A label outside the vocabulary: NaN, no gradient, nothing else touched."""
     h, w, b, y, up = _loss_inputs(50, 40, 32, dt, True, 0.2)

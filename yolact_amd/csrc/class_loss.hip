@@ -483,26 +483,32 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_reduce_kernel(const double* 
   if (threadIdx.x == 0) reduced.put(ts, tc);
 }
 
-// {by / largest |g|, largest |g| / by}
-__global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, int64_t n, float by, float* factor) {
+// {by / largest |g|, largest |g| / by} over the rows that take part (whose g is finite: what an infinity gives is no
+// matter of scale)
+__global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, const yp_labels labels, int64_t n, float by, float* factor) {
   __shared__ float red[16];
   float top = 0.0f;
+  auto see = [&](float v, int label) {
+    v = fabsf(v);
+    top = fmaxf(top, label >= 0 && v < INFINITY ? v : 0.0f);
+  };
   int64_t i = threadIdx.x;
   for (; i + 3 * 1024 < n; i += 4 * 1024) {
     float v[4];
+    int l[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = grad[i + u * 1024];
+    for (int u = 0; u < 4; ++u) { v[u] = grad[i + u * 1024]; l[u] = labels.counted(i + u * 1024); }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) top = fmaxf(top, fabsf(v[u]));
+    for (int u = 0; u < 4; ++u) see(v[u], l[u]);
   }
-  for (; i < n; i += 1024) top = fmaxf(top, fabsf(grad[i]));
+  for (; i < n; i += 1024) see(grad[i], labels.counted(i));
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
-    if (!(top >= 0x1p-100f && top <= 0x1p100f)) top = 1.0f;      // (nothing to go by)
+    if (!(top >= 0x1p-112f)) top = 1.0f;      // (nothing to go by)
     factor[0] = by / top;
     factor[1] = top / by;
   }
@@ -802,7 +808,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     back = yp_scale{nullptr, a.count, 1.0f, {}};
     if (TYPE != YP_T_F32) {                                 // (f32 as it is: dz is not rounded)
       factor = (float*)(ws + p.o_factor);
-      hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, (int64_t)a.n, up, factor);
+      hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, labels, (int64_t)a.n, up, factor);
       CL_TRY(hipGetLastError());
       back.a = factor + 1;
     }
