@@ -119,6 +119,23 @@ def test_class_loss_a_gradient_that_is_not_finite_stays_with_its_row(n, v, d, dt
     assert not torch.isfinite(gh[5]).any() and not torch.isfinite(gw).any()
 
 
+@pytest.mark.parametrize("n,v,d", [(100, 333, 64), (2048, 8192, 130)])
+@pytest.mark.parametrize("what", [math.inf, NAN], ids=str)
+def test_class_loss_features_that_are_not_finite_stay_with_their_row(n, v, d, what):
+    from yolact_amd import heads
+    h, w, b, y, up = _loss_inputs(n, v, d, torch.float32, True, 0.0)
+    h, w = h * 2.0 ** 30, w * 2.0 ** -30
+    bad = h.clone()
+    bad[7, 3] = what
+    losses, lse = heads.class_loss(bad, w, y, bias=b)
+    gh, gw, _ = heads.class_loss_backward(bad, w, y, lse, up, bias=b)
+    want = ref.class_loss(h, w, b, y, up)
+    rest = torch.arange(n, device="cuda") != 7
+    for got, name in ((losses, "losses"), (lse, "lse"), (gh, "grad_h")):
+        ref.within(got[rest], want[name][0][rest], want[name][1][rest], name)
+        assert not torch.isfinite(got[7]).any()
+
+
 @pytest.mark.parametrize("dt", TYPES, ids=str)
 def test_class_loss_labels_that_cannot_be(dt):
     """A masked class as label: +inf.  A label outside the vocabulary: NaN, no gradient, nothing else touched."""

@@ -319,8 +319,8 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
   }
 }
 
-// The largest magnitudes of features and weight among the rows that take part - a wave a row -, a part per workgroup; and
-// the powers of two that bring them to [2^14, 2^15), scales[0] and [1].
+// The largest finite magnitudes of features and weight among the rows that take part - a wave a row -, a part per workgroup;
+// and the powers of two that bring them to [2^14, 2^15), scales[0] and [1].
 struct yp_peak_args {
   const float* src[2];
   int64_t rows[2];
@@ -336,6 +336,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     float top = 0.0f;
+    auto see = [&](float v) { v = fabsf(v); top = fmaxf(top, v < INFINITY ? v : 0.0f); };
     for (int64_t r = (int64_t)blockIdx.x * (YP_CL_THREADS / 64) + wave; r < a.rows[j]; r += YP_PEAK_BLOCKS * (YP_CL_THREADS / 64)) {
       if (j == 0 ? a.labels.counted(r) < 0 : a.bias && a.bias[r] == -INFINITY) continue;
       const float* const p = a.src[j] + r * a.d;
@@ -348,12 +349,12 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
 #pragma unroll
           for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[u][e]));
+            for (int e = 0; e < 4; ++e) see(v[u][e]);
         }
         for (; c < a.d; c += 256) {
           const yp_f4 v = *reinterpret_cast<const yp_f4*>(p + c);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[e]));
+          for (int e = 0; e < 4; ++e) see(v[e]);
         }
       } else {
         for (c = lane; c + 448 < a.d; c += 512) {
@@ -361,9 +362,9 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
 #pragma unroll
           for (int u = 0; u < 8; ++u) v[u] = p[c + u * 64];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(v[u]));
+          for (int u = 0; u < 8; ++u) see(v[u]);
         }
-        for (; c < a.d; c += 64) top = fmaxf(top, fabsf(p[c]));
+        for (; c < a.d; c += 64) see(p[c]);
       }
     }
 #pragma unroll
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(128) void yp_scales_kernel(const float* part, float
   for (int i = lane; i < YP_PEAK_BLOCKS; i += 64) top = fmaxf(top, part[j * YP_PEAK_BLOCKS + i]);
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-  if (lane == 0) scales[j] = top > 0.0f && top < INFINITY ? ldexpf(1.0f, min(max(14 - ilogbf(top), -100), 100)) : 1.0f;
+  if (lane == 0) scales[j] = top > 0.0f ? ldexpf(1.0f, min(max(14 - ilogbf(top), -100), 100)) : 1.0f;
 }
 
 __device__ __forceinline__ double yp_block_sum(double v, double* lds) {   // fixed order; result in thread 0
@@ -732,7 +733,7 @@ static hipError_t copy_rows(yp_copy_args a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// TYPE: the matrix instructions'; ELEM: the tensors'.  SPLIT: f32 by three bf16 planes.
+// TYPE: the matrix instructions'; ELEM: the tensors'.  SPLIT: f32 by two f16 planes.
 template <int TYPE, int ELEM, bool SPLIT>
 static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   constexpr int b = yp_type<ELEM>::bytes;
