@@ -283,10 +283,31 @@ def test_python_refusals():
             heads.quantized_linear(x, wq, **kw)
     with pytest.raises(ValueError):
         heads.quantize_rows(h.t())
+    for index in (1 << 63, (1 << 64) - 1, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="ignore_index"):
+            heads.class_loss(h, w, y, ignore_index=index)
+        with pytest.raises(ValueError, match="ignore_index"):
+            heads.ClassLoss.apply(h, w, b, y, index)
     state = torch.zeros(2, dtype=torch.int64, device="cuda")
     for x, p, s in ((h, 1.5, state), (h, 0.5, state[:1]), (h, 0.5, state.int()), (h.t(), 0.5, state), (y, 0.5, state)):
         with pytest.raises(ValueError):
             heads.dropout(x, p, s)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """2^32 + 5 is not 5 (the tensors are large, nothing touches them)."""
+    from yolact_amd import heads
+    many = (1 << 32) + 5
+    long = torch.empty(many, dtype=torch.bfloat16, device="cuda")
+    labels = torch.empty(many, dtype=torch.int32, device="cuda")
+    small, one = torch.zeros(5, 1, dtype=torch.bfloat16, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    wq = heads.quantize_rows(small)
+    for call in (lambda: heads.class_loss(long[:, None], small, labels), lambda: heads.class_loss(small, long[:, None], one),
+                 lambda: heads.class_loss(long[None], long[None], one[:1]), lambda: heads.class_loss_backward(long[:, None], small, labels, labels, labels),
+                 lambda: heads.ClassLoss.apply(long[:, None], small, None, labels), lambda: heads.quantize_rows(long[None]),
+                 lambda: heads.quantize_rows(long[:, None]), lambda: heads.quantized_linear(long[:, None], wq)):
+        with pytest.raises(ValueError, match="too large"):
+            call()
 
 
 # ---- quantized linear ------------------------------------------------------------------------------------------------

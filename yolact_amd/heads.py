@@ -33,6 +33,12 @@ def _check(name, t, dtypes, shape=None, device=None):
                      f", got {t.dtype} {tuple(t.shape)}")
 
 
+def _fits(name, *sizes):
+    for n in sizes:
+        if n > 0x7FFFFFFF:                       # (what the C entries take; a larger one would arrive as another number)
+            raise ValueError(f"{name} of {n} is too large")
+
+
 def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)      # (torch.cuda.current_stream makes an object: 1.9 us of 4)
 
@@ -59,7 +65,15 @@ def _class_loss_args(features, weight, labels, bias):
     p_h = _check("features", features, (weight.dtype,), device=dev)
     p_y = _check("labels", labels, (torch.int64, torch.int32), lead, dev)
     p_b = _check("bias", bias, (weight.dtype,), (V,), dev) if bias is not None else None
+    _fits("rows, classes or features", labels.numel(), V, D)
     return p_h, p_w, p_b, p_y, labels.numel(), V, D, lead, dev
+
+
+def _label(ignore_index):
+    ignore_index = int(ignore_index)
+    if not -1 << 63 <= ignore_index < 1 << 63:
+        raise ValueError("ignore_index must fit an int64")
+    return ignore_index
 
 
 def _class_loss_forward(args, label_bytes, type_, ignore_index, p_losses, p_lse, p_sum=None, p_mean=None, p_count=None):
@@ -82,7 +96,7 @@ def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
     lead, dev = args[-2:]
     losses = torch.empty(lead, dtype=torch.float32, device=dev)
     lse = torch.empty(lead, dtype=torch.float32, device=dev)
-    _class_loss_forward(args, labels.element_size(), _TYPES[weight.dtype], int(ignore_index), losses.data_ptr(), lse.data_ptr())
+    _class_loss_forward(args, labels.element_size(), _TYPES[weight.dtype], _label(ignore_index), losses.data_ptr(), lse.data_ptr())
     return losses, lse
 
 
@@ -108,7 +122,7 @@ def class_loss_backward(features, weight, labels, lse, grad_losses, bias=None, i
     lead, dev = _class_loss_args(features, weight, labels, bias)[-2:]
     _check("lse", lse, (torch.float32,), lead, dev)
     p_grad = _check("grad_losses", grad_losses, (torch.float32,), lead, dev)
-    return _class_loss_backward(features, weight, labels, bias, int(ignore_index), lse.data_ptr(), p_grad, 1, None)
+    return _class_loss_backward(features, weight, labels, bias, _label(ignore_index), lse.data_ptr(), p_grad, 1, None)
 
 
 class ClassLoss(torch.autograd.Function):
@@ -123,7 +137,7 @@ class ClassLoss(torch.autograd.Function):
             raise ValueError(f"reduction must be one of {_REDUCTIONS}")
         features, weight, labels = features.contiguous(), weight.contiguous(), labels.contiguous()
         bias = bias.contiguous() if bias is not None else None
-        ignore_index = int(ignore_index)
+        ignore_index = _label(ignore_index)
         args = _class_loss_args(features, weight, labels, bias)
         N, lead, dev = args[4], args[-2], args[-1]
         kept = torch.empty((N + 1,), dtype=torch.float32, device=dev)          # lse of the rows, and how many count
@@ -220,6 +234,7 @@ def quantize_rows(x) -> QuantizedRows:
         raise ValueError("x must have at least one element per row")
     dev, k, lead = x.device, x.shape[-1], x.shape[:-1]
     rows = x.numel() // k
+    _fits("rows or k", rows, k)
     L = _lib.load()
     kp = int(L.yp_quantized_row_bytes(k))
     if kp < 0:
@@ -252,6 +267,7 @@ def quantized_linear(x, weight: QuantizedRows, bias=None, out_dtype=torch.float3
         if x.dim() < 1 or x.shape[-1] != k:
             raise ValueError(f"x must have rows of {k}")
         lead, rows, dt = x.shape[:-1], x.numel() // k, _TYPES[x.dtype]
+        _fits("rows", rows)
         ws = _workspace(L.yp_quantized_linear_workspace(rows, k), dev)
     out = torch.empty((*lead, v), dtype=out_dtype, device=dev)
     _lib.check(L.yp_quantized_linear(dev.index, rows, v, k, dt, p_x, p_s, weight.q.data_ptr(), weight.scale.data_ptr(), p_b, _ptr(ws),
