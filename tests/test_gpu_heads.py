@@ -409,6 +409,20 @@ def test_quantized_linear_empty_and_unaligned():
     assert torch.equal(heads.quantized_linear(x[0], wq), heads.quantized_linear(x, wq)[0])
 
 
+def test_quantized_rows_made_by_hand():
+    from yolact_amd import heads
+    x = torch.randn(2, 3, 200, generator=_gen(4), device="cuda")
+    w = heads.quantize_rows(torch.randn(9, 200, generator=_gen(5), device="cuda"))
+    a = heads.quantize_rows(x)
+    kept = heads.QuantizedRows(a.q.cpu().cuda(), a.scale.clone(), 200, (2, 3))
+    assert torch.equal(heads.quantized_linear(kept, w), heads.quantized_linear(x, w))
+    for q, scale, k, lead in ((a.q.cpu(), a.scale, 200, (2, 3)), (a.q, a.scale.cpu(), 200, (2, 3)), (a.q[:, :200].contiguous(), a.scale, 200, (2, 3)),
+                              (a.q, a.scale[:5], 200, (2, 3)), (a.q, a.scale, 200, (7,)), (a.q, a.scale, 300, (2, 3)), (a.q, a.scale, 0, (2, 3)),
+                              (a.q.int(), a.scale, 200, (2, 3)), (a.q, a.scale.double(), 200, (2, 3)), (a.q.t().contiguous().t(), a.scale, 200, (2, 3))):
+        with pytest.raises((ValueError, RuntimeError)):
+            heads.QuantizedRows(q, scale, k, lead)
+
+
 # ---- dropout ---------------------------------------------------------------------------------------------------------
 def _state(key, first):
     return torch.tensor([key, first], dtype=torch.int64, device="cuda")

@@ -14,6 +14,8 @@ the call itself, so calls on different streams or captured graphs share nothing.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -211,11 +213,22 @@ def class_head_loss(features, weight, bias, labels, dropout_p: float = 0.0, stat
 
 # ---- quantized linear ------------------------------------------------------------------------------------------------
 class QuantizedRows:
-    """Rows in 8 bits: ``q`` int8 [rows, padded k] (the padding is zero), ``scale`` float32 [rows], ``k``; row r stands for
-    ``q[r, :k] * scale[r]``."""
+    """Rows in 8 bits: ``q`` int8 [rows, padded k] (k up to the next multiple of 128, the padding zero), ``scale`` float32
+    [rows], ``k``, and the shape ``lead`` that the rows had; row r stands for ``q[r, :k] * scale[r]``.  ``quantize_rows`` makes
+    them; so may a caller who has kept ``q`` and ``scale``."""
 
     def __init__(self, q, scale, k, lead):
+        kp = int(_lib.load().yp_quantized_row_bytes(k))
+        if kp < 0:
+            _lib.check(kp)
+        rows = math.prod(lead)
+        _check("q", q, (torch.int8,), (rows, kp))
+        _check("scale", scale, (torch.float32,), (rows,), q.device)
+        self._set(q, scale, k, lead)
+
+    def _set(self, q, scale, k, lead):
         self.q, self.scale, self.k, self.lead = q, scale, int(k), tuple(lead)
+        return self
 
     @property
     def device(self):
@@ -242,7 +255,7 @@ def quantize_rows(x) -> QuantizedRows:
     q = torch.empty((rows, kp), dtype=torch.int8, device=dev)
     scale = torch.empty((rows,), dtype=torch.float32, device=dev)
     _lib.check(L.yp_quantize_rows(dev.index, rows, k, _TYPES[x.dtype], p_x, q.data_ptr(), scale.data_ptr(), _stream(dev)))
-    return QuantizedRows(q, scale, k, lead)
+    return QuantizedRows.__new__(QuantizedRows)._set(q, scale, k, lead)      # (nothing to check)
 
 
 def quantized_linear(x, weight: QuantizedRows, bias=None, out_dtype=torch.float32):
