@@ -339,7 +339,8 @@ int yp_quantized_linear(int32_t device_id, int32_t rows, int32_t v, int32_t k, i
  * Philox4x32-10 (Salmon et al. 2011) under the 64-bit key state[0] at the 64-bit counter state[1] + i / 4 is
  * >= floor(p 2^32), and then y = x / (1 - p); otherwise y = 0, whatever x holds.  0 <= p <= 1, 0 <= count <= 2^40.  The backward pass is the
  * same call on the gradient with the same state.  state [2] int64 on the device: a captured call reads it on every
- * replay; advance state[1] by (count + 3) / 4 between uses.  y may be x.  Asynchronous on hip_stream. */
+ * replay; advance state[1] by (count + 3) / 4 between uses.  y may be x, but not overlap it
+ * otherwise.  Asynchronous on hip_stream. */
 int yp_dropout(int32_t device_id, int64_t count, int32_t dtype, double p, const int64_t* state, const void* x, void* y, void* hip_stream);
 
 /* Bytes of device scratch the handle holds. */

@@ -464,6 +464,22 @@ def test_dropout_any_counter_unaligned_in_place_and_not_finite():
     assert heads.dropout(torch.empty(0, 5, device="cuda"), 0.5, _state(1, 2)).shape == (0, 5)
 
 
+def test_dropout_into_a_tensor_that_a_graph_has_kept_is_seen():
+    from yolact_amd import heads
+    state = torch.tensor([3, 0], device="cuda")
+    x = torch.randn(64, device="cuda", requires_grad=True)
+    y = x * 2.0
+    z = y * y
+    heads.dropout(y.detach(), 0.5, state, out=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    with pytest.raises(RuntimeError, match="overlap"):
+        heads.dropout(x.detach()[:32], 0.5, state, out=x.detach()[8:40])
+    with torch.inference_mode():
+        a = torch.ones(10, device="cuda")
+        assert heads.dropout(a, 1.0, state, out=a) is a and not a.any()
+
+
 @pytest.mark.parametrize("dt", TYPES, ids=str)
 def test_dropout_autograd(dt):
     from yolact_amd import heads

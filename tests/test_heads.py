@@ -120,6 +120,12 @@ def test_quantize_rows_and_dropout_refuse():
     assert L.yp_dropout(0, 0, 0, 0.5, None, None, None, None) == 0
 
 
+def test_dropout_refuses_tensors_that_overlap_in_part():
+    L = _lib.load()
+    for dtype, apart in ((0, 12), (0, -12), (1, 6), (2, -2)):
+        _refused(L.yp_dropout(0, 4, dtype, 0.5, P, ctypes.c_void_p(8192), ctypes.c_void_p(8192 + apart), None), "overlap")
+
+
 def test_workspace_sizes():
     L = _lib.load()
     assert L.yp_quantized_row_bytes(1) == 128 and L.yp_quantized_row_bytes(129) == 256

@@ -863,6 +863,8 @@ extern "C" int yp_dropout(int32_t device_id, int64_t count, int32_t dtype, doubl
   if (count == 0) return YP_OK;
   if (!state || !x || !y) return fail(YP_EINVAL, "yp_dropout: null argument");
   if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || ((uintptr_t)state & 7) != 0) return fail(YP_EINVAL, "yp_dropout: a tensor is not aligned to its elements");
+  const uintptr_t from = (uintptr_t)x, to = (uintptr_t)y, apart = from < to ? to - from : from - to;
+  if (apart != 0 && apart < (uint64_t)count * (dtype == YP_F32 ? 4 : 2)) return fail(YP_EINVAL, "yp_dropout: y may be x, but not overlap it otherwise");
   YP_ON_DEVICE(device_id);
   YP_HIP(yp_launch_dropout(count, dtype, p, state, x, y, (hipStream_t)hip_stream));
   return YP_OK;

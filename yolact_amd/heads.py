@@ -170,17 +170,21 @@ def dropout(x, p: float, state, out=None):
     0 (also where x is not finite).  ``state`` is an int64 CUDA tensor [2]: the key and the first counter; element i uses
     word i % 4 of Philox4x32-10 at counter ``state[1] + i // 4``.  The same state gives the same mask - which is how the
     backward pass has it - so advance ``state[1]`` by ``(x.numel() + 3) // 4`` before the next use, and not before the
-    backward of this one.  It is read on the device: a captured call follows it on every replay.  ``out`` may be x.
+    backward of this one.  It is read on the device: a captured call follows it on every replay.  ``out`` may be x, but not
+    overlap it otherwise; torch sees it change, as by an operation in place.
     No gradient is recorded here: ``Dropout`` is the differentiable form."""
     p_x = _check("x", x, _TYPES)
     dev = x.device
     p_s = _check("state", state, (torch.int64,), (2,), dev)
     if not 0.0 <= float(p) <= 1.0:
         raise ValueError("p must be in [0, 1]")
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty_like(x)
     p_o = _check("out", out, (x.dtype,), x.shape, dev)
     _lib.check(_lib.load().yp_dropout(dev.index, x.numel(), _TYPES[x.dtype], float(p), p_s, p_x, p_o, _stream(dev)))
+    if not (made or out.is_inference()):
+        torch.autograd.graph.increment_version(out)
     return out
 
 
