@@ -136,6 +136,38 @@ def test_class_loss_features_that_are_not_finite_stay_with_their_row(n, v, d, wh
         assert not torch.isfinite(got[7]).any()
 
 
+@pytest.mark.parametrize("far", [2.0 ** 16, 2.0 ** 24, 2.0 ** 36], ids=str)
+def test_class_loss_large_float32_beside_far_larger_values(far):
+    """Every value is off by at most 2^-22 of itself or 2^-39 of the largest of its tensor, dz by 2^-38 of the largest g: one
+    row of features and one class are `far` times the others.  A logit is then off by sum_d (eh |w| + |h| ew) more, eh and ew
+    being those errors, and what follows from it by the same part."""
+    from yolact_amd import heads
+    n, v, d = 2048, 8192, 128
+    h, w, b, y, up = _loss_inputs(n, v, d, torch.float32, True, 0.1)
+    h[17] *= far
+    y[17] = -1 if far > 2.0 ** 30 else y[17]        # (a row that takes no part sets no scale)
+    w[99] *= min(far, 2.0 ** 24)
+    losses, lse = heads.class_loss(h, w, y, bias=b)
+    gh, gw, gb = heads.class_loss_backward(h, w, y, lse, up, bias=b)
+    want = ref.class_loss(h, w, b, y, up)
+    kept = y >= 0
+    ah, aw = h.double().abs() * kept[:, None], w.double().abs()
+    eh, ew = torch.maximum(ah * 2.0 ** -22, ah.max() * 2.0 ** -39 * kept[:, None]), torch.maximum(aw * 2.0 ** -22, aw.max() * 2.0 ** -39 + 0 * aw)
+    ez = (eh @ (aw + ew).t() + ah @ ew.t()).amax(dim=1)                                  # [n]
+    ref.within(losses[kept], want["losses"][0][kept], (want["losses"][1] + 2 * ez)[kept], "losses")
+    ref.within(lse[kept], want["lse"][0][kept], (want["lse"][1] + ez)[kept], "lse")
+    g = up.double() * kept
+    z = torch.where(kept[:, None], h, 0 * h).double() @ w.double().t() + b.double()
+    p = torch.exp(z - torch.logsumexp(z, dim=1, keepdim=True))
+    dz = p.clone()
+    dz[torch.arange(n, device="cuda")[kept], y[kept]] -= 1.0
+    dz = dz.abs() * g[:, None]
+    ep = torch.nan_to_num(p * torch.expm1(2 * ez)[:, None], nan=1.0, posinf=1.0).clamp(max=1.0)     # (both are in [0, 1])
+    edz = g[:, None] * ep + torch.maximum(dz * 2.0 ** -22, g.max() * 2.0 ** -38 * (g > 0)[:, None])
+    ref.within(gh, want["grad_h"][0], want["grad_h"][1] + edz @ (aw + ew) + dz @ ew, "grad_features")
+    ref.within(gw, want["grad_w"][0], want["grad_w"][1] + edz.t() @ (ah + eh) + dz.t() @ eh, "grad_weight")
+
+
 @pytest.mark.parametrize("dt", TYPES, ids=str)
 def test_class_loss_labels_that_cannot_be(dt):
     """A masked class as label: +inf.  A label outside the vocabulary: NaN, no gradient, nothing else touched."""
@@ -171,6 +203,31 @@ def test_class_loss_nothing_left():
     assert float(loss.detach()) == 0.0
     gs = torch.autograd.grad(loss, (h0, ww, bb))
     assert gs[0].shape == (0, 32) and not gs[1].any() and not gs[2].any()
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_class_loss_logits_beyond_the_precision_of_their_exponentials(dt):
+    """z = +-c beside zeros, c about 2^20 to 2^40 (f16: 2^30): z log2 e is off by 2^-24 of itself, which is more than any
+    exponent for the larger ones.  lse is c to a few half steps; the gradient lies between 0 and g w, whatever p came to."""
+    from yolact_amd import heads
+    for c in range(20, 41 if dt != torch.float16 else 31):
+        h = torch.zeros(40, 8, dtype=dt, device="cuda")
+        w = torch.zeros(300, 8, dtype=dt, device="cuda")
+        h[:20, 0], h[20:, 0] = 1.3 * 2.0 ** (c // 2), -1.3 * 2.0 ** (c // 2)
+        w[7, 0] = 1.2 * 2.0 ** (c - c // 2)
+        z = float(h[0, 0].double() * w[7, 0].double())
+        y = torch.tensor([7, 9, 7, 9], device="cuda").repeat_interleave(10)
+        up = torch.full((40,), 2.0 ** -12, device="cuda")
+        losses, lse = heads.class_loss(h, w, y)
+        gh, gw, _ = heads.class_loss_backward(h, w, y, lse, up)
+        low = math.log(299)
+        rows = lambda *v: torch.tensor(v, dtype=torch.float64, device="cuda").repeat_interleave(10)
+        ref.within(lse, rows(z, z, low, low), rows(z, z, 0, 0) * 2.0 ** -22 + 2e-6, "lse")
+        ref.within(losses, rows(0, z, z + low, low), rows(z, z, z, 0) * 2.0 ** -22 + 2e-6, "losses")
+        assert torch.isfinite(gh).all() and torch.isfinite(gw).all()
+        top = float(w[7, 0]) * 2.0 ** -12 * (1 + ref.HALF[dt])
+        assert float(gh[:, 0].double().abs().max()) <= top and not gh[30:].any() and not gh[:, 1:].any()
+        assert bool((gh[:10, 0] <= 0).all()) and bool((gh[10:20, 0] >= 0).all())
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=str)

@@ -18,7 +18,9 @@
 // is taken out altogether -, which the results get back in f32: with g inside, every row's -g would be rounded the same
 // way, and sums over rows be off by as much as one of them.  f16 with 2^13 more, so that probabilities down to 2^-38 are
 // kept.  Where rows are few, their roundings do not average out, and dz has two planes (twice the precision).
-// f32 of any size worth it runs on the f16 matrix instructions, as two f16 planes per operand (SPLIT; gemm_tile.hpp).
+// f32 of any size worth it runs on the f16 matrix instructions, as two f16 planes per operand (SPLIT; gemm_tile.hpp): 22 bits
+// of a value, or 2^-39 of the largest one where that is more - a value below 2^-17 of the largest has fewer bits than f32,
+// its share of a sum over both is as good.
 // What takes no part has dz = 0, but 0 times NaN is NaN: the gradient products read a copy of h in which ignored rows are
 // zero (and of w, if a bias may mask classes).
 // All sums are f32 in a fixed order: no float atomics, the same call gives the same bits.
@@ -114,6 +116,8 @@ struct yp_epi_stats {
       for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][r], YP_LOG2E, c));
+      // between 1 and the number of terms, whatever the rounding of c makes of it (2^-24 of ref: for 10^9, anything)
+      if (top != -INFINITY) sum = sum < 1.0f ? 1.0f : sum > MI * 4.0f ? MI * 4.0f : sum;
       const int64_t l = j < g.J ? labels.at(j) - first - ib : -1;
       const bool mine = l >= 0 && l < S::BM;
       if (__builtin_amdgcn_ballot_w64(mine)) {      // (mostly no lane of the wave)
@@ -184,8 +188,9 @@ struct yp_epi_dz {
       const int j = jb + yp_frag_at<S::BN, NJ>(n);
       const int label = j < g.J ? labels.counted(j) : -1;
       const float l = label >= 0 ? lse[j] : INFINITY;
-      const float gr = label < 0 ? 0.0f : grad ? grad[j] * by : by;
-      // exp(z - lse) = 2^(z log2e + c); a row that takes no part, or has no class left: 2^-inf = 0
+      // exp(z - lse) = 2^min(z log2e + c, 0) - rounding may bring z above lse, by any amount where large products cancel -; a
+      // row that takes no part, or has no class left: 2^-inf = 0; one with NaN among its z has it in lse, and here in gr
+      const float gr = label < 0 ? 0.0f : l != l ? l : grad ? grad[j] * by : by;
       const float c = l == -INFINITY ? -INFINITY : -l * YP_LOG2E;
       const int hit = label < 0 ? -1 : label - first - ib;
       if (__builtin_amdgcn_ballot_w64(hit >= 0 && hit < S::BM)) {      // (mostly no lane of the wave)
@@ -193,14 +198,14 @@ struct yp_epi_dz {
         for (int m = 0; m < MI; ++m)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float z = acc[m][n][r], p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, YP_LOG2E, c));
+            const float z = acc[m][n][r], p = __builtin_amdgcn_exp2f(fminf(__builtin_fmaf(z, YP_LOG2E, c), 0.0f));
             acc[m][n][r] = (hit == yp_frag_at<S::BM, MI>(m) + r && z != -INFINITY ? p - 1.0f : p) * gr;
           }
       } else {
 #pragma unroll
         for (int m = 0; m < MI; ++m)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[m][n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][r], YP_LOG2E, c)) * gr;
+          for (int r = 0; r < 4; ++r) acc[m][n][r] = __builtin_amdgcn_exp2f(fminf(__builtin_fmaf(acc[m][n][r], YP_LOG2E, c), 0.0f)) * gr;
       }
     }
     if (bias_out) {   // sums over the tile's rows: 16 lanes, then the waves that share the classes

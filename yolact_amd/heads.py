@@ -93,6 +93,7 @@ def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
 
     A row labelled ``ignore_index`` takes no part (loss 0) whatever its features hold; any other label outside [0, V) has
     loss NaN.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf.
+    Large float32 calls (2^31 multiplications and more) take each value to 2^-22 of itself or 2^-39 of the largest in its tensor.
     No gradient is recorded here: ``ClassLoss`` is the differentiable form."""
     args = _class_loss_args(features, weight, labels, bias)
     lead, dev = args[-2:]
@@ -130,8 +131,8 @@ def class_loss_backward(features, weight, labels, lse, grad_losses, bias=None, i
 class ClassLoss(torch.autograd.Function):
     """Differentiable class loss: ``ClassLoss.apply(features, weight, bias, labels, ignore_index=-1, reduction="mean")``.
     ``reduction`` "none" gives the rows' losses, "sum" and "mean" one value, "mean" over the rows that are not ignored (0 if
-    there are none).  Gradients flow to features, weight and bias (which may be None); those nobody needs are not computed.  When forward and backward are
-    captured into a graph, capture both, on leaves whose eager graphs are gone."""
+    there are none).  Gradients flow to features, weight and bias (which may be None); those nobody needs are not computed.
+    When forward and backward are captured into a graph, capture both, on leaves whose eager graphs are gone."""
 
     @staticmethod
     def forward(ctx, features, weight, bias, labels, ignore_index=-1, reduction="mean"):
