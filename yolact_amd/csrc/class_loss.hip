@@ -383,10 +383,17 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
     }
   }
 }
-__global__ __launch_bounds__(128) void yp_scales_kernel(const float* part, float* scales) {   // a wave each
+// (a wave each, its loads all in flight: one after the other they took 10 us)
+__global__ __launch_bounds__(128) void yp_scales_kernel(const float* part, float* scales) {
   const int lane = (int)threadIdx.x & 63, j = (int)threadIdx.x >> 6;
+  yp_f4 v[YP_PEAK_BLOCKS / 256];
+#pragma unroll
+  for (int i = 0; i < YP_PEAK_BLOCKS / 256; ++i) v[i] = reinterpret_cast<const yp_f4*>(part + j * YP_PEAK_BLOCKS)[i * 64 + lane];
   float top = 0.0f;
-  for (int i = lane; i < YP_PEAK_BLOCKS; i += 64) top = fmaxf(top, part[j * YP_PEAK_BLOCKS + i]);
+#pragma unroll
+  for (int i = 0; i < YP_PEAK_BLOCKS / 256; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = fmaxf(top, v[i][e]);
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
   if (lane == 0) scales[j] = top > 0.0f ? ldexpf(1.0f, min(max(14 - ilogbf(top), -100), 100)) : 1.0f;
@@ -678,7 +685,7 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   p.o_w = take(copy_fwd ? p.fwd_piece * p.kd * planes : 0);
   p.o_part = take((int64_t)p.fwd_pieces * p.parts * N * sizeof(yp_softmax_part));
   p.o_picked = take(N * 4);
-  p.o_block = take((N <= 1024 ? (N + 1) / 2 : (N + 31) / 32) * 16);
+  p.o_block = take((N <= 1024 ? (N + 1) / 2 : N <= 4096 ? (N + 7) / 8 : (N + 31) / 32) * 16);
   p.fwd_total = off;
 
   off = both;
@@ -783,12 +790,15 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   yp_join_args j;
   j.part = part; j.parts = parts; j.picked = (const float*)(ws + p.o_picked); j.labels = labels;
   j.N = a.n; j.losses = a.losses; j.lse = a.lse; j.reduced = yp_reduced{a.sum, a.mean, a.counted}; j.block_part = (double*)(ws + p.o_block);
-  // few rows of many parts: 128 threads a row; else 8.  A few rows of few parts are one workgroup's, which sums their losses
+  // few rows of many parts: 128 threads a row, or 32; else 8.  A few rows of few parts are one workgroup's, which sums their losses
   // itself: a launch less.
   int blocks;
   if (a.n <= 1024 && parts > 64) {
     blocks = (a.n + 1) / 2;
     hipLaunchKernelGGL(yp_join_kernel<2>, dim3(blocks), dim3(YP_CL_THREADS), 0, st, j);
+  } else if (a.n <= 4096 && parts > 64) {
+    blocks = (a.n + 7) / 8;
+    hipLaunchKernelGGL(yp_join_kernel<8>, dim3(blocks), dim3(YP_CL_THREADS), 0, st, j);
   } else {
     blocks = a.n <= 256 ? 1 : (a.n + 31) / 32;
     hipLaunchKernelGGL(yp_join_kernel<32>, dim3(blocks), dim3(YP_CL_THREADS), 0, st, j);
