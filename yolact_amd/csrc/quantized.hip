@@ -160,8 +160,9 @@ hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x,
 
 // ---- one row: the weight is read once and that is all there is -----------------------------------------------------
 // A workgroup holds the row in LDS, quantized by itself - 8 KB from L2 cost less than another launch - and its waves walk
-// over rows of the weight, YP_OR_W at a time: a lane reads 16 bytes of k of each, multiplies with 4-wide dot products and
-// the wave adds up.  YP_OR_C chunks of each are on their way at a time - 16 KB a wave -, the first ones while x is
+// over rows of the weight, YP_OR_W at a time: a lane reads 16 bytes of k of each.  The matrix instruction takes lane l's 16
+// bytes as quarter l >> 4 of row and column l & 15, of the weight and of x alike: its diagonal holds the sums of four lanes'
+// products, which the wave adds up at the end.  YP_OR_C chunks of each are on their way at a time - 16 KB a wave -, the first ones while x is
 // quantized.  26.6 us for 32000 x 4096 (131 MB: 4.9 TB/s); from two rows on the matrix cores are faster (30 us, where this
 // took 43 for two and 100 for eight).
 #define YP_OR_W 4
@@ -169,7 +170,7 @@ hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x,
 #define YP_OR_LDS 61440
 
 template <int XTYPE, int OUT>
-__global__ __launch_bounds__(YP_QR_THREADS) void yp_one_row_kernel(const void* x, const float* x_scale, int v, int k, int kp, const char* wq, const float* w_scale,
+__global__ __launch_bounds__(YP_QR_THREADS, 4) void yp_one_row_kernel(const void* x, const float* x_scale, int v, int k, int kp, const char* wq, const float* w_scale,
                                                                    const float* bias, void* out, int vec) {
   typedef typename yp_type<OUT>::elem oelem;
   extern __shared__ __align__(16) char xl[];      // [kp]
@@ -209,24 +210,25 @@ __global__ __launch_bounds__(YP_QR_THREADS) void yp_one_row_kernel(const void* x
   }
   __syncthreads();
   for (; j0 < v; j0 += (int64_t)waves * YP_OR_W) {
-    int acc[YP_OR_W] = {0, 0, 0, 0};
+    yp_i4 acc[YP_OR_W];
+#pragma unroll
+    for (int u = 0; u < YP_OR_W; ++u) acc[u] = yp_i4{0, 0, 0, 0};
     for (int c0 = lane; c0 - lane < chunks; c0 += YP_OR_C * 64) {
       if (c0 != lane) get_w((int)j0, c0);
 #pragma unroll
       for (int c = 0; c < YP_OR_C; ++c) {
-        if (c0 + c * 64 < chunks) {
-          const yp_i4 xv = *reinterpret_cast<const yp_i4*>(xl + (c0 + c * 64) * 16);
+        if (c0 - lane + c * 64 < chunks) {              // (for the whole wave: a lane past the row has zeros)
+          const yp_i4 xv = *reinterpret_cast<const yp_i4*>(xl + min(c0 + c * 64, chunks - 1) * 16);
 #pragma unroll
-          for (int u = 0; u < YP_OR_W; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[u] = __builtin_amdgcn_sdot4(w[c][u][e], xv[e], acc[u], false);
+          for (int u = 0; u < YP_OR_W; ++u) acc[u] = yp_mma<YP_T_I8>(w[c][u], xv, acc[u]);
         }
       }
     }
     if (j0 + (int64_t)waves * YP_OR_W < v) get_w((int)j0 + waves * YP_OR_W, lane);
 #pragma unroll
     for (int u = 0; u < YP_OR_W; ++u) {
-      int t = acc[u];
+      const int r = (lane & 15) - (lane >> 4) * 4;      // C[i][i]: lane i + 16 (i / 4), register i % 4
+      int t = r == 0 ? acc[u][0] : r == 1 ? acc[u][1] : r == 2 ? acc[u][2] : r == 3 ? acc[u][3] : 0;
 #pragma unroll
       for (int s = 32; s > 0; s >>= 1) t += __shfl_xor(t, s);
       const int64_t j = j0 + u;
