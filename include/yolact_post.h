@@ -307,7 +307,8 @@ enum { YP_F32 = 0, YP_BF16 = 1, YP_F16 = 2, YP_INT8 = 3 };
  * grad (softmax - onehot) is rounded to dtype before its products, relative to the largest |grad| (f16: steps of at least
  * 2^-37 of it).  YP_F32 with n v d >= 2^31 multiplies each value as the sum of two f16 under one scale per tensor: off by at
  * most 2^-22 of itself or 2^-39 of the largest finite magnitude in its tensor's rows that take part, whichever is more (dz:
- * 2^-38 of the largest |grad|).  Fixed order of sums, no float atomics.
+ * 2^-38 of the largest |grad|).  Probabilities are exp(z - lse), so 2^-23 |lse| is their relative error where logits are
+ * large.  Fixed order of sums, no float atomics.
  * 0 <= n <= 2^20, 1 <= v <= 2^24, n v <= 2^38, 1 <= d <= 65536; contiguous tensors, aligned to their elements.  All pointers on the
  * device; asynchronous on hip_stream; allocates nothing, may be captured. */
 int64_t yp_class_loss_workspace(int32_t n, int32_t v, int32_t d, int32_t dtype, int32_t has_bias, int32_t backward);

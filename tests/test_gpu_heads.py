@@ -169,6 +169,29 @@ def test_class_loss_large_float32_beside_far_larger_values(far):
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(200, 333, 64), (2048, 8192, 130)])
+def test_class_loss_masks_of_the_lowest_value(n, v, d, dt):
+    """A bias of the type's lowest value masks as one of -inf does: its exponentials are zero.  Where it is every class's, and
+    beyond what lse can tell apart, results stay finite."""
+    from yolact_amd import heads
+    h, w, b, y, up = _loss_inputs(n, v, d, dt, True, 0.2)
+    y = torch.where((y >= 0) & (y % 5 == 0), (y + 1) % v, y)
+    out = []
+    for low in (-math.inf, torch.finfo(dt).min):
+        b[::5] = low
+        losses, lse = heads.class_loss(h, w, y, bias=b)
+        out.append((losses, lse, *heads.class_loss_backward(h, w, y, lse, up, bias=b)))
+    off = y % 5 == 0                                          # (the wrap round v may have put a label on a masked class)
+    assert not bool(off[y >= 0].any())
+    for a, c, name in zip(*out, ("losses", "lse", "grad_features", "grad_weight", "grad_bias")):
+        assert torch.equal(a, c), name
+    b[:] = torch.finfo(dt).min
+    losses, lse = heads.class_loss(h, w, y, bias=b)
+    for t in (losses, lse, *heads.class_loss_backward(h, w, y, lse, up, bias=b)):
+        assert torch.isfinite(t).all()
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
 def test_class_loss_labels_that_cannot_be(dt):
     """A masked class as label: +inf.  A label outside the vocabulary: NaN, no gradient, nothing else touched."""
     h, w, b, y, up = _loss_inputs(50, 40, 32, dt, True, 0.2)

@@ -56,7 +56,7 @@ struct yp_gemm {
 // SEGS > 1: operands as the sum of two planes of their type, and the products of planes one after the other along a k
 // axis SEGS times as long:
 //   2  B has two planes: twice its precision
-//   3  f32 operands, scaled by a power of two, as two f16 planes each (22 bits, to 2^-40 of the largest element); of the
+//   3  f32 operands, scaled by a power of two, as two f16 planes each (22 bits, to 2^-39 of the largest element); of the
 //      four products of planes the three whose terms are not below 2^-24 of the result.  The f16 matrix instructions are
 //      16 times as fast as the f32 ones: three of them for one.  Sums are f32 as ever.
 #define YP_SEGMENT_A(s) ((s) == 2)
