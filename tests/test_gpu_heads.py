@@ -192,6 +192,34 @@ def test_class_loss_masks_of_the_lowest_value(n, v, d, dt):
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n,v,d", [(200, 333, 64), (2048, 8192, 130)])
+def test_class_loss_one_class_of_the_highest_value(n, v, d, dt):
+    """It has all of the probability: its rows have loss 0, the others pull from it to their label.  The sum of exponentials
+    and a probability exp(z - lse) take log2 e times the largest logit, or lse, rounded: factors of 1 +- 2^-24 |lse| each,
+    lse's own rounding another.  f16's 65504 is small enough for that to show, as 2^-7 of g and 2^-7 in the loss; the other
+    types' 3.4e38 is not: there the sum is 1, and p, which would be above 1 or 0, the one or the other."""
+    from_p = 2.0 ** -7 if dt == torch.float16 else 0.0
+    from yolact_amd import heads
+    h, w, b, y, up = _loss_inputs(n, v, d, dt, True, 0.2)
+    b[7] = torch.finfo(dt).max
+    h /= 4 if dt == torch.float16 else 1                      # (the sum with the bias stays finite in float32 in any case)
+    y[::3] = 7
+    losses, lse = heads.class_loss(h, w, y, bias=b)
+    gh, gw, gb = heads.class_loss_backward(h, w, y, lse, up, bias=b)
+    assert bool((losses[y == 7].abs() <= from_p).all()) and (from_p or not gh[y == 7].any())
+    rest = (y >= 0) & (y != 7)
+    assert torch.isfinite(losses).all() and bool((losses[rest] > 6e4).all())
+    onehot = torch.zeros(n, v, dtype=torch.float64, device="cuda")
+    onehot[rest, y[rest]] = -1.0
+    onehot[rest, 7] = 1.0
+    dz = onehot * up.double()[:, None]
+    most = dz.abs()
+    most[y >= 0, 7] = up.double()[y >= 0]                     # (where p enters)
+    for got, want, size in ((gh, dz @ w.double(), most @ w.double().abs()), (gw, dz.t() @ h.double(), most.t() @ h.double().abs()), (gb, dz.sum(0), most.sum(0))):
+        ref.within(got, want, (from_p + 4 * ref.HALF[dt] + (n + 8) * ref.F) * size + 2.0 ** -24, "gradient")
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
 def test_class_loss_labels_that_cannot_be(dt):
     """A masked class as label: +inf.  A label outside the vocabulary: NaN, no gradient, nothing else touched."""
     h, w, b, y, up = _loss_inputs(50, 40, 32, dt, True, 0.2)

@@ -192,7 +192,7 @@ struct yp_epi_dz {
       // exp(z - lse) = 2^min(z log2e + c, 0) - rounding may bring z above lse, by any amount where large products cancel -; a
       // row that takes no part, or has no class left: 2^-inf = 0; one with NaN among its z has it in lse, and here in gr
       const float gr = label < 0 ? 0.0f : l != l ? l : grad ? grad[j] * by : by;
-      const float c = l == -INFINITY ? -INFINITY : fminf(-l * YP_LOG2E, 0x1.fffffep127f);
+      const float c = fabsf(l) == INFINITY ? -INFINITY : __builtin_amdgcn_fmed3f(-l * YP_LOG2E, -0x1.fffffep127f, 0x1.fffffep127f);
       const int hit = label < 0 ? -1 : label - first - ib;
       if (__builtin_amdgcn_ballot_w64(hit >= 0 && hit < S::BM)) {      // (mostly no lane of the wave)
 #pragma unroll
