@@ -303,8 +303,8 @@ enum { YP_F32 = 0, YP_BF16 = 1, YP_F16 = 2, YP_INT8 = 3 };
  *   workspace    yp_class_loss_workspace(n, v, d, dtype, has_bias, backward) bytes, 256-byte aligned
  * The backward pass takes the forward's inputs and its lse, and grad = dL/dlosses: [n] float32 (grad_stride 1) or one
  * value for every row (grad_stride 0); with count != NULL the values are divided by max(*count, 1) (the mean: pass the
- * forward's count).  Gradients that are NULL are not computed.  Products accumulate in float32, gradients are rounded once; dz =
- * grad (softmax - onehot) is rounded to dtype before its products, relative to the largest |grad| (f16: steps of at least
+ * forward's count).  Gradients that are NULL are not computed (one at least is wanted, unless n is 0).  Products
+ * accumulate in float32, gradients are rounded once; dz = grad (softmax - onehot) is rounded to dtype before its products, relative to the largest |grad| (f16: steps of at least
  * 2^-37 of it).  YP_F32 with n v d >= 2^31 multiplies each value as the sum of two f16 under one scale per tensor: off by at
  * most 2^-22 of itself or 2^-39 of the largest finite magnitude in its tensor's rows that take part, whichever is more (dz:
  * 2^-38 of the largest |grad|).  Probabilities are exp(z - lse), so 2^-23 |lse| is their relative error where logits are

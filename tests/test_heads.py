@@ -90,6 +90,13 @@ def test_class_loss_backward_refuses(change, needle):
                                                 a["count"], a["ws"], a["gh"], a["gw"], a["gb"], None), needle)
 
 
+def test_class_loss_backward_of_no_rows_needs_no_gradient_pointer():
+    """The gradient of features that have no row is an empty tensor, whose address is null."""
+    L = _lib.load()
+    for bias in (None, P):
+        assert L.yp_class_loss_backward(0, 0, 9, 8, 0, None, P, bias, None, 8, -1, None, None, 1, None, None, None, None, None, None) == 0
+
+
 @pytest.mark.parametrize("change,needle", [
     (dict(rows=-1), "rows"), (dict(k=0), "k must"), (dict(k=131073), "k must"), (dict(dtype=4), "dtype"), (dict(out_dtype=3), "out_dtype"),
     (dict(v=0), "v must"), (dict(x=None), "null"), (dict(ws=None), "null"), (dict(dtype=3), "null"), (dict(out=None), "null"),

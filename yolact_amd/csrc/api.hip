@@ -797,11 +797,12 @@ extern "C" int yp_class_loss_backward(int32_t device_id, int32_t n, int32_t v, i
   const int rc = check_class_loss("yp_class_loss_backward", a);
   if (rc != YP_OK) return rc;
   if (grad_stride != 0 && grad_stride != 1) return fail(YP_EINVAL, "yp_class_loss_backward: grad_stride must be 0 or 1");
-  if ((n > 0 && !grad) || (!grad_features && !grad_weight && !grad_bias)) return fail(YP_EINVAL, "yp_class_loss_backward: null argument");
+  if (n > 0 && (!grad || (!grad_features && !grad_weight && !grad_bias))) return fail(YP_EINVAL, "yp_class_loss_backward: null argument");
   if (grad_bias && !bias) return fail(YP_EINVAL, "yp_class_loss_backward: grad_bias without bias");
   if (!elem_aligned(grad_features, dtype) || !elem_aligned(grad_weight, dtype) || !elem_aligned(grad_bias, dtype) ||
       (((uintptr_t)grad | (uintptr_t)count) & 3) != 0)
     return fail(YP_EINVAL, "yp_class_loss_backward: a tensor is not aligned to its elements");
+  if (n == 0 && !grad_weight && !grad_bias) return YP_OK;   // (the features' gradient has no element, and so no address)
   YP_ON_DEVICE(device_id);
   YP_HIP(yp_launch_class_loss_backward(a, (hipStream_t)hip_stream));
   return YP_OK;
