@@ -37,3 +37,21 @@ def test_no_rows_and_one_gradient_wanted(dt, reduction):
         loss = heads.ClassLoss.apply(*leaves, y, -1, reduction)
         grad, = torch.autograd.grad(loss.sum(), [leaves[which]])
         assert grad.shape == leaves[which].shape and not grad.any()
+
+
+@pytest.mark.parametrize("dt,n,v,d,bias", [(t, 300, 333, 64, True) for t in TYPES] + [(t, 2048, 8192, 130, bias) for t in TYPES for bias in (True, False)])
+def test_lse_of_every_row(dt, n, v, d, bias):
+    """lse is the logits' own, whatever the label: of ignored rows, of rows whose label is outside the vocabulary, and of rows
+    2^40 apart in magnitude (f16: 2^8).  A NaN stays in its row."""
+    from yolact_amd import heads
+    h, w, b, y, _ = _inputs(n, v, d, dt, bias)
+    span = 4 if dt == torch.float16 else 20
+    h *= torch.exp2(torch.randint(-span, span + 1, (n, 1), generator=_gen(1), device="cuda").float()).to(dt)
+    y[::3], y[1::7], y[2::7] = -1, v, -7
+    want = ref.class_loss(h, w, b, torch.zeros_like(y), None)["lse"]
+    losses, lse = heads.class_loss(h, w, y, bias=b)
+    ref.within(lse, *want, "lse")
+    ref.within(losses, *ref.class_loss(h, w, b, y, None)["losses"], "losses")
+    h[0, 3] = math.nan
+    again = heads.class_loss(h, w, y, bias=b)[1]
+    assert again[0].isnan() and torch.equal(again[1:], lse[1:])

@@ -20,7 +20,9 @@
 // kept.  Where rows are few, their roundings do not average out, and dz has two planes (twice the precision).
 // f32 of any size worth it runs on the f16 matrix instructions, as two f16 planes per operand (SPLIT; gemm_tile.hpp): 22 bits
 // of a value, or 2^-39 of the largest one where that is more - a value below 2^-17 of the largest has fewer bits than f32,
-// its share of a sum over both is as good.
+// its share of a sum over both is as good.  In z, whose sums run along the rows, the largest is the row's own, of h and of w
+// alike: each row has an exponent of its own, which its results get back, so no row's logits depend on another row, ignored
+// or not.  The gradient products add up over the rows of h, and of w: those have one scale each, another two planes.
 // What takes no part has dz = 0, but 0 times NaN is NaN: the gradient products read a copy of h in which ignored rows are
 // zero (and of w, if a bias may mask classes).
 // All sums are f32 in a fixed order: no float atomics, the same call gives the same bits.
@@ -58,6 +60,27 @@ __device__ __forceinline__ float yp_plane_rest(float x) {
   return fabsf(h) < INFINITY ? x - h : 0.0f;
 }
 
+// Of the two planes' rows: a row of f32 whose largest finite magnitude lies in [2^(e-1), 2^e) is held times 2^(15-e), e = 0 for
+// one of zeros.  (The integer exponents undo it: products of two float scales would leave f32's range.)
+struct yp_row_exponents {
+  const int *i, *j;            // [V], of the piece, and [N]; both padded to 256, which is as far as a tile reaches
+  template <int SHAPE, int MI, int NJ, class Acc>
+  __device__ __forceinline__ void give_back(Acc (&acc)[MI][NJ], int ib, int jb) const {
+    typedef yp_shape<SHAPE> S;
+    int ej[NJ];
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) ej[n] = j[jb + yp_frag_at<S::BN, NJ>(n)] - 30;
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      const yp_i4 ei = *reinterpret_cast<const yp_i4*>(i + ib + yp_frag_at<S::BM, MI>(m));
+#pragma unroll
+      for (int n = 0; n < NJ; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[m][n][r] = __builtin_amdgcn_ldexpf(acc[m][n][r], ei[r] + ej[n]);
+    }
+  }
+};
+
 struct yp_labels {
   const void* labels;
   int bytes;
@@ -79,19 +102,13 @@ struct yp_epi_stats {
   int first;                   // first class of the piece
   yp_softmax_part* part;       // [tiles_i * WI][N] of the piece
   float* picked;               // [N] z of the label
-  yp_scale zscale;             // SPLIT
+  yp_row_exponents exponents;  // SPLIT
   template <int TYPE, int SHAPE, int MI, int NJ, class Acc>
   __device__ __forceinline__ void apply(const yp_gemm& g, Acc (&acc)[MI][NJ], const yp_place& at) const {
     typedef yp_shape<SHAPE> S;
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
-    if constexpr (SPLIT) {
-      const float zs = zscale.get();
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NJ; ++n) acc[m][n] = acc[m][n] * zs;
-    }
+    if constexpr (SPLIT) exponents.give_back<SHAPE>(acc, ib, jb);
     if (bias || (at.ti + 1) * S::BM > g.I) {
 #pragma unroll
       for (int m = 0; m < MI; ++m)
@@ -152,7 +169,7 @@ struct yp_epi_dz {
   const float* factor;
   float up;
   yp_scale scale;              // what the bias gradient gets back
-  yp_scale zscale;             // SPLIT
+  yp_row_exponents exponents;  // SPLIT
   int first;                   // first class of the piece
   void* dz;                    // [kn][kv], zero in [N, kn) and [V, kv); or PLANES of it
   int64_t plane;               // bytes of one
@@ -166,13 +183,7 @@ struct yp_epi_dz {
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
     const float by = grad && factor ? *factor : up;
-    if constexpr (SPLIT) {
-      const float zs = zscale.get();
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NJ; ++n) acc[m][n] = acc[m][n] * zs;
-    }
+    if constexpr (SPLIT) exponents.give_back<SHAPE>(acc, ib, jb);
     if (bias || (at.ti + 1) * S::BM > g.I) {      // a class that takes no part, or does not exist: z = -inf
 #pragma unroll
       for (int m = 0; m < MI; ++m)
@@ -260,7 +271,9 @@ struct yp_copy_job {
   int vec;                // rows of src are multiples of 16 bytes and so is their address
   int by_label;
   const void* bias;
-  int64_t plane;          // 0, or: f32 rows times *scale to two f16 planes, this many bytes apart (row_bytes, kb: of a plane's row)
+  int64_t plane;          // 0, or: f32 rows to two f16 planes, this many bytes apart (row_bytes, kb: of a plane's row),
+  const int* exponent;    //   each held by its own exponent (yp_row_exponents)
+  char* common;           //   and, unless null, to two more, times *scale: for products that add up over the rows
   const float* scale;
 };
 struct yp_copy_args {
@@ -282,7 +295,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
     if (in && j.by_label) in = a.labels.counted(r) >= 0;
     if (in && j.bias) in = yp_load_as_float(j.bias, r, a.type) != -INFINITY;
     if (j.plane) {        // 8 elements
-      const float sc = *j.scale;
+      const int up = in ? 15 - j.exponent[r] : 0;
       float x[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) x[u] = 0.0f;
@@ -297,14 +310,22 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
           for (int u = 0; u < 8; ++u) if (at + 2 * u < j.row_bytes) x[u] = reinterpret_cast<const float*>(s)[u];
         }
       }
+      auto put = [&](char* dst, auto val) {
+        float y[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] *= sc;
+        for (int u = 0; u < 8; ++u) y[u] = val(x[u]);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        yp_h8 o;
+        for (int q = 0; q < 2; ++q) {
+          yp_h8 o;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) { o[u] = (_Float16)x[u]; x[u] = yp_plane_rest<_Float16>(x[u]); }
-        *reinterpret_cast<yp_h8*>(j.dst + q * j.plane + r * j.kb + at) = o;
+          for (int u = 0; u < 8; ++u) { o[u] = (_Float16)y[u]; y[u] = yp_plane_rest<_Float16>(y[u]); }
+          *reinterpret_cast<yp_h8*>(dst + q * j.plane + r * j.kb + at) = o;
+        }
+      };
+      put(j.dst, [&](float v) { return __builtin_amdgcn_ldexpf(v, up); });
+      if (j.common) {
+        const float sc = *j.scale;
+        put(j.common, [&](float v) { return v * sc; });
       }
       continue;
     }
@@ -325,15 +346,17 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
   }
 }
 
-// The largest finite magnitudes of features and weight among the rows that take part - a wave a row -, a part per workgroup;
-// and the powers of two that bring them to [2^14, 2^15), scales[0] and [1].
+// The exponents of all rows of features and weight (yp_row_exponents), a wave a row; and, unless `part` is null, the largest finite
+// magnitudes of either among the rows that take part, a part per workgroup, for the powers of two that bring them to
+// [2^14, 2^15), scales[0] and [1].
 struct yp_peak_args {
   const float* src[2];
   int64_t rows[2];
   int d, vec;
   yp_labels labels;            // of the first
   const float* bias;           // of the second, may be null
-  float* part;                 // [2][YP_PEAK_BLOCKS]
+  int* exponent[2];
+  float* part;                 // [2][YP_PEAK_BLOCKS], may be null
 };
 #define YP_PEAK_BLOCKS 2048
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_args a) {
@@ -341,11 +364,11 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    float top = 0.0f;
-    auto see = [&](float v) { v = fabsf(v); top = fmaxf(top, v < INFINITY ? v : 0.0f); };
+    float most = 0.0f;
     for (int64_t r = (int64_t)blockIdx.x * (YP_CL_THREADS / 64) + wave; r < a.rows[j]; r += YP_PEAK_BLOCKS * (YP_CL_THREADS / 64)) {
-      if (j == 0 ? a.labels.counted(r) < 0 : a.bias && a.bias[r] == -INFINITY) continue;
       const float* const p = a.src[j] + r * a.d;
+      float top = 0.0f;
+      auto see = [&](float v) { v = fabsf(v); top = fmaxf(top, v < INFINITY ? v : 0.0f); };
       int c = lane * 4;
       if (a.vec) {
         for (; c + 768 < a.d; c += 1024) {      // four loads in flight
@@ -372,15 +395,18 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
         }
         for (; c < a.d; c += 64) see(p[c]);
       }
-    }
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+      for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+      if (lane == 0) a.exponent[j][r] = __builtin_amdgcn_frexp_expf(top);      // (0 of 0)
+      if (a.part && (j == 0 ? a.labels.counted(r) >= 0 : !a.bias || a.bias[r] != -INFINITY)) most = fmaxf(most, top);
+    }
+    if (!a.part) continue;
     __syncthreads();
-    if (lane == 0) red[wave] = top;
+    if (lane == 0) red[wave] = most;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < YP_CL_THREADS / 64; ++w) top = fmaxf(top, red[w]);
-      a.part[j * YP_PEAK_BLOCKS + blockIdx.x] = top;
+      for (int w = 1; w < YP_CL_THREADS / 64; ++w) most = fmaxf(most, red[w]);
+      a.part[j * YP_PEAK_BLOCKS + blockIdx.x] = most;
     }
   }
 }
@@ -646,9 +672,10 @@ struct ClassLossPlan {
   int64_t kn, kv;              // rows of dz padded to a step, elements; bytes of a row
   yp_tile_plan dzp, dwp, dhp;
   // workspace offsets
-  int64_t o_scales, o_peaks;   // both passes
+  int64_t o_eh, o_ew;          // both passes
+  int64_t o_scales, o_peaks;   // backward
   int64_t o_h, o_w, o_part, o_picked, o_block, fwd_total;
-  int64_t o_factor, o_hc, o_wc, o_dz, o_bp, o_dwpart, o_dhpart, bwd_total;
+  int64_t o_factor, o_hc, o_wc, o_hs, o_ws, o_dz, o_bp, o_dwpart, o_dhpart, bwd_total;
 };
 
 static void cut_pieces(int64_t V, int64_t most, int* pieces, int* piece) {   // equal pieces, multiples of 256
@@ -673,8 +700,8 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   p.kd = yp_pad_k(D, b);
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = up256(off + bytes); return o; };
-  p.o_scales = take(p.split ? 8 : 0);
-  p.o_peaks = take(p.split ? 2 * YP_PEAK_BLOCKS * 4 : 0);
+  p.o_eh = take(p.split ? up256(N) * 4 : 0);
+  p.o_ew = take(p.split ? up256(V) * 4 : 0);
   const int64_t both = off;
   if (copy_fwd) cut_pieces(V, YP_CL_PIECE_BYTES / (p.kd * planes), &p.fwd_pieces, &p.fwd_piece);
   else { p.fwd_pieces = 1; p.fwd_piece = (int)V; }
@@ -700,9 +727,13 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   p.dzp = p.split ? yp_plan_shape(YP_TILE_M, p.piece, p.kn) : yp_plan_tiles(p.piece, p.kn, dsteps, largest);
   // the two gradient products share a launch and so a tile shape
   yp_plan_two(D, p.piece, p.kn / kr * p.segs, D, N, p.kv / YP_TILE_KB * p.segs, largest, &p.dwp, &p.dhp);
+  p.o_scales = take(p.split ? 8 : 0);
+  p.o_peaks = take(p.split ? 2 * YP_PEAK_BLOCKS * 4 : 0);
   p.o_factor = take(8);
   p.o_hc = take(p.kn * p.kd * planes);
   p.o_wc = take(p.piece * p.kd * planes);
+  p.o_hs = take(p.split ? p.kn * p.kd * planes : 0);
+  p.o_ws = take(p.split ? p.piece * p.kd * planes : 0);
   p.o_dz = take(p.kn * p.kv * p.dzplanes);
   p.o_bp = take(has_bias && p.dzp.tiles_j > 1 ? (int64_t)p.dzp.tiles_j * p.piece * 4 : 0);
   p.o_dwpart = take(p.dwp.splits > 1 ? (int64_t)p.dwp.splits * p.piece * D * 4 : 0);
@@ -728,15 +759,16 @@ static yp_copy_job copy_job(const void* src, char* dst, int64_t d, const ClassLo
   j.vec = row_bytes % 16 == 0 && ((uintptr_t)src & 15) == 0;
   return j;
 }
-// scales[0], [1]: of the features and of the weight
-static hipError_t find_scales(const yp_class_loss_args& a, const yp_labels& labels, char* ws, const ClassLossPlan& p, hipStream_t st) {
+// the rows' exponents; and scales[0], [1], of the features and of the weight, for the backward pass
+static hipError_t find_scales(const yp_class_loss_args& a, const yp_labels& labels, char* ws, const ClassLossPlan& p, bool backward, hipStream_t st) {
   yp_peak_args k;
   k.src[0] = (const float*)a.features; k.src[1] = (const float*)a.weight;
   k.rows[0] = a.n; k.rows[1] = a.v; k.d = a.d;
   k.vec = a.d % 4 == 0 && (((uintptr_t)a.features | (uintptr_t)a.weight) & 15) == 0;
-  k.labels = labels; k.bias = (const float*)a.bias; k.part = (float*)(ws + p.o_peaks);
+  k.labels = labels; k.bias = (const float*)a.bias; k.part = backward ? (float*)(ws + p.o_peaks) : nullptr;
+  k.exponent[0] = (int*)(ws + p.o_eh); k.exponent[1] = (int*)(ws + p.o_ew);
   hipLaunchKernelGGL(yp_peak_kernel, dim3(YP_PEAK_BLOCKS), dim3(YP_CL_THREADS), 0, st, k);
-  hipLaunchKernelGGL(yp_scales_kernel, dim3(1), dim3(128), 0, st, (const float*)k.part, (float*)(ws + p.o_scales));
+  if (backward) hipLaunchKernelGGL(yp_scales_kernel, dim3(1), dim3(128), 0, st, (const float*)k.part, (float*)(ws + p.o_scales));
   return hipGetLastError();
 }
 static hipError_t copy_rows(yp_copy_args a, hipStream_t st) {
@@ -755,8 +787,8 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   const ClassLossPlan p = plan_class_loss(a.n, a.v, a.d, ELEM, a.bias != nullptr, copy);
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
-  float* const scales = SPLIT ? (float*)(ws + p.o_scales) : nullptr;
-  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, st));
+  const int *const eh = (const int*)(ws + p.o_eh), *const ew = (const int*)(ws + p.o_ew);     // SPLIT
+  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, false, st));
   yp_softmax_part* const part = (yp_softmax_part*)(ws + p.o_part);
   int parts = 0;
   for (int s = 0; s < p.fwd_pieces; ++s) {
@@ -769,10 +801,7 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
       c.job[0] = copy_job(g.a + v0 * row, ws + p.o_w, a.d, p, nv, nv);
       if (s == 0) c.job[1] = copy_job(g.b, ws + p.o_h, a.d, p, a.n, a.n);
       c.labels = labels;
-      if (SPLIT) {       // (a row that takes no part may hold anything, beyond f16 too)
-        c.job[0].scale = scales + 1; c.job[0].bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
-        c.job[1].scale = scales; c.job[1].by_label = 1;
-      }
+      if (SPLIT) { c.job[0].exponent = ew + v0; c.job[1].exponent = eh; }
       g.aplane = nv * p.kd; g.bplane = a.n * p.kd;
       CL_TRY(copy_rows(c, st));
       g.a = ws + p.o_w; g.b = ws + p.o_h;
@@ -782,7 +811,7 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
     yp_tile_plan tp = p.fwd;
     tp.tiles_i = (nv + tp.bi - 1) / tp.bi;
     yp_epi_stats<ELEM, SPLIT> e;
-    e.zscale = yp_scale{nullptr, nullptr, 1.0f, {scales, SPLIT ? scales + 1 : nullptr}};
+    e.exponents = yp_row_exponents{ew + v0, eh};
     e.bias = a.bias ? (const char*)a.bias + (int64_t)v0 * b : nullptr;
     e.labels = labels; e.first = v0; e.part = part + (int64_t)parts * a.n; e.picked = (float*)(ws + p.o_picked);
     CL_TRY(yp_launch_gemm<TYPE, SPLIT ? 3 : 1>(tp, g, e, st));
@@ -816,8 +845,9 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   const bool copy_w = SPLIT || a.bias || row % YP_TILE_KB != 0 || ((uintptr_t)a.weight & 15) != 0;
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
+  const int *const re_h = (const int*)(ws + p.o_eh), *const re_w = (const int*)(ws + p.o_ew);   // SPLIT
   float* const scales = SPLIT ? (float*)(ws + p.o_scales) : nullptr;
-  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, st));
+  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, true, st));
   const float up = TYPE == YP_T_F16 ? 8192.0f : 1.0f;
   float* factor = nullptr;
   yp_scale back = {a.grad, a.count, 1.0f / up, {}};         // one g for all rows
@@ -845,8 +875,19 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
       c.type = ELEM;
       c.labels = labels;
       int n = 0;
-      if (s == 0) { c.job[n] = copy_job(a.features, ws + p.o_hc, a.d, p, a.n, p.kn); c.job[n].scale = scales; c.job[n++].by_label = 1; }
-      if (copy_w) { c.job[n] = copy_job(w, ws + p.o_wc, a.d, p, nv, nv); c.job[n].scale = scales ? scales + 1 : nullptr; c.job[n++].bias = bias; w = ws + p.o_wc; }
+      if (s == 0) {
+        yp_copy_job& j = c.job[n++];
+        j = copy_job(a.features, ws + p.o_hc, a.d, p, a.n, p.kn);
+        j.by_label = 1;
+        if (SPLIT) { j.exponent = re_h; j.common = ws + p.o_hs; j.scale = scales; }
+      }
+      if (copy_w) {
+        yp_copy_job& j = c.job[n++];
+        j = copy_job(w, ws + p.o_wc, a.d, p, nv, nv);
+        j.bias = bias;
+        if (SPLIT) { j.exponent = re_w + v0; j.common = ws + p.o_ws; j.scale = scales + 1; }
+        w = ws + p.o_wc;
+      }
       CL_TRY(copy_rows(c, st));
     }
     const int kv = (int)(yp_pad_k(nv, tb) / tb);
@@ -858,7 +899,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     g.I = nv; g.J = a.n; g.steps = (int)(p.kd / YP_TILE_KB);
     yp_epi_dz<ELEM, SPLIT, PLANES> e;
     e.plane = dzplane;
-    e.zscale = yp_scale{nullptr, nullptr, 1.0f, {scales, SPLIT ? scales + 1 : nullptr}};
+    e.exponents = yp_row_exponents{re_w + v0, re_h};
     e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = up; e.scale = back;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
     e.bias_out = a.grad_bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
@@ -868,7 +909,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     CL_TRY(yp_launch_gemm<TYPE, SPLIT ? 3 : 1>(tp, g, e, st));
     // dw[v][d] = sum_n dz[n][v] h[n][d]
     yp_gemm gw = {};
-    gw.a = ws + p.o_hc; gw.lda = p.kd; gw.I = a.d; gw.aplane = hplane; gw.bplane = dzplane;
+    gw.a = ws + (SPLIT ? p.o_hs : p.o_hc); gw.lda = p.kd; gw.I = a.d; gw.aplane = hplane; gw.bplane = dzplane;
     gw.b = ws + p.o_dz; gw.ldb = (int64_t)kv * tb; gw.J = nv;
     gw.K = (int)p.kn; gw.steps = (int)(p.kn * tb / YP_TILE_KB);
     char* const gwo = a.grad_weight ? (char*)a.grad_weight + v0 * row : nullptr;
@@ -881,7 +922,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     twp.tiles_j = (nv + twp.bj - 1) / twp.bj;
     // dh[n][d] (+)= sum_v dz[n][v] w[v][d]
     yp_gemm gh = {};
-    gh.a = w; gh.lda = copy_w ? p.kd : row; gh.I = a.d; gh.aplane = wplane; gh.bplane = dzplane;
+    gh.a = SPLIT ? ws + p.o_ws : w; gh.lda = copy_w ? p.kd : row; gh.I = a.d; gh.aplane = wplane; gh.bplane = dzplane;
     gh.b = ws + p.o_dz; gh.ldb = (int64_t)kv * tb; gh.J = a.n;
     gh.K = nv; gh.steps = (int)((int64_t)kv * tb / YP_TILE_KB);
     yp_epi_store<ELEM> eh = {};

@@ -92,8 +92,8 @@ def class_loss(features, weight, labels, bias=None, ignore_index: int = -1):
     int32), with ``lse = log sum exp`` of the logits and ``losses = lse - logit[label]``.
 
     A row labelled ``ignore_index`` takes no part (loss 0) whatever its features hold; any other label outside [0, V) has
-    loss NaN.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf.
-    Large float32 calls (2^31 multiplications and more) take each value to 2^-22 of itself or 2^-39 of the largest in its tensor.
+    loss NaN.  ``lse`` is the logits' own in these rows too.  A class whose bias is -inf takes no part, whatever its weights hold; as a label its loss is +inf.
+    Large float32 calls (2^31 multiplications and more) take each value to 2^-22 of itself or 2^-39 of the largest in its row.
     No gradient is recorded here: ``ClassLoss`` is the differentiable form."""
     args = _class_loss_args(features, weight, labels, bias)
     lead, dev = args[-2:]
