@@ -55,3 +55,65 @@ def test_lse_of_every_row(dt, n, v, d, bias):
     h[0, 3] = math.nan
     again = heads.class_loss(h, w, y, bias=b)[1]
     assert again[0].isnan() and torch.equal(again[1:], lse[1:])
+
+
+def _large_float32_bounds(h, w, b, y, up):
+    """What large float32 calls are allowed beyond the reference's bounds.  Logits: each value is off by 2^-22 of itself - three
+    such errors a product, 12 F, are within the reference's (D + 2) F - or by 2^-39 of its row's largest, which is less than that
+    beside the row's largest product.  Gradients: the softmax's difference d by 2^-22 of itself or 2^-38 (half a step
+    of f16's subnormals, of d times 2^13), the weight by 2^-39 of the largest, gradient times features by 2^-39 of theirs."""
+    want = ref.class_loss(h, w, b, y, up)
+    kept = (y >= 0) & (y < w.shape[0])
+    hk = torch.where(kept[:, None], h, 0 * h).double().nan_to_num(0.0)
+    gh = hk * torch.where(kept, up, 0 * up).double()[:, None]
+    g = torch.where(kept, up, 0 * up).double().abs()
+    wd = w.double()
+    z = hk @ wd.t() + (b.double() if b is not None else 0.0)
+    dd = torch.exp(z - torch.logsumexp(z, dim=1, keepdim=True))
+    dd[torch.arange(len(y), device="cuda")[kept], y[kept]] -= 1.0
+    dd = dd.abs() * kept[:, None]
+    off = 2.0 ** -38 * kept[:, None] + 0 * dd
+    more_h = g[:, None] * (off @ wd.abs() + dd.sum(dim=1, keepdim=True) * wd.abs().max() * 2.0 ** -39)
+    more_w = off.t() @ gh.abs() + dd.t().sum(dim=1, keepdim=True) * gh.abs().max() * 2.0 ** -39
+    want["grad_h"] = (want["grad_h"][0], want["grad_h"][1] + 1.01 * more_h)
+    want["grad_w"] = (want["grad_w"][0], want["grad_w"][1] + 1.01 * more_w)
+    return want
+
+
+def _check_large_float32(h, w, b, y, up, wild=()):
+    """wild: rows whose own results are not finite; if one of them takes part, neither is the weight's gradient."""
+    from yolact_amd import heads
+    losses, lse = heads.class_loss(h, w, y, bias=b)
+    grads = heads.class_loss_backward(h, w, y, lse, up, bias=b)
+    rest = torch.ones_like(y, dtype=torch.bool)
+    rest[list(wild)] = False
+    tame = h.clone()
+    tame[~rest] = 0.0
+    want = _large_float32_bounds(tame, w, b, y, up)
+    for got, name in ((losses, "losses"), (lse, "lse"), (grads[0], "grad_h")):
+        ref.within(got[rest], want[name][0][rest], want[name][1][rest], name)
+    if all(int(y[i]) < 0 for i in wild):
+        for got, name in zip(grads[1:], ("grad_w", "grad_b") if b is not None else ("grad_w",)):
+            ref.within(got, *want[name], name)
+
+
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("row,features,weight", [(1.0, 2.0 ** 112, 2.0 ** -112), (1.0, 2.0 ** 118, 2.0 ** -119),
+                                                 (2.0 ** -100, 2.0 ** -110, 2.0 ** 112), (1.0, 1.0, 2.0 ** -125)])
+def test_large_float32_values_at_the_ends_of_the_type(row, features, weight, bias):
+    """Values of 2^116 and more, and tensors whose largest value is 2^-110 and less, with logits of ordinary size."""
+    h, w, b, y, up = _inputs(2048, 8192, 130, torch.float32, bias)
+    h, w = h * features, w * weight
+    h[5] *= row
+    _check_large_float32(h, w, b, y, up * 2048)
+
+
+def test_large_float32_rows_of_zeros_beside_very_large_ones():
+    """One row of 2^100 against a class of 2^60: its logit is infinite.  Rows of zeros have the bias as logits."""
+    h, w, b, y, up = _inputs(2048, 8192, 130, torch.float32, True)
+    h[0] *= 2.0 ** 100
+    h[1:9] = 0.0
+    w[3] *= 2.0 ** 60
+    _check_large_float32(h, w, b, y, up, wild=(0,))
+    y[0] = -1
+    _check_large_float32(h, w, b, y, up, wild=(0,))

@@ -273,8 +273,8 @@ struct yp_copy_job {
   const void* bias;
   int64_t plane;          // 0, or: f32 rows to two f16 planes, this many bytes apart (row_bytes, kb: of a plane's row),
   const int* exponent;    //   each held by its own exponent (yp_row_exponents)
-  char* common;           //   and, unless null, to two more, times *scale: for products that add up over the rows
-  const float* scale;
+  char* common;           //   and, unless null, to two more, times 2^-*back: for products that add up over the rows
+  const int* back;
 };
 struct yp_copy_args {
   yp_copy_job job[2];
@@ -324,8 +324,8 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
       };
       put(j.dst, [&](float v) { return __builtin_amdgcn_ldexpf(v, up); });
       if (j.common) {
-        const float sc = *j.scale;
-        put(j.common, [&](float v) { return v * sc; });
+        const int all = -*j.back;
+        put(j.common, [&](float v) { return __builtin_amdgcn_ldexpf(v, all); });
       }
       continue;
     }
@@ -346,9 +346,10 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
   }
 }
 
-// The exponents of all rows of features and weight (yp_row_exponents), a wave a row; and, unless `part` is null, the largest finite
-// magnitudes of either among the rows that take part, a part per workgroup, for the powers of two that bring them to
-// [2^14, 2^15), scales[0] and [1].
+// The exponents of all rows of features and weight (yp_row_exponents), a wave a row; and, unless `part` is null, the largest of
+// either among the rows that take part, a part per workgroup, for back[0] and [1]: times 2^-back, those rows' largest finite
+// magnitude lies in [2^14, 2^15).
+#define YP_NO_EXPONENT (-100000)
 struct yp_peak_args {
   const float* src[2];
   int64_t rows[2];
@@ -356,15 +357,15 @@ struct yp_peak_args {
   yp_labels labels;            // of the first
   const float* bias;           // of the second, may be null
   int* exponent[2];
-  float* part;                 // [2][YP_PEAK_BLOCKS], may be null
+  int* part;                   // [2][YP_PEAK_BLOCKS], may be null; YP_NO_EXPONENT: only zeros
 };
 #define YP_PEAK_BLOCKS 2048
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_args a) {
-  __shared__ float red[YP_CL_THREADS / 64];
+  __shared__ int red[YP_CL_THREADS / 64];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    float most = 0.0f;
+    int most = YP_NO_EXPONENT;
     for (int64_t r = (int64_t)blockIdx.x * (YP_CL_THREADS / 64) + wave; r < a.rows[j]; r += YP_PEAK_BLOCKS * (YP_CL_THREADS / 64)) {
       const float* const p = a.src[j] + r * a.d;
       float top = 0.0f;
@@ -397,33 +398,34 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
       }
 #pragma unroll
       for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-      if (lane == 0) a.exponent[j][r] = __builtin_amdgcn_frexp_expf(top);      // (0 of 0)
-      if (a.part && (j == 0 ? a.labels.counted(r) >= 0 : !a.bias || a.bias[r] != -INFINITY)) most = fmaxf(most, top);
+      const int e = __builtin_amdgcn_frexp_expf(top);      // (0 of 0)
+      if (lane == 0) a.exponent[j][r] = e;
+      if (a.part && top > 0.0f && (j == 0 ? a.labels.counted(r) >= 0 : !a.bias || a.bias[r] != -INFINITY)) most = max(most, e);
     }
     if (!a.part) continue;
     __syncthreads();
     if (lane == 0) red[wave] = most;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < YP_CL_THREADS / 64; ++w) most = fmaxf(most, red[w]);
+      for (int w = 1; w < YP_CL_THREADS / 64; ++w) most = max(most, red[w]);
       a.part[j * YP_PEAK_BLOCKS + blockIdx.x] = most;
     }
   }
 }
 // (a wave each, its loads all in flight: one after the other they took 10 us)
-__global__ __launch_bounds__(128) void yp_scales_kernel(const float* part, float* scales) {
+__global__ __launch_bounds__(128) void yp_back_kernel(const int* part, int* back) {
   const int lane = (int)threadIdx.x & 63, j = (int)threadIdx.x >> 6;
-  yp_f4 v[YP_PEAK_BLOCKS / 256];
+  yp_i4 v[YP_PEAK_BLOCKS / 256];
 #pragma unroll
-  for (int i = 0; i < YP_PEAK_BLOCKS / 256; ++i) v[i] = reinterpret_cast<const yp_f4*>(part + j * YP_PEAK_BLOCKS)[i * 64 + lane];
-  float top = 0.0f;
+  for (int i = 0; i < YP_PEAK_BLOCKS / 256; ++i) v[i] = reinterpret_cast<const yp_i4*>(part + j * YP_PEAK_BLOCKS)[i * 64 + lane];
+  int most = YP_NO_EXPONENT;
 #pragma unroll
   for (int i = 0; i < YP_PEAK_BLOCKS / 256; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = fmaxf(top, v[i][e]);
+    for (int e = 0; e < 4; ++e) most = max(most, v[i][e]);
 #pragma unroll
-  for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-  if (lane == 0) scales[j] = top > 0.0f ? ldexpf(1.0f, min(max(14 - ilogbf(top), -100), 100)) : 1.0f;
+  for (int x = 32; x > 0; x >>= 1) most = max(most, __shfl_xor(most, x));
+  if (lane == 0) back[j] = most == YP_NO_EXPONENT ? 0 : most - 15;
 }
 
 __device__ __forceinline__ double yp_block_sum(double v, double* lds) {   // fixed order; result in thread 0
@@ -603,7 +605,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_su
   };
   for (int j = 0; j < a.jobs; ++j) {
     const yp_sum_job& b = a.job[j];
-    const float sc = b.scale.get();
+    const yp_factor sc = b.scale.get();
     if (b.parts < 4) {   // (or none: zeros) a thread an element
       for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < b.total; e += (int64_t)gridDim.x * YP_CL_THREADS) {
         float s = 0.0f;
@@ -655,7 +657,7 @@ static void add_sum(yp_sum_args& a, const float* part, int parts, int64_t stride
 static hipError_t zero(void* out, int64_t n, int type, hipStream_t st) {   // (a kernel, not a memset: the call may be captured)
   yp_sum_args a = {};
   a.out_type = type;
-  add_sum(a, nullptr, 0, 0, n, out, yp_scale{nullptr, nullptr, 1.0f, {}});
+  add_sum(a, nullptr, 0, 0, n, out, yp_scale{nullptr, nullptr, 0, nullptr});
   return sum_parts(a, st);
 }
 
@@ -673,7 +675,7 @@ struct ClassLossPlan {
   yp_tile_plan dzp, dwp, dhp;
   // workspace offsets
   int64_t o_eh, o_ew;          // both passes
-  int64_t o_scales, o_peaks;   // backward
+  int64_t o_back, o_peaks;   // backward
   int64_t o_h, o_w, o_part, o_picked, o_block, fwd_total;
   int64_t o_factor, o_hc, o_wc, o_hs, o_ws, o_dz, o_bp, o_dwpart, o_dhpart, bwd_total;
 };
@@ -727,7 +729,7 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   p.dzp = p.split ? yp_plan_shape(YP_TILE_M, p.piece, p.kn) : yp_plan_tiles(p.piece, p.kn, dsteps, largest);
   // the two gradient products share a launch and so a tile shape
   yp_plan_two(D, p.piece, p.kn / kr * p.segs, D, N, p.kv / YP_TILE_KB * p.segs, largest, &p.dwp, &p.dhp);
-  p.o_scales = take(p.split ? 8 : 0);
+  p.o_back = take(p.split ? 8 : 0);
   p.o_peaks = take(p.split ? 2 * YP_PEAK_BLOCKS * 4 : 0);
   p.o_factor = take(8);
   p.o_hc = take(p.kn * p.kd * planes);
@@ -759,16 +761,16 @@ static yp_copy_job copy_job(const void* src, char* dst, int64_t d, const ClassLo
   j.vec = row_bytes % 16 == 0 && ((uintptr_t)src & 15) == 0;
   return j;
 }
-// the rows' exponents; and scales[0], [1], of the features and of the weight, for the backward pass
-static hipError_t find_scales(const yp_class_loss_args& a, const yp_labels& labels, char* ws, const ClassLossPlan& p, bool backward, hipStream_t st) {
+// the rows' exponents; and back[0], [1], of the features and of the weight, for the backward pass
+static hipError_t find_exponents(const yp_class_loss_args& a, const yp_labels& labels, char* ws, const ClassLossPlan& p, bool backward, hipStream_t st) {
   yp_peak_args k;
   k.src[0] = (const float*)a.features; k.src[1] = (const float*)a.weight;
   k.rows[0] = a.n; k.rows[1] = a.v; k.d = a.d;
   k.vec = a.d % 4 == 0 && (((uintptr_t)a.features | (uintptr_t)a.weight) & 15) == 0;
-  k.labels = labels; k.bias = (const float*)a.bias; k.part = backward ? (float*)(ws + p.o_peaks) : nullptr;
+  k.labels = labels; k.bias = (const float*)a.bias; k.part = backward ? (int*)(ws + p.o_peaks) : nullptr;
   k.exponent[0] = (int*)(ws + p.o_eh); k.exponent[1] = (int*)(ws + p.o_ew);
   hipLaunchKernelGGL(yp_peak_kernel, dim3(YP_PEAK_BLOCKS), dim3(YP_CL_THREADS), 0, st, k);
-  if (backward) hipLaunchKernelGGL(yp_scales_kernel, dim3(1), dim3(128), 0, st, (const float*)k.part, (float*)(ws + p.o_scales));
+  if (backward) hipLaunchKernelGGL(yp_back_kernel, dim3(1), dim3(128), 0, st, (const int*)k.part, (int*)(ws + p.o_back));
   return hipGetLastError();
 }
 static hipError_t copy_rows(yp_copy_args a, hipStream_t st) {
@@ -788,7 +790,7 @@ static hipError_t forward_t(const yp_class_loss_args& a, hipStream_t st) {
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
   const int *const eh = (const int*)(ws + p.o_eh), *const ew = (const int*)(ws + p.o_ew);     // SPLIT
-  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, false, st));
+  if (SPLIT) CL_TRY(find_exponents(a, labels, ws, p, false, st));
   yp_softmax_part* const part = (yp_softmax_part*)(ws + p.o_part);
   int parts = 0;
   for (int s = 0; s < p.fwd_pieces; ++s) {
@@ -846,24 +848,24 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   char* const ws = (char*)a.workspace;
   const yp_labels labels = {a.labels, a.label_bytes, a.ignore_index, a.v};
   const int *const re_h = (const int*)(ws + p.o_eh), *const re_w = (const int*)(ws + p.o_ew);   // SPLIT
-  float* const scales = SPLIT ? (float*)(ws + p.o_scales) : nullptr;
-  if (SPLIT) CL_TRY(find_scales(a, labels, ws, p, true, st));
-  const float up = TYPE == YP_T_F16 ? 8192.0f : 1.0f;
+  const int* const common = SPLIT ? (const int*)(ws + p.o_back) : nullptr;
+  if (SPLIT) CL_TRY(find_exponents(a, labels, ws, p, true, st));
+  const int up = TYPE == YP_T_F16 ? 13 : 0;                 // dz is held times 2^up
   float* factor = nullptr;
-  yp_scale back = {a.grad, a.count, 1.0f / up, {}};         // one g for all rows
+  yp_scale back = {a.grad, a.count, -up, nullptr};          // one g for all rows
   if (a.grad_stride) {
-    back = yp_scale{nullptr, a.count, 1.0f, {}};
+    back = yp_scale{nullptr, a.count, 0, nullptr};
     if (TYPE != YP_T_F32) {                                 // (f32 as it is: dz is not rounded)
       factor = (float*)(ws + p.o_factor);
-      hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, labels, (int64_t)a.n, up, factor);
+      hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, labels, (int64_t)a.n, ldexpf(1.0f, up), factor);
       CL_TRY(hipGetLastError());
       back.a = factor + 1;
     }
   }
   float* const dhpart = (float*)(ws + p.o_dhpart);
   float* const biaspart = a.grad_bias && p.dzp.tiles_j > 1 ? (float*)(ws + p.o_bp) : nullptr;
-  yp_scale back_w = back, back_h = back;                    // of grad_weight, which has the features' scale, and the other way round
-  if (SPLIT) { back_w.over[0] = scales; back_h.over[0] = scales + 1; }
+  yp_scale back_w = back, back_h = back;                    // of grad_weight, which has the features' exponent, and the other way round
+  if (SPLIT) { back_w.more = common; back_h.more = common + 1; }
   yp_sum_args sums = {};
   sums.out_type = ELEM;
   for (int s = 0; s < p.pieces; ++s) {
@@ -879,13 +881,13 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
         yp_copy_job& j = c.job[n++];
         j = copy_job(a.features, ws + p.o_hc, a.d, p, a.n, p.kn);
         j.by_label = 1;
-        if (SPLIT) { j.exponent = re_h; j.common = ws + p.o_hs; j.scale = scales; }
+        if (SPLIT) { j.exponent = re_h; j.common = ws + p.o_hs; j.back = common; }
       }
       if (copy_w) {
         yp_copy_job& j = c.job[n++];
         j = copy_job(w, ws + p.o_wc, a.d, p, nv, nv);
         j.bias = bias;
-        if (SPLIT) { j.exponent = re_w + v0; j.common = ws + p.o_ws; j.scale = scales + 1; }
+        if (SPLIT) { j.exponent = re_w + v0; j.common = ws + p.o_ws; j.back = common + 1; }
         w = ws + p.o_wc;
       }
       CL_TRY(copy_rows(c, st));
@@ -900,7 +902,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     yp_epi_dz<ELEM, SPLIT, PLANES> e;
     e.plane = dzplane;
     e.exponents = yp_row_exponents{re_w + v0, re_h};
-    e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = up; e.scale = back;
+    e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = ldexpf(1.0f, up); e.scale = back;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
     e.bias_out = a.grad_bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
     e.bias_part = biaspart;

@@ -108,21 +108,24 @@ __device__ __forceinline__ float yp_load_as_float(const void* p, int64_t i, int 
   return type == YP_F32 ? reinterpret_cast<const float*>(p)[i]
        : type == YP_BF16 ? (float)reinterpret_cast<const __bf16*>(p)[i] : (float)reinterpret_cast<const _Float16*>(p)[i];
 }
-// A factor that lies on the device: by * (a ? *a : 1) / (count ? max(*count, 1) : 1) / (over[i] ? *over[i] : 1).
+// A factor that lies on the device, 2^by * (a ? *a : 1) / (count ? max(*count, 1) : 1) * (more ? 2^*more : 1), as m 2^e with m in
+// [1, 2): the factor itself may be outside f32's range where the products that it gives are not.
+struct yp_factor { float m; int e; };
+__device__ __forceinline__ yp_factor yp_factor_of(float v, int e) {      // v 2^e (0, infinities and NaN stay in m)
+  return {2.0f * __builtin_amdgcn_frexp_mantf(v), e + __builtin_amdgcn_frexp_expf(v) - 1};
+}
 struct yp_scale {
   const float* a;
   const float* count;
-  float by;
-  const float* over[2];
-  __device__ __forceinline__ float get() const {
-    float v = (a ? *a : 1.0f) * by / (count ? fmaxf(*count, 1.0f) : 1.0f);
-    if (over[0]) v /= *over[0];
-    if (over[1]) v /= *over[1];
-    return v;
+  int by;
+  const int* more;
+  __device__ __forceinline__ yp_factor get() const {
+    yp_factor f = yp_factor_of(a ? *a : 1.0f, by + (more ? *more : 0));
+    return count ? yp_factor_of(f.m / fmaxf(*count, 1.0f), f.e) : f;
   }
 };
 // (what is exactly zero stays so, whatever the factor)
-__device__ __forceinline__ float yp_times(float v, float scale) { return v == 0.0f ? 0.0f : v * scale; }
+__device__ __forceinline__ float yp_times(float v, const yp_factor& f) { return v == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(v * f.m, f.e); }
 
 // out[j][i] = scale * (C + before[j][i]), in type OUT; or, with `part`, the f32 sums of this split for a later join
 // (part[split][j][i], added to what is there if `add`).
@@ -143,7 +146,7 @@ struct yp_epi_store {
       if (add) yp_put_tile<YP_T_F32, SHAPE, true, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
       else yp_put_tile<YP_T_F32, SHAPE, false, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
     } else {
-      const float sc = scale.get();
+      const yp_factor sc = scale.get();
       if (OUT != YP_T_F32 && before) {
         typedef yp_shape<SHAPE> S;
         int i0, j0;
