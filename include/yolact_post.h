@@ -304,11 +304,12 @@ enum { YP_F32 = 0, YP_BF16 = 1, YP_F16 = 2, YP_INT8 = 3 };
  * The backward pass takes the forward's inputs and its lse, and grad = dL/dlosses: [n] float32 (grad_stride 1) or one
  * value for every row (grad_stride 0); with count != NULL the values are divided by max(*count, 1) (the mean: pass the
  * forward's count).  Gradients that are NULL are not computed (one at least is wanted, unless n is 0).  Products
- * accumulate in float32, gradients are rounded once; dz = grad (softmax - onehot) is rounded to dtype before its products, relative to the largest |grad| (f16: steps of at least
- * 2^-37 of it).  YP_F32 with n v d >= 2^31 multiplies each value as the sum of two f16: off by at most 2^-22 of itself or, if
- * that is more, 2^-39 of the largest finite magnitude in its row where logits are computed, in its tensor's rows that take
- * part where gradients are (dz: 2^-38 of the largest |grad|).  Probabilities are exp(z - lse), so 2^-23 |lse| is their relative error where logits are
- * large.  Fixed order of sums, no float atomics.
+ * accumulate in float32, gradients are rounded once; dz = grad (softmax - onehot) is rounded to dtype before its products,
+ * relative to the largest |grad| (f16: steps of at least 2^-37 of it).  YP_F32 with n v d >= 2^31 multiplies each value as
+ * the sum of two f16, off by at most 2^-22 of itself or, if that is more, 2^-39 of the largest finite magnitude: in its own
+ * row where logits are computed, in its tensor's rows that take part where gradients are - for the weight's gradient,
+ * features times their row's grad; softmax - onehot is off by 2^-22 of itself or 2^-38.  Probabilities are exp(z - lse), so
+ * 2^-23 |lse| is their relative error where logits are large.  Fixed order of sums, no float atomics.
  * 0 <= n <= 2^20, 1 <= v <= 2^24, n v <= 2^38, 1 <= d <= 65536; contiguous tensors, aligned to their elements.  All pointers on the
  * device; asynchronous on hip_stream; allocates nothing, may be captured. */
 int64_t yp_class_loss_workspace(int32_t n, int32_t v, int32_t d, int32_t dtype, int32_t has_bias, int32_t backward);

@@ -98,7 +98,7 @@ def _check_large_float32(h, w, b, y, up, wild=()):
 
 
 @pytest.mark.parametrize("bias", [True, False])
-@pytest.mark.parametrize("row,features,weight", [(1.0, 2.0 ** 112, 2.0 ** -112), (1.0, 2.0 ** 118, 2.0 ** -119),
+@pytest.mark.parametrize("row,features,weight", [(2.0 ** 120, 1.0, 2.0 ** -116), (1.0, 2.0 ** 112, 2.0 ** -112), (1.0, 2.0 ** 118, 2.0 ** -119),
                                                  (2.0 ** -100, 2.0 ** -110, 2.0 ** 112), (1.0, 1.0, 2.0 ** -125)])
 def test_large_float32_values_at_the_ends_of_the_type(row, features, weight, bias):
     """Values of 2^116 and more, and tensors whose largest value is 2^-110 and less, with logits of ordinary size."""
@@ -117,3 +117,9 @@ def test_large_float32_rows_of_zeros_beside_very_large_ones():
     _check_large_float32(h, w, b, y, up, wild=(0,))
     y[0] = -1
     _check_large_float32(h, w, b, y, up, wild=(0,))
+
+
+def test_large_float32_rows_of_far_smaller_gradients():
+    h, w, b, y, up = _inputs(2048, 8192, 130, torch.float32, True)
+    up[::2] *= 2.0 ** -30
+    _check_large_float32(h, w, b, y, up)

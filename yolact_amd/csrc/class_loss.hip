@@ -17,7 +17,8 @@
 // half a step of that type, like the gradients themselves.  It is held relative to the largest |g| - one g for all rows
 // is taken out altogether -, which the results get back in f32: with g inside, every row's -g would be rounded the same
 // way, and sums over rows be off by as much as one of them.  f16 with 2^13 more, so that probabilities down to 2^-38 are
-// kept.  Where rows are few, their roundings do not average out, and dz has two planes (twice the precision).
+// kept; in the planes of f32 (below) g stays outside altogether: dh's rows get theirs at the end, dw's product
+// reads g h instead of h, so that a row of far smaller g keeps its bits.  Where rows are few, their roundings do not average out, and dz has two planes (twice the precision).
 // f32 of any size worth it runs on the f16 matrix instructions, as two f16 planes per operand (SPLIT; gemm_tile.hpp): 22 bits
 // of a value, or 2^-39 of the largest one where that is more - a value below 2^-17 of the largest has fewer bits than f32,
 // its share of a sum over both is as good.  In z, whose sums run along the rows, the largest is the row's own, of h and of w
@@ -165,7 +166,8 @@ struct yp_epi_dz {
   const void* bias;            // of the tensors' type ELEM; of the piece
   const float* lse;
   yp_labels labels;
-  const float* grad;           // of every row, times *factor (if there is one); null: `up` for all of them
+  const float* grad;           // of every row, times *factor (if there is one); null: `up` for all of them.  SPLIT: `up`
+                               // for all of them in dz, `grad` in the bias gradient only
   const float* factor;
   float up;
   yp_scale scale;              // what the bias gradient gets back
@@ -183,6 +185,7 @@ struct yp_epi_dz {
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
     const float by = grad && factor ? *factor : up;
+    float own[NJ];
     if constexpr (SPLIT) exponents.give_back<SHAPE>(acc, ib, jb);
     if (bias || (at.ti + 1) * S::BM > g.I) {      // a class that takes no part, or does not exist: z = -inf
 #pragma unroll
@@ -202,7 +205,8 @@ struct yp_epi_dz {
       const float l = label >= 0 ? lse[j] : INFINITY;
       // exp(z - lse) = 2^min(z log2e + c, 0) - rounding may bring z above lse, by any amount where large products cancel -; a
       // row that takes no part, or has no class left: 2^-inf = 0; one with NaN among its z has it in lse, and here in gr
-      const float gr = label < 0 ? 0.0f : l != l ? l : grad ? grad[j] * by : by;
+      const float gr = label < 0 ? 0.0f : l != l ? l : grad && !SPLIT ? grad[j] * by : by;
+      own[n] = SPLIT && grad && label >= 0 ? grad[j] : 1.0f;
       const float c = fabsf(l) == INFINITY ? -INFINITY : __builtin_amdgcn_fmed3f(-l * YP_LOG2E, -0x1.fffffep127f, 0x1.fffffep127f);
       const int hit = label < 0 ? -1 : label - first - ib;
       if (__builtin_amdgcn_ballot_w64(hit >= 0 && hit < S::BM)) {      // (mostly no lane of the wave)
@@ -229,7 +233,7 @@ struct yp_epi_dz {
         for (int r = 0; r < 4; ++r) {
           float col = 0.0f;
 #pragma unroll
-          for (int n = 0; n < NJ; ++n) col += acc[m][n][r];
+          for (int n = 0; n < NJ; ++n) col += SPLIT ? acc[m][n][r] * own[n] : acc[m][n][r];
 #pragma unroll
           for (int x = 1; x < 16; x <<= 1) col += __shfl_xor(col, x);
           if ((at.lane & 15) == 0) lds[at.wj * S::BM + il + yp_frag_at<S::BM, MI>(m) + r] = col;
@@ -273,8 +277,9 @@ struct yp_copy_job {
   const void* bias;
   int64_t plane;          // 0, or: f32 rows to two f16 planes, this many bytes apart (row_bytes, kb: of a plane's row),
   const int* exponent;    //   each held by its own exponent (yp_row_exponents)
-  char* common;           //   and, unless null, to two more, times 2^-*back: for products that add up over the rows
+  char* common;           //   and, unless null, to two more, times 2^-*back: for products that add up over the rows;
   const int* back;
+  const float* grad;      //   and times this of its row, unless null
 };
 struct yp_copy_args {
   yp_copy_job job[2];
@@ -324,8 +329,10 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
       };
       put(j.dst, [&](float v) { return __builtin_amdgcn_ldexpf(v, up); });
       if (j.common) {
-        const int all = -*j.back;
-        put(j.common, [&](float v) { return __builtin_amdgcn_ldexpf(v, all); });
+        // (the product of the row as it is held and the gradient's mantissa: neither leaves f32's range on the way)
+        const float gr = j.grad && in ? j.grad[r] : 1.0f, gm = __builtin_amdgcn_frexp_mantf(gr);
+        const int by = __builtin_amdgcn_frexp_expf(gr) - up - *j.back;
+        put(j.common, [&](float v) { return __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(v, up) * gm, by); });
       }
       continue;
     }
@@ -348,7 +355,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
 
 // The exponents of all rows of features and weight (yp_row_exponents), a wave a row; and, unless `part` is null, the largest of
 // either among the rows that take part, a part per workgroup, for back[0] and [1]: times 2^-back, those rows' largest finite
-// magnitude lies in [2^14, 2^15).
+// magnitude (times its row's `grad`, if there is one) lies in [2^14, 2^15).
 #define YP_NO_EXPONENT (-100000)
 struct yp_peak_args {
   const float* src[2];
@@ -356,6 +363,7 @@ struct yp_peak_args {
   int d, vec;
   yp_labels labels;            // of the first
   const float* bias;           // of the second, may be null
+  const float* grad;           // of the first, may be null
   int* exponent[2];
   int* part;                   // [2][YP_PEAK_BLOCKS], may be null; YP_NO_EXPONENT: only zeros
 };
@@ -400,7 +408,11 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_peak_kernel(const yp_peak_ar
       for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
       const int e = __builtin_amdgcn_frexp_expf(top);      // (0 of 0)
       if (lane == 0) a.exponent[j][r] = e;
-      if (a.part && top > 0.0f && (j == 0 ? a.labels.counted(r) >= 0 : !a.bias || a.bias[r] != -INFINITY)) most = max(most, e);
+      if (a.part && top > 0.0f && (j == 0 ? a.labels.counted(r) >= 0 : !a.bias || a.bias[r] != -INFINITY)) {
+        const float g = j == 0 && a.grad ? fabsf(a.grad[r]) : 1.0f;
+        if (g > 0.0f && g < INFINITY)       // the product's exponent, without the product: f32's range may be too small for it
+          most = max(most, e + __builtin_amdgcn_frexp_expf(g) + __builtin_amdgcn_frexp_expf(__builtin_amdgcn_frexp_mantf(top) * __builtin_amdgcn_frexp_mantf(g)));
+      }
     }
     if (!a.part) continue;
     __syncthreads();
@@ -593,24 +605,28 @@ struct yp_bias_sum {
 
 // Up to two arrays, each out[e] = its scale * sum over its parts.  64 elements and 4 waves a workgroup: wave w adds parts
 // w, w + 4, ... in their order, then the four sums are added in theirs.
-struct yp_sum_job { const float* part; int parts; int64_t stride, total; void* out; yp_scale scale; };
+struct yp_sum_job {
+  const float* part; int parts; int64_t total; void* out; yp_scale scale;
+  const float* row; int cols;      // null, or another factor for every row of as many elements
+};
 struct yp_sum_args { yp_sum_job job[2]; int jobs, out_type; };
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_sum_args a) {
   __shared__ float red[YP_CL_THREADS / 64][64];
   const int x = (int)threadIdx.x & 63, y = (int)threadIdx.x >> 6;
-  auto put = [&](void* out, int64_t e, float s) {
-    if (a.out_type == YP_F32) reinterpret_cast<float*>(out)[e] = s;
-    else if (a.out_type == YP_BF16) reinterpret_cast<__bf16*>(out)[e] = (__bf16)s;
-    else reinterpret_cast<_Float16*>(out)[e] = (_Float16)s;
-  };
   for (int j = 0; j < a.jobs; ++j) {
     const yp_sum_job& b = a.job[j];
     const yp_factor sc = b.scale.get();
+    auto put = [&](int64_t e, float s) {
+      s = yp_times(s, b.row ? yp_with(sc, b.row[e / b.cols]) : sc);
+      if (a.out_type == YP_F32) reinterpret_cast<float*>(b.out)[e] = s;
+      else if (a.out_type == YP_BF16) reinterpret_cast<__bf16*>(b.out)[e] = (__bf16)s;
+      else reinterpret_cast<_Float16*>(b.out)[e] = (_Float16)s;
+    };
     if (b.parts < 4) {   // (or none: zeros) a thread an element
       for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < b.total; e += (int64_t)gridDim.x * YP_CL_THREADS) {
         float s = 0.0f;
-        for (int p = 0; p < b.parts; ++p) s += b.part[(int64_t)p * b.stride + e];
-        put(b.out, e, yp_times(s, sc));
+        for (int p = 0; p < b.parts; ++p) s += b.part[(int64_t)p * b.total + e];
+        put(e, s);
       }
       continue;
     }
@@ -622,16 +638,16 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_sum_parts_kernel(const yp_su
         for (; p + 12 < b.parts; p += 16) {
           float v[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = b.part[(int64_t)(p + 4 * u) * b.stride + e];
+          for (int u = 0; u < 4; ++u) v[u] = b.part[(int64_t)(p + 4 * u) * b.total + e];
 #pragma unroll
           for (int u = 0; u < 4; ++u) s += v[u];
         }
-        for (; p < b.parts; p += 4) s += b.part[(int64_t)p * b.stride + e];
+        for (; p < b.parts; p += 4) s += b.part[(int64_t)p * b.total + e];
       }
       __syncthreads();
       red[y][x] = s;
       __syncthreads();
-      if (y == 0 && e < b.total) put(b.out, e, yp_times(((red[0][x] + red[1][x]) + red[2][x]) + red[3][x], sc));
+      if (y == 0 && e < b.total) put(e, ((red[0][x] + red[1][x]) + red[2][x]) + red[3][x]);
     }
   }
 }
@@ -651,13 +667,13 @@ static hipError_t sum_parts(const yp_sum_args& a, hipStream_t st) {
   hipLaunchKernelGGL(yp_sum_parts_kernel, dim3(blocks_for(most, 1, 8192)), dim3(YP_CL_THREADS), 0, st, a);
   return hipGetLastError();
 }
-static void add_sum(yp_sum_args& a, const float* part, int parts, int64_t stride, int64_t total, void* out, const yp_scale& scale) {
-  a.job[a.jobs++] = yp_sum_job{part, parts, stride, total, out, scale};
+static void add_sum(yp_sum_args& a, const float* part, int parts, int64_t total, void* out, const yp_scale& scale, const float* row, int cols) {
+  a.job[a.jobs++] = yp_sum_job{part, parts, total, out, scale, row, cols};
 }
 static hipError_t zero(void* out, int64_t n, int type, hipStream_t st) {   // (a kernel, not a memset: the call may be captured)
   yp_sum_args a = {};
   a.out_type = type;
-  add_sum(a, nullptr, 0, 0, n, out, yp_scale{nullptr, nullptr, 0, nullptr});
+  add_sum(a, nullptr, 0, n, out, yp_scale{nullptr, nullptr, 0, nullptr}, nullptr, 1);
   return sum_parts(a, st);
 }
 
@@ -767,7 +783,7 @@ static hipError_t find_exponents(const yp_class_loss_args& a, const yp_labels& l
   k.src[0] = (const float*)a.features; k.src[1] = (const float*)a.weight;
   k.rows[0] = a.n; k.rows[1] = a.v; k.d = a.d;
   k.vec = a.d % 4 == 0 && (((uintptr_t)a.features | (uintptr_t)a.weight) & 15) == 0;
-  k.labels = labels; k.bias = (const float*)a.bias; k.part = backward ? (int*)(ws + p.o_peaks) : nullptr;
+  k.labels = labels; k.bias = (const float*)a.bias; k.grad = backward && a.grad_stride ? a.grad : nullptr; k.part = backward ? (int*)(ws + p.o_peaks) : nullptr;
   k.exponent[0] = (int*)(ws + p.o_eh); k.exponent[1] = (int*)(ws + p.o_ew);
   hipLaunchKernelGGL(yp_peak_kernel, dim3(YP_PEAK_BLOCKS), dim3(YP_CL_THREADS), 0, st, k);
   if (backward) hipLaunchKernelGGL(yp_back_kernel, dim3(1), dim3(128), 0, st, (const int*)k.part, (int*)(ws + p.o_back));
@@ -854,8 +870,8 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   float* factor = nullptr;
   yp_scale back = {a.grad, a.count, -up, nullptr};          // one g for all rows
   if (a.grad_stride) {
-    back = yp_scale{nullptr, a.count, 0, nullptr};
-    if (TYPE != YP_T_F32) {                                 // (f32 as it is: dz is not rounded)
+    back = yp_scale{nullptr, a.count, SPLIT ? -up : 0, nullptr};
+    if (!SPLIT && TYPE != YP_T_F32) {                       // (f32 as it is: dz is not rounded)
       factor = (float*)(ws + p.o_factor);
       hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, labels, (int64_t)a.n, ldexpf(1.0f, up), factor);
       CL_TRY(hipGetLastError());
@@ -881,7 +897,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
         yp_copy_job& j = c.job[n++];
         j = copy_job(a.features, ws + p.o_hc, a.d, p, a.n, p.kn);
         j.by_label = 1;
-        if (SPLIT) { j.exponent = re_h; j.common = ws + p.o_hs; j.back = common; }
+        if (SPLIT) { j.exponent = re_h; j.common = ws + p.o_hs; j.back = common; j.grad = a.grad_stride ? a.grad : nullptr; }
       }
       if (copy_w) {
         yp_copy_job& j = c.job[n++];
@@ -928,7 +944,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     gh.b = ws + p.o_dz; gh.ldb = (int64_t)kv * tb; gh.J = a.n;
     gh.K = nv; gh.steps = (int)((int64_t)kv * tb / YP_TILE_KB);
     yp_epi_store<ELEM> eh = {};
-    eh.out = a.grad_features; eh.ld = a.d; eh.scale = back_h;
+    eh.out = a.grad_features; eh.ld = a.d; eh.scale = back_h; eh.row = SPLIT && a.grad_stride ? a.grad : nullptr;
     eh.vec = row % 16 == 0 && ((uintptr_t)a.grad_features & 15) == 0;
     eh.part_vec = a.d % 4 == 0;
     // (over pieces dh adds up in f32; for 16-bit types without a split the last one adds what lies there and rounds,
@@ -940,8 +956,8 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     yp_bias_sum bs = {};
     bs.part = biaspart; bs.parts = p.dzp.tiles_j; bs.total = nv; bs.type = ELEM; bs.scale = back; bs.out = e.bias_out;
     CL_TRY(yp_launch_two<TYPE, SPLIT ? 3 : PLANES>(twp, gw, ew, p.dhp, gh, eh, bs, biaspart ? (nv + yp_bias_sum::CLASSES - 1) / yp_bias_sum::CLASSES : 0, st));
-    if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, (int64_t)nv * a.d, gwo, back_w);
-    if (s == p.pieces - 1 && eh.part && a.grad_features) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, (int64_t)a.n * a.d, a.grad_features, back_h);
+    if (ew.part) add_sum(sums, ew.part, p.dwp.splits, (int64_t)nv * a.d, gwo, back_w, nullptr, a.d);
+    if (s == p.pieces - 1 && eh.part && a.grad_features) add_sum(sums, dhpart, p.dhp.splits, (int64_t)a.n * a.d, a.grad_features, back_h, eh.row, a.d);
     CL_TRY(sum_parts(sums, st));
     sums.jobs = 0;
   }

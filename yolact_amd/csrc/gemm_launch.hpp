@@ -124,6 +124,10 @@ struct yp_scale {
     return count ? yp_factor_of(f.m / fmaxf(*count, 1.0f), f.e) : f;
   }
 };
+__device__ __forceinline__ yp_factor yp_with(const yp_factor& f, float v) {
+  const yp_factor x = yp_factor_of(v, f.e);
+  return {x.m * f.m, x.e};
+}
 // (what is exactly zero stays so, whatever the factor)
 __device__ __forceinline__ float yp_times(float v, const yp_factor& f) { return v == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(v * f.m, f.e); }
 
@@ -135,6 +139,7 @@ struct yp_epi_store {
   int64_t ld;             // elements
   int vec, part_vec;      // rows of out / of part are multiples of 16 bytes
   yp_scale scale;
+  const float* row;       // null, or another factor for every row j (f32 in f16 planes only)
   const float* before;    // null: nothing (16-bit types only: those of f32 lose more to the registers it takes)
   float* part;
   int add;
@@ -147,6 +152,23 @@ struct yp_epi_store {
       else yp_put_tile<YP_T_F32, SHAPE, false, MI, NJ>(at, to, g.I, g.I, g.J, part_vec != 0, val);
     } else {
       const yp_factor sc = scale.get();
+      if constexpr (TYPE == YP_T_F16 && OUT == YP_T_F32) {
+        if (row) {
+          typedef yp_shape<SHAPE> S;
+          int i0, j0;
+          yp_origin<SHAPE>(at, i0, j0);
+          yp_factor f[NJ];
+#pragma unroll
+          for (int n = 0; n < NJ; ++n) { const int j = j0 + yp_frag_at<S::BN, NJ>(n); f[n] = yp_with(sc, j < g.J ? row[j] : 0.0f); }
+          yp_put_tile<OUT, SHAPE, false, MI, NJ>(at, out, ld, g.I, g.J, vec != 0, [&](int m, int n) {
+            yp_f4 v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = yp_times(acc[m][n][r], f[n]);
+            return v;
+          });
+          return;
+        }
+      }
       if (OUT != YP_T_F32 && before) {
         typedef yp_shape<SHAPE> S;
         int i0, j0;
