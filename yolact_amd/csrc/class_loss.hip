@@ -161,14 +161,17 @@ struct yp_epi_stats {
 };
 
 // ---- epilogue of the backward product -----------------------------------------------------------------------------
+// What g is held by, relative to the largest |g| = m 2^e, m in [1, 2), of the rows that take part (and whose g is finite: what an
+// infinity gives is no matter of scale): g 2^-e (2^up / m), and the results get m 2^-up 2^e back.
+struct yp_relative { float by, back; int e; };
 template <int ELEM, bool SPLIT, int PLANES>
 struct yp_epi_dz {
   const void* bias;            // of the tensors' type ELEM; of the piece
   const float* lse;
   yp_labels labels;
-  const float* grad;           // of every row, times *factor (if there is one); null: `up` for all of them.  SPLIT: `up`
+  const float* grad;           // of every row, as `relative` says (if there is one); null: `up` for all of them.  SPLIT: `up`
                                // for all of them in dz, `grad` in the bias gradient only
-  const float* factor;
+  const yp_relative* relative;
   float up;
   yp_scale scale;              // what the bias gradient gets back
   yp_row_exponents exponents;  // SPLIT
@@ -184,7 +187,7 @@ struct yp_epi_dz {
     typedef typename yp_type<ELEM>::elem elem;
     int ib, jb;
     yp_origin<SHAPE>(at, ib, jb);
-    const float by = grad && factor ? *factor : up;
+    const yp_relative held = relative ? *relative : yp_relative{1.0f, 1.0f, 0};
     float own[NJ];
     if constexpr (SPLIT) exponents.give_back<SHAPE>(acc, ib, jb);
     if (bias || (at.ti + 1) * S::BM > g.I) {      // a class that takes no part, or does not exist: z = -inf
@@ -205,7 +208,7 @@ struct yp_epi_dz {
       const float l = label >= 0 ? lse[j] : INFINITY;
       // exp(z - lse) = 2^min(z log2e + c, 0) - rounding may bring z above lse, by any amount where large products cancel -; a
       // row that takes no part, or has no class left: 2^-inf = 0; one with NaN among its z has it in lse, and here in gr
-      const float gr = label < 0 ? 0.0f : l != l ? l : grad && !SPLIT ? grad[j] * by : by;
+      const float gr = label < 0 ? 0.0f : l != l ? l : grad && !SPLIT ? __builtin_amdgcn_ldexpf(grad[j], -held.e) * held.by : up;
       own[n] = SPLIT && grad && label >= 0 ? grad[j] : 1.0f;
       const float c = fabsf(l) == INFINITY ? -INFINITY : __builtin_amdgcn_fmed3f(-l * YP_LOG2E, -0x1.fffffep127f, 0x1.fffffep127f);
       const int hit = label < 0 ? -1 : label - first - ib;
@@ -537,9 +540,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_reduce_kernel(const double* 
   if (threadIdx.x == 0) reduced.put(ts, tc);
 }
 
-// {by / largest |g|, largest |g| / by} over the rows that take part (whose g is finite: what an infinity gives is no
-// matter of scale)
-__global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, const yp_labels labels, int64_t n, float by, float* factor) {
+__global__ __launch_bounds__(1024) void yp_relative_kernel(const float* grad, const yp_labels labels, int64_t n, int up, yp_relative* out) {
   __shared__ float red[16];
   float top = 0.0f;
   auto see = [&](float v, int label) {
@@ -562,9 +563,8 @@ __global__ __launch_bounds__(1024) void yp_factor_kernel(const float* grad, cons
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
-    if (!(top >= 0x1p-112f)) top = 1.0f;      // (nothing to go by)
-    factor[0] = by / top;
-    factor[1] = top / by;
+    const yp_factor f = yp_factor_of(top > 0.0f ? top : 1.0f, 0);      // (1: nothing to go by)
+    *out = {__builtin_amdgcn_ldexpf(1.0f, up) / f.m, __builtin_amdgcn_ldexpf(f.m, -up), f.e};
   }
 }
 
@@ -693,7 +693,7 @@ struct ClassLossPlan {
   int64_t o_eh, o_ew;          // both passes
   int64_t o_back, o_peaks;   // backward
   int64_t o_h, o_w, o_part, o_picked, o_block, fwd_total;
-  int64_t o_factor, o_hc, o_wc, o_hs, o_ws, o_dz, o_bp, o_dwpart, o_dhpart, bwd_total;
+  int64_t o_relative, o_hc, o_wc, o_hs, o_ws, o_dz, o_bp, o_dwpart, o_dhpart, bwd_total;
 };
 
 static void cut_pieces(int64_t V, int64_t most, int* pieces, int* piece) {   // equal pieces, multiples of 256
@@ -747,7 +747,7 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   yp_plan_two(D, p.piece, p.kn / kr * p.segs, D, N, p.kv / YP_TILE_KB * p.segs, largest, &p.dwp, &p.dhp);
   p.o_back = take(p.split ? 8 : 0);
   p.o_peaks = take(p.split ? 2 * YP_PEAK_BLOCKS * 4 : 0);
-  p.o_factor = take(8);
+  p.o_relative = take(sizeof(yp_relative));
   p.o_hc = take(p.kn * p.kd * planes);
   p.o_wc = take(p.piece * p.kd * planes);
   p.o_hs = take(p.split ? p.kn * p.kd * planes : 0);
@@ -867,15 +867,16 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
   const int* const common = SPLIT ? (const int*)(ws + p.o_back) : nullptr;
   if (SPLIT) CL_TRY(find_exponents(a, labels, ws, p, true, st));
   const int up = TYPE == YP_T_F16 ? 13 : 0;                 // dz is held times 2^up
-  float* factor = nullptr;
+  yp_relative* relative = nullptr;
   yp_scale back = {a.grad, a.count, -up, nullptr};          // one g for all rows
   if (a.grad_stride) {
     back = yp_scale{nullptr, a.count, SPLIT ? -up : 0, nullptr};
     if (!SPLIT && TYPE != YP_T_F32) {                       // (f32 as it is: dz is not rounded)
-      factor = (float*)(ws + p.o_factor);
-      hipLaunchKernelGGL(yp_factor_kernel, dim3(1), dim3(1024), 0, st, a.grad, labels, (int64_t)a.n, ldexpf(1.0f, up), factor);
+      relative = (yp_relative*)(ws + p.o_relative);
+      hipLaunchKernelGGL(yp_relative_kernel, dim3(1), dim3(1024), 0, st, a.grad, labels, (int64_t)a.n, up, relative);
       CL_TRY(hipGetLastError());
-      back.a = factor + 1;
+      back.a = &relative->back;
+      back.more = &relative->e;
     }
   }
   float* const dhpart = (float*)(ws + p.o_dhpart);
@@ -918,7 +919,7 @@ static hipError_t backward_t(const yp_class_loss_args& a, hipStream_t st) {
     yp_epi_dz<ELEM, SPLIT, PLANES> e;
     e.plane = dzplane;
     e.exponents = yp_row_exponents{re_w + v0, re_h};
-    e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.factor = factor; e.up = ldexpf(1.0f, up); e.scale = back;
+    e.bias = bias; e.lse = a.lse; e.labels = labels; e.grad = a.grad_stride ? a.grad : nullptr; e.relative = relative; e.up = ldexpf(1.0f, up); e.scale = back;
     e.first = v0; e.dz = ws + p.o_dz; e.kv = kv; e.kn = (int)p.kn;
     e.bias_out = a.grad_bias ? (char*)a.grad_bias + (int64_t)v0 * b : nullptr;
     e.bias_part = biaspart;
