@@ -291,6 +291,8 @@ struct yp_copy_args {
   yp_labels labels;
   int type;
 };
+// (PLANES apart: the few rows of 16-bit copies that a thread takes waited for its registers and arguments, 22 -> 38 us, 30011 x 1000)
+template <bool PLANES>
 __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_copy_args a) {
   for (int64_t e = (int64_t)blockIdx.x * YP_CL_THREADS + threadIdx.x; e < a.chunks; e += (int64_t)gridDim.x * YP_CL_THREADS) {
     const bool second = e >= a.chunks0;
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(YP_CL_THREADS) void yp_copy_rows_kernel(const yp_co
     bool in = r < j.rows;
     if (in && j.by_label) in = a.labels.counted(r) >= 0;
     if (in && j.bias) in = yp_load_as_float(j.bias, r, a.type) != -INFINITY;
-    if (j.plane) {        // 8 elements
+    if constexpr (PLANES) {        // 8 elements
       const int up = in ? 15 - j.exponent[r] : 0;
       float x[8];
 #pragma unroll
@@ -792,7 +794,9 @@ static hipError_t find_exponents(const yp_class_loss_args& a, const yp_labels& l
 static hipError_t copy_rows(yp_copy_args a, hipStream_t st) {
   a.chunks0 = a.job[0].rows_out * (a.job[0].kb / 16);
   a.chunks = a.chunks0 + (a.job[1].src ? a.job[1].rows_out * (a.job[1].kb / 16) : 0);
-  hipLaunchKernelGGL(yp_copy_rows_kernel, dim3(blocks_for(a.chunks, YP_CL_THREADS, 8192)), dim3(YP_CL_THREADS), 0, st, a);
+  const dim3 grid(blocks_for(a.chunks, YP_CL_THREADS, 8192));
+  if (a.job[0].plane) hipLaunchKernelGGL(yp_copy_rows_kernel<true>, grid, dim3(YP_CL_THREADS), 0, st, a);
+  else hipLaunchKernelGGL(yp_copy_rows_kernel<false>, grid, dim3(YP_CL_THREADS), 0, st, a);
   return hipGetLastError();
 }
 
