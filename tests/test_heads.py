@@ -161,3 +161,16 @@ def test_python_refuses_what_is_not_on_the_device():
         heads.ClassLoss.apply(x, torch.zeros(9, 8), None, torch.zeros(3, dtype=torch.int64), -1, "all")
     with pytest.raises(ValueError, match="state"):
         heads.class_head_loss(x, torch.zeros(9, 8), None, torch.zeros(3, dtype=torch.int64), dropout_p=0.5)
+
+
+def test_assembly_names_the_registers_it_writes():
+    """A register that an asm block writes by name is in its clobber list: the compiler may keep something there."""
+    csrc = os.path.join(ROOT, "yolact_amd", "csrc")
+    seen = 0
+    for name in sorted(os.listdir(csrc)):
+        for block in re.findall(r"asm\s+volatile\s*\((.*?)\);", open(os.path.join(csrc, name)).read(), flags=re.S):
+            code, *rest = re.split(r"(?<!:):(?!:)|::", block)
+            for reg in re.findall(r"\b[sv]_\w+\s+(m0|vcc|exec|scc|[sv]\d+)\b", code):
+                seen += 1
+                assert f'"{reg}"' in rest[-1], (name, block)
+    assert seen > 0

@@ -106,10 +106,14 @@ __device__ __forceinline__ int64_t yp_uniform(int64_t v) {
 
 // 64 lanes x 16 bytes from base + off (per lane) to LDS at `lds` (uniform) + lane * 16.  Written as assembly because the
 // compiler would wait for it before every later LDS read that it cannot tell apart; the kernel below waits itself
-// (yp_arrive).  It writes no register.
+// (yp_arrive).  It writes no register but m0, and says so: nothing of the compiler's may stand between its own write of m0 and
+// the use.  (That it restores nothing is what the compiler would warn of at every use; nobody expects m0 to last.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void yp_load_lds16(const char* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // All but the last N of this wave's loads have landed and its LDS reads are done; then everybody's.
 template <int N>
 __device__ __forceinline__ void yp_arrive() {
