@@ -326,7 +326,7 @@ int yp_class_loss_backward(int32_t device_id, int32_t n, int32_t v, int32_t d, i
  *   zeros)                              out[i,j] = (sum_k xq[i,k] wq[j,k]) x_scale[i] w_scale[j] + bias[j]
  * q rows are yp_quantized_row_bytes(k) bytes apart (k padded to 128), the padding is zero; 16-byte aligned.  A row that
  * holds an infinity or NaN gets the scale NaN, so its results are NaN.  1 <= k <= 131072 (the integer sums fit 32 bits);
- * rows v <= 2^37.
+ * 1 <= v <= 2^24, rows v <= 2^37.
  *   yp_quantize_rows     x [rows,k] contiguous, dtype YP_F32 / YP_BF16 / YP_F16 -> q, scale [rows] float32
  *   yp_quantized_linear  x: dtype YP_INT8 (x = q rows, x_scale their scales) or a float type, x [rows,k] contiguous,
  *                        quantized on the way into workspace (yp_quantized_linear_workspace(rows, k) bytes, 256-byte

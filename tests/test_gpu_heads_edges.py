@@ -143,3 +143,19 @@ def test_gradients_below_the_smallest_normal_ones(dt, n, v, d):
     leaf = w.clone().requires_grad_()
     gw, = torch.autograd.grad(heads.ClassLoss.apply(h, leaf, b, y, -1, "sum"), [leaf], one)
     ref.within(gw, *bounds(h, w, b, y, torch.full_like(up, 1.0) * one)["grad_w"], "grad_w")
+
+
+@pytest.mark.parametrize("rows,v", [((1 << 28) + 3, 20), ((1 << 23) + 3, 600)])
+def test_quantized_linear_past_32_bits_of_results(rows, v):
+    """A row's results depend on that row alone: those at the ends of a call of 2^32 results are a small call's."""
+    from yolact_amd import heads
+    x = torch.randint(-100, 100, (rows, 1), generator=_gen(rows), device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    w = heads.quantize_rows(torch.randn(v, 1, generator=_gen(v), device="cuda"))
+    b = torch.randn(v, generator=_gen(v + 1), device="cuda")
+    y = heads.quantized_linear(x, w, bias=b, out_dtype=torch.bfloat16)
+    assert y.numel() > 1 << 32
+    for at in (0, (1 << 32) // v - 50, rows - 100):
+        part = x[at:at + 100].contiguous()
+        few = heads.quantized_linear(part, w, bias=b, out_dtype=torch.bfloat16)
+        assert torch.equal(y[at:at + 100], few)
+        ref.within(few, *ref.quantized_linear(*ref.quantize(part), w.q[:, :1].long(), w.scale, b, torch.bfloat16), "quantized_linear")

@@ -3,6 +3,7 @@ and in Python."""
 import ctypes
 import os
 import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -174,3 +175,49 @@ def test_assembly_names_the_registers_it_writes():
                 seen += 1
                 assert f'"{reg}"' in rest[-1], (name, block)
     assert seen > 0
+
+
+def test_quantized_linear_takes_every_size_that_is_stated():
+    """rows v <= 2^37 and v <= 2^24, narrow weights too (refused here for the workspace's alignment, after the sizes)."""
+    bad = ctypes.c_void_p(4096 + 64)
+    for rows, v, needle in (((1 << 31) - 1, 4, "256-byte"), ((1 << 31) - 1, 64, "256-byte"), ((1 << 31) - 1, 65, "too large"), (1 << 30, 128, "256-byte"),
+                            (1 << 13, 1 << 24, "256-byte"), ((1 << 13) + 1, 1 << 24, "too large"), (1 << 13, (1 << 24) + 1, "v must")):
+        _refused(_lib.load().yp_quantized_linear(0, rows, v, 8, 0, P, None, P, P, None, bad, P, 0, None), needle)
+
+
+_PLANS = r"""
+#include "gemm_launch.hpp"
+#include <cstdio>
+int main() {
+  long long bad = 0;
+  auto see = [&](const char* what, long long wgs, long long i, long long j, long long steps) {
+    if (wgs < YP_MAX_WORKGROUPS) return;
+    if (bad++ < 5) printf("%s %lld %lld %lld\n", what, i, j, steps);
+  };
+  for (long long steps : {1, 2, 5, 40, 1024})
+    for (long long v = 1; v <= (1 << 24); v += 1 + v / 40) {
+      const long long rows = (1ll << 37) / v < 2147483647ll ? (1ll << 37) / v : 2147483647ll, n = (1ll << 38) / v < (1 << 20) ? (1ll << 38) / v : (1 << 20);
+      for (long long j : {rows, rows - rows / 40, rows / 2}) see("quantized", yp_plan_workgroups(yp_plan_tiles(v, j, steps, YP_TILE_L)), v, j, steps);
+      for (long long j : {n, n - n / 40, n / 2}) if (j > 0) see("loss", yp_plan_workgroups(yp_plan_tiles(v, j, steps, YP_TILE_L)), v, j, steps);
+    }
+  for (long long d : {1, 64, 4096, 65536})
+    for (long long n = 1; n <= (1 << 20); n += 1 + n / 10)
+      for (long long piece : {1, 256, 4096, 1 << 17})
+        for (int largest : {YP_TILE_L, YP_TILE_M}) {
+          yp_tile_plan a = {}, b = {};
+          yp_plan_two(d, piece, (n + 31) / 32, d, n, (piece + 31) / 32, largest, &a, &b);
+          see("gradients", yp_plan_workgroups(a) + yp_plan_workgroups(b) + (piece + 31) / 32, d, n, piece);
+        }
+  return bad != 0;
+}
+"""
+
+
+def test_plans_fit_a_launch(tmp_path):
+    """Every size that the entries take gets a plan whose workgroups one launch can hold (host code only)."""
+    src, exe = tmp_path / "plans.hip", tmp_path / "plans"
+    src.write_text(_PLANS)
+    subprocess.check_call([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-host-only", "-O1", "-std=c++17", "-x", "hip",
+                           "-I" + os.path.join(ROOT, "yolact_amd", "csrc"), str(src), "-o", str(exe)])
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout

@@ -845,7 +845,7 @@ extern "C" int yp_quantized_linear(int32_t device_id, int32_t rows, int32_t v, i
   if (dtype != YP_INT8 && !head_type(dtype)) return fail(YP_EINVAL, "yp_quantized_linear: dtype must be YP_INT8, YP_F32, YP_BF16 or YP_F16");
   if (!head_type(out_dtype)) return fail(YP_EINVAL, "yp_quantized_linear: out_dtype must be YP_F32, YP_BF16 or YP_F16");
   if (v < 1 || v > (1 << 24)) return fail(YP_EINVAL, "yp_quantized_linear: v must be in [1, 2^24]");
-  if (((int64_t)rows + 127) / 128 * (((int64_t)v + 127) / 128) >= (1ll << 23)) return fail(YP_EINVAL, "yp_quantized_linear: rows * v is too large");
+  if ((int64_t)rows * v > (1ll << 37)) return fail(YP_EINVAL, "yp_quantized_linear: rows * v is too large (at most 2^37)");
   if (rows == 0) return YP_OK;
   if (!x || !wq || !w_scale || !out || (dtype == YP_INT8 ? !x_scale : !workspace)) return fail(YP_EINVAL, "yp_quantized_linear: null argument");
   if (((uintptr_t)wq & 15) != 0 || (dtype == YP_INT8 ? ((uintptr_t)x & 15) != 0 : !elem_aligned(x, dtype)) || !elem_aligned(out, out_dtype) ||

@@ -32,12 +32,14 @@ static inline double yp_plan_cost(int shape, double wgs, double steps) {
   if (shape == YP_TILE_M) return wgs <= 256 ? steps * 0.49 + 5 : wgs <= 512 ? steps * 0.79 + 6 : steps * 0.93 * ceil(wgs / 256) / 2 + 6 * ceil(wgs / 512);
   return wgs <= 256 ? steps * 0.28 + 3 : wgs <= 512 ? steps * 0.45 + 3 : wgs <= 1280 ? steps * 0.75 + 4 : steps * 0.92 * wgs / 1280 + 4 * ceil(wgs / 1280);
 }
-// `largest`: YP_TILE_M for f32 as it is, else YP_TILE_L
+#define YP_MAX_WORKGROUPS (1 << 24)   // of 256 threads: a launch's work items are counted in 32 bits
+// `largest`: YP_TILE_M for f32 as it is, else YP_TILE_L.  Smaller shapes only where their workgroups fit a launch.
 static inline yp_tile_plan yp_plan_tiles(int64_t I, int64_t J, int64_t steps, int largest) {
   yp_tile_plan best = {};
   double least = 1e30;
   for (int s = largest; s <= YP_TILE_T; ++s) {
     const yp_tile_plan p = yp_plan_shape(s, I, J);
+    if (s != largest && (int64_t)p.tiles_i * p.tiles_j >= YP_MAX_WORKGROUPS) continue;
     const double c = yp_plan_cost(s, (double)p.tiles_i * p.tiles_j, (double)steps);
     if (c < least) { least = c; best = p; }
   }
@@ -50,6 +52,7 @@ static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I
   for (int shape = largest; shape <= YP_TILE_T; ++shape) {
     yp_tile_plan a = yp_plan_shape(shape, I1, J1), b = yp_plan_shape(shape, I2, J2);
     const double ta = (double)a.tiles_i * a.tiles_j, tb = (double)b.tiles_i * b.tiles_j;
+    if (shape != largest && ta + tb >= YP_MAX_WORKGROUPS - (1 << 16)) continue;      // (room for what else the launch does)
     const double alone = shape == YP_TILE_L ? 1.57 : shape == YP_TILE_M ? 0.79 : 0.45;
     for (int64_t sa = 1; sa == 1 || (sa <= steps1 / 8 && ta * sa <= 1024); sa *= 2)
       for (int64_t sb = 1; sb == 1 || (sb <= steps2 / 8 && tb * sb <= 1024); sb *= 2) {
@@ -69,7 +72,6 @@ static inline void yp_plan_two(int64_t I1, int64_t J1, int64_t steps1, int64_t I
 }
 
 #ifdef __HIPCC__
-#define YP_MAX_WORKGROUPS (1 << 24)   // of 256 threads: a launch's work items are counted in 32 bits
 static inline yp_gemm yp_with_plan(yp_gemm g, const yp_tile_plan& p) { g.tiles_i = p.tiles_i; g.tiles_j = p.tiles_j; g.splits = p.splits; return g; }
 static inline int64_t yp_plan_workgroups(const yp_tile_plan& p) { return (int64_t)p.tiles_i * p.tiles_j * p.splits; }
 
