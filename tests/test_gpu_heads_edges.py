@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+import heads_precision as precision
 import heads_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -159,3 +160,48 @@ def test_quantized_linear_past_32_bits_of_results(rows, v):
         few = heads.quantized_linear(part, w, bias=b, out_dtype=torch.bfloat16)
         assert torch.equal(y[at:at + 100], few)
         ref.within(few, *ref.quantized_linear(*ref.quantize(part), w.q[:, :1].long(), w.scale, b, torch.bfloat16), "quantized_linear")
+
+
+@pytest.mark.parametrize("dt", TYPES[1:], ids=str)
+@pytest.mark.parametrize("n,v,d", [(200, 333, 64), (512, 4099, 130), (700, 300, 257), (100, 81, 256)])
+def test_precision_of_two_planes_of_dz(n, v, d, dt):
+    """Up to 512 rows, or 2^30 multiplications, the gradients of 16-bit calls are off by their own rounding and little more."""
+    from yolact_amd import heads
+    h, w, b, y, up = _inputs(n, v, d, dt, True)
+    up *= n
+    y[::5] = -1
+    _, lse = heads.class_loss(h, w, y, bias=b)
+    got = dict(zip(("grad_h", "grad_w"), heads.class_loss_backward(h, w, y, lse, up, bias=b)))
+    for name, (value, bound) in precision.two_planes(h, w, b, y, up).items():
+        ref.within(got[name], value, bound, name)
+        assert precision.relative(got[name], value) <= precision.ROUNDED * ref.HALF[dt], name
+
+
+@pytest.mark.parametrize("dt", TYPES[1:], ids=str)
+def test_precision_of_one_plane_of_dz(dt):
+    """Beyond that dz is rounded once, like the gradients."""
+    from yolact_amd import heads
+    h, w, b, y, up = _inputs(1300, 1290, 1290, dt, True)
+    up *= 1300
+    _, lse = heads.class_loss(h, w, y, bias=b)
+    got = heads.class_loss_backward(h, w, y, lse, up, bias=b)
+    dz, _, _ = precision.softmax_difference(h, w, b, y, up)
+    for have, value in zip(got, (dz @ w.double(), dz.t() @ h.double())):
+        assert precision.relative(have, value) <= precision.ROUNDED_TWICE * ref.HALF[dt]
+
+
+def test_precision_of_large_float32():
+    """2.16e9 multiplications: two f16 planes.  Losses: a logit's error (the terms of one have a root mean square of 1.5 over
+    sqrt d, so 1.5 in all), and four roundings to float32 of numbers between 8 and 16 - lse, its logarithm's two units,
+    the difference -, half a step of which is two of 2^-22, again a third of the square in the mean; a third more allowed."""
+    from yolact_amd import heads
+    n, v, d = 1300, 1290, 1290
+    h, w, b, y, up = _inputs(n, v, d, torch.float32, False)
+    losses, lse = heads.class_loss(h, w, y)
+    gh, gw, _ = heads.class_loss_backward(h, w, y, lse, up)
+    dz, z, _ = precision.softmax_difference(h, w, None, y, up)
+    assert precision.relative(gh, dz @ w.double()) <= precision.rms_of_planes(v)
+    assert precision.relative(gw, dz.t() @ h.double()) <= precision.rms_of_planes(n)
+    off = losses.double() - (torch.logsumexp(z, dim=1) - z.gather(1, y[:, None])[:, 0])
+    allowed = math.hypot(1.5 * precision.rms_of_planes(d), 4.0 / 3.0 * math.sqrt(4 * 4 / 3.0) * precision.STEP)
+    assert float(off.square().mean().sqrt()) <= allowed

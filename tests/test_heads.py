@@ -1,6 +1,7 @@
 """Prediction-head operators without a GPU: the 64-bit references themselves, sizes of workspaces, refusals at the C ABI
 and in Python."""
 import ctypes
+import math
 import os
 import re
 import subprocess
@@ -11,6 +12,7 @@ import torch
 
 from yolact_amd import _lib, heads
 
+import heads_precision as precision
 import heads_reference as ref
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -221,3 +223,26 @@ def test_plans_fit_a_launch(tmp_path):
                            "-I" + os.path.join(ROOT, "yolact_amd", "csrc"), str(src), "-o", str(exe)])
     run = subprocess.run([str(exe)], capture_output=True, text=True)
     assert run.returncode == 0, run.stdout
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=str)
+def test_precision_bounds_tell_one_plane_of_dz_from_two(dt):
+    """The gradients as the kernels compute them, in 64 bits but for dz's planes and the result's rounding: two planes are
+    within the bounds, one is not."""
+    g = torch.Generator().manual_seed(1)
+    n, v, d = 200, 333, 64
+    h = torch.randn(n, d, generator=g).to(dt)
+    w = (torch.randn(v, d, generator=g) * (1.5 / math.sqrt(d))).to(dt)
+    y = torch.randint(-1, v, (n,), generator=g)
+    up = torch.rand(n, generator=g)
+    dz, _, gg = precision.softmax_difference(h, w, None, y, up)
+    by = (2.0 ** 13 if dt == torch.float16 else 1.0) / gg.max()
+    want = precision.two_planes(h, w, None, y, up)
+    for planes in (1, 2):
+        first = (dz * by).to(dt).double()
+        q = (first + ((dz * by - first).to(dt).double() if planes == 2 else 0.0)) / by
+        for name, got in (("grad_h", (q @ w.double()).to(dt)), ("grad_w", (q.t() @ h.double()).to(dt))):
+            value, bound = want[name]
+            inside = bool(((got.double() - value).abs() <= bound).all())
+            near = precision.relative(got, value) <= precision.ROUNDED * ref.HALF[dt]
+            assert inside == near == (planes == 2), (planes, name)
