@@ -205,3 +205,25 @@ def test_precision_of_large_float32():
     off = losses.double() - (torch.logsumexp(z, dim=1) - z.gather(1, y[:, None])[:, 0])
     allowed = math.hypot(1.5 * precision.rms_of_planes(d), 4.0 / 3.0 * math.sqrt(4 * 4 / 3.0) * precision.STEP)
     assert float(off.square().mean().sqrt()) <= allowed
+
+
+def test_quantized_heads_of_a_convolution():
+    """A head whose last layer is a 3 x 3 convolution with all anchors of a place in its channels: on unfolded neighbourhoods."""
+    from yolact_amd import heads
+    B, ch, H, W, A, classes, k = 2, 24, 7, 9, 3, 5, 3
+    fmap = torch.randn(B, ch, H, W, generator=_gen(1), device="cuda")
+    kernels = [torch.randn(A * n, ch, k, k, generator=_gen(n), device="cuda") / math.sqrt(ch * k * k) for n in (classes, 4, 32)]
+    bias = torch.randn(A * classes, generator=_gen(9), device="cuda")
+    rows = torch.nn.functional.unfold(fmap, k, padding=1).transpose(1, 2).contiguous()
+    net = heads.QuantizedHeads((kernels[0].flatten(1), bias), kernels[1].flatten(1), kernels[2].flatten(1))(rows)
+    q, s = ref.quantize(rows.reshape(B * H * W, -1))
+    for (name, got), kernel, b in zip(net.items(), kernels, (bias, None, None)):
+        qw, sw = ref.quantize(kernel.flatten(1))
+        ref.within(got.reshape(B * H * W, -1), *ref.quantized_linear(q, s, qw, sw, b, torch.float32), name)
+        # and near the convolution itself: each of the products is off by half a step of either operand at most
+        conv = torch.nn.functional.conv2d(fmap.cpu().double(), kernel.cpu().double(), b.cpu().double() if b is not None else None, padding=1)
+        conv = conv.permute(0, 2, 3, 1).reshape(B * H * W, -1).cuda()
+        x, w = rows.reshape(B * H * W, -1).double().abs(), kernel.flatten(1).double().abs()
+        half_x, half_w = 0.5 * s.double()[:, None] + 0 * x, 0.5 * sw.double()[:, None] + 0 * w
+        ref.within(got.reshape(B * H * W, -1), conv, 1.0001 * (half_x @ (w + half_w).t() + x @ half_w.t()) + 1e-5, name)
+        assert got.reshape(B, H * W * A, -1).shape[2] == got.shape[2] // A

@@ -32,8 +32,10 @@
 #define YP_CL_THREADS 256
 // f32 products of as many multiplications go through f16 planes; below, the scales and copies cost more
 #define YP_CL_SPLIT_FROM (1ll << 31)
-// up to as many rows, or as many multiplications, dz has two planes: 12 instead of 8 N V D operations where reading w,
-// writing dw or the launches are what takes time
+// Up to as many rows, or as many multiplications, dz has two planes: 12 instead of 8 N V D operations where reading w,
+// writing dw or the launches are a good part of the time.  The backward pass in bf16, with two planes and with one: 19248 x 81 x
+// 256 46 and 42 us, 1024 x 1024 x 1024 38 and 30, 128 x 32000 x 2048 141 and 109, 512 x 32000 x 2048 380 and 228; past
+// the limits 2048 x 1024 x 1024 59 and 40, 1024 x 32000 x 2048 656 and 418.
 #define YP_CL_FINE_ROWS 512
 #define YP_CL_FINE_WORK (1ll << 30)
 #define YP_CL_PIECE_MAX (1 << 17)
@@ -743,7 +745,8 @@ static ClassLossPlan plan_class_loss(int64_t N, int64_t V, int64_t D, int type, 
   if (most > YP_CL_PIECE_BYTES / (p.kd * planes)) most = YP_CL_PIECE_BYTES / (p.kd * planes);
   cut_pieces(V, most, &p.pieces, &p.piece);
   p.kv = yp_pad_k(p.piece, b);
-  // (two planes of dz to write: M's epilogues hide better)
+  // (two planes of dz to write: M's epilogues hide better.  The backward pass, 2048 x 8192 x 1024: 347 us, with L 355;
+  // 4096 x 32000 x 1024: 2300 and 2323; the same where the plan takes M anyway)
   p.dzp = p.split ? yp_plan_shape(YP_TILE_M, p.piece, p.kn) : yp_plan_tiles(p.piece, p.kn, dsteps, largest);
   // the two gradient products share a launch and so a tile shape
   yp_plan_two(D, p.piece, p.kn / kr * p.segs, D, N, p.kv / YP_TILE_KB * p.segs, largest, &p.dwp, &p.dhp);

@@ -121,7 +121,10 @@ def _class_loss_backward(features, weight, labels, bias, ignore_index, p_lse, p_
 def class_loss_backward(features, weight, labels, lse, grad_losses, bias=None, ignore_index: int = -1):
     """Gradients of ``class_loss``'s losses: ``(grad_features, grad_weight, grad_bias or None)`` given ``lse`` as the forward
     returned it for the same inputs and ``grad_losses`` (float32, the shape of ``labels``).  The logits are computed again,
-    in pieces of the vocabulary; sums run in float32 in a fixed order, each gradient is rounded once."""
+    in pieces of the vocabulary; sums run in float32 in a fixed order.  16-bit gradients are rounded twice beyond 512 rows
+    and 2^30 multiplications: the logits' gradients to the type, relative to the largest of ``grad_losses``, and the results;
+    up to there the first is held twice as precise.  Large float32 calls: as ``class_loss``, the weight's gradient
+    to 2^-39 of the largest feature times its row's gradient, the features' to 2^-39 of the largest weight."""
     lead, dev = _class_loss_args(features, weight, labels, bias)[-2:]
     _check("lse", lse, (torch.float32,), lead, dev)
     p_grad = _check("grad_losses", grad_losses, (torch.float32,), lead, dev)
@@ -132,6 +135,7 @@ class ClassLoss(torch.autograd.Function):
     """Differentiable class loss: ``ClassLoss.apply(features, weight, bias, labels, ignore_index=-1, reduction="mean")``.
     ``reduction`` "none" gives the rows' losses, "sum" and "mean" one value, "mean" over the rows that are not ignored (0 if
     there are none).  Gradients flow to features, weight and bias (which may be None); those nobody needs are not computed.
+    The three are of one type, under autocast too: cast a master weight of another (``weight.to(features.dtype)``).
     When forward and backward are captured into a graph, capture both, on leaves whose eager graphs are gone."""
 
     @staticmethod
@@ -294,9 +298,12 @@ def quantized_linear(x, weight: QuantizedRows, bias=None, out_dtype=torch.float3
 
 
 class QuantizedHeads:
-    """The three products of the prediction head in 8 bits: class logits, box offsets and mask coefficients of every anchor's
-    features, in the shapes and the type ``Detect`` takes.  Each head is a float weight [out, D], or a pair of it and a
-    float32 bias [out] (layers/head.py's last layers, with an anchor's features as the row)."""
+    """Three products on the same rows of features in 8 bits: class logits, box offsets and mask coefficients, in the type
+    ``Detect`` takes.  Each head is a float weight [out, D], or a pair of it and a float32 bias [out].  With a row of features per
+    anchor the shapes are ``Detect``'s.  The reference's last layers (layers/head.py) are convolutions whose channels hold all
+    anchors of a place: there a row is a place's unfolded neighbourhood, D its k * k * channels values, a head's
+    weight the kernel as [anchors * values, D], and the results are reshaped from [B, places, anchors * values] to
+    [B, places * anchors, values]."""
 
     def __init__(self, cls, offset, mask_coef):
         def keep(h):
@@ -305,8 +312,8 @@ class QuantizedHeads:
         self.heads = {"pred_cls": keep(cls), "pred_offset": keep(offset), "pred_mask_coef": keep(mask_coef)}
 
     def __call__(self, features):
-        """features [B, A, D] -> {"pred_cls": [B, A, C], "pred_offset": [B, A, 4], "pred_mask_coef": [B, A, K]} float32, the
-        features quantized once.  The coefficients are what the product gives: the reference's tanh (layers/head.py:81) is
+        """features [..., D] -> {"pred_cls": [..., C], "pred_offset": [..., 4], "pred_mask_coef": [..., K]} float32 (as many
+        values as the heads' weights have rows), the features quantized once.  The coefficients are what the product gives: the reference's tanh (layers/head.py:81) is
         the caller's, who may want it in place."""
         x = quantize_rows(features)
         return {name: quantized_linear(x, w, bias=b) for name, (w, b) in self.heads.items()}
