@@ -163,8 +163,8 @@ hipError_t yp_launch_quantize_rows(int64_t rows, int k, int type, const void* x,
 // over rows of the weight, YP_OR_W at a time: a lane reads 16 bytes of k of each.  The matrix instruction takes lane l's 16
 // bytes as quarter l >> 4 of row and column l & 15, of the weight and of x alike: its diagonal holds the sums of four lanes'
 // products, which the wave adds up at the end.  YP_OR_C chunks of each are on their way at a time - 16 KB a wave -, the first ones while x is
-// quantized.  26.6 us for 32000 x 4096 (131 MB: 4.9 TB/s); from two rows on the matrix cores are faster (30 us, where this
-// took 43 for two and 100 for eight).
+// quantized.  26 us for 32000 x 4096 (131 MB: 5.0 TB/s); from two rows on the tile engine is faster (30 us; a kernel of this kind,
+// with dot products, took 43 for two rows and 100 for eight).
 #define YP_OR_W 4
 #define YP_OR_C 4
 #define YP_OR_LDS 61440
