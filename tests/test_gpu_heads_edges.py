@@ -227,3 +227,56 @@ def test_quantized_heads_of_a_convolution():
         half_x, half_w = 0.5 * s.double()[:, None] + 0 * x, 0.5 * sw.double()[:, None] + 0 * w
         ref.within(got.reshape(B * H * W, -1), conv, 1.0001 * (half_x @ (w + half_w).t() + x @ half_w.t()) + 1e-5, name)
         assert got.reshape(B, H * W * A, -1).shape[2] == got.shape[2] // A
+
+
+def test_large_float32_nothing_left():
+    """No row takes part, no class does, or all values are zeros: in the size that runs through planes."""
+    from yolact_amd import heads
+    h, w, b, y, up = _inputs(2048, 8192, 130, torch.float32, True)
+    none = torch.full_like(y, -1)
+    for reduction in ("mean", "sum", "none"):
+        leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+        loss = heads.ClassLoss.apply(*leaves, none, -1, reduction)
+        assert not loss.any() and not any(g.any() for g in torch.autograd.grad(loss.sum(), leaves))
+    off = torch.full_like(b, -math.inf)
+    losses, lse = heads.class_loss(h, w, y, bias=off)
+    assert bool((losses == math.inf).all()) and bool((lse == -math.inf).all())
+    assert not any(g.any() for g in heads.class_loss_backward(h, w, y, lse, up, bias=off))
+    _check_large_float32(0 * h, 0 * w, b, y, up)
+    _check_large_float32(0 * h, w, b, y, up)
+    _check_large_float32(h, 0 * w, b, y, 0 * up)
+
+
+def test_large_float32_gradients_that_nobody_needs_and_replays():
+    """Each gradient alone is the same as beside the others; a captured step with a gradient a row follows its inputs."""
+    from yolact_amd import heads
+    h, w, b, y, up = _inputs(1300, 3001, 600, torch.float32, True)
+    y[::4] = -1
+    _, lse = heads.class_loss(h, w, y, bias=b)
+    full = heads.class_loss_backward(h, w, y, lse, up, bias=b)
+    for i in range(3):
+        leaves = [t.clone().requires_grad_(k == i) for k, t in enumerate((h, w, b))]
+        got, = torch.autograd.grad(heads.ClassLoss.apply(*leaves, y, -1, "none"), [leaves[i]], up)
+        assert torch.equal(got, full[i])
+
+    def step():
+        losses, lse = heads.class_loss(h, w, y, bias=b)
+        return [losses, lse, *heads.class_loss_backward(h, w, y, lse, up, bias=b)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for r in range(3):
+        h.mul_(3.0)
+        w.mul_(0.2)
+        up.mul_(2.0 ** -20)
+        want = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(outs, want))
